@@ -297,6 +297,37 @@ int t2sp_relayout_plan(int nd, const int *extents, const int64_t *src_strides, c
 int t2sp_capsule_packed_f32(const float *P2, int64_t ldp, const float *W2, int64_t ldw, float *V, int64_t ldv,
                             int N, int NN, int CI, int CO, int CII, void *stream);
 
+/* ---- The products of a language model's layers: elements of 16 or 32 bits, sums in 32 bits. ----
+ * They have no counterpart in the reference, whose pipelines are single precision and of one size.
+ * `type` is the element type of the operands, `out_type` that of the result: the same type or
+ * T2SP_TYPE_F32.  Leading dimensions and strides are in elements and must not be negative. */
+#define T2SP_TYPE_F32 0
+#define T2SP_TYPE_F16 1
+#define T2SP_TYPE_BF16 2
+
+/* Products grouped by expert, with ragged group sizes.  The T rows of X are sorted by group; group e is
+ * the rows offsets[e] <= r < offsets[e+1] (E + 1 integers of `offset_bits` = 32 or 64 in device memory,
+ * so sizes that a router computes on the device need no copy to the host):
+ *   t2sp_gemm_grouped        Y[r,:] = X[r,:] * op(W[e]);  W[e] is K x N, or N x K with `opb`
+ *   t2sp_gemm_grouped_wgrad  dW[e]  = X_e^T * dY_e, K x N; zeros for an empty group
+ * The gradient of X is t2sp_gemm_grouped of dY with the other `opb`.  Rows of Y outside every group keep
+ * what they held, and rows of X and dY outside every group are never used.  Offsets must not decrease; they
+ * are clamped to 0 .. T, so that no value leads outside the buffers.  sw: elements between the matrices.
+ * Every result element is one sum in a fixed order, whatever the group sizes.
+ * Operands whose rows are not whole 16-byte chunks (pointer, leading dimension, extent) are first copied
+ * to padded rows in `workspace` (16-byte aligned; t2sp_gemm_grouped*_workspace_bytes, 0 when nothing needs
+ * a copy): with less room the call is refused with T2SP_ERR_SHAPE.  E * rows of a matrix is at most T2SP_MAX_EXTENT. */
+size_t t2sp_gemm_grouped_workspace_bytes(int type, int opb, const void *X, const void *W, int T, int E, int K, int N,
+                                         int64_t ldx, int64_t ldw, int64_t sw);
+int t2sp_gemm_grouped(int type, int out_type, int opb, const void *X, const void *W, const void *offsets,
+                      int offset_bits, void *Y, int T, int E, int K, int N, int64_t ldx, int64_t ldw, int64_t sw,
+                      int64_t ldy, void *workspace, size_t workspace_bytes, void *stream);
+size_t t2sp_gemm_grouped_wgrad_workspace_bytes(int type, const void *X, const void *dY, int T, int E, int K, int N,
+                                               int64_t ldx, int64_t ldy);
+int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, const void *dY, const void *offsets,
+                            int offset_bits, void *dW, int T, int E, int K, int N, int64_t ldx, int64_t ldy,
+                            int64_t ldw, int64_t sw, void *workspace, size_t workspace_bytes, void *stream);
+
 /* dst[sum_d c_d*dst_strides[d]] = src[sum_d c_d*src_strides[d]] for every coordinate c of the
  * box `extents` (nd <= T2SP_MAX_DIMS, dimension 0 fastest).  Device-side replacement of the
  * host serializer/deserializer loops the reference's generated interface runs around its

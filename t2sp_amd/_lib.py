@@ -117,3 +117,10 @@ def _declare(L):
     L.t2sp_last_kernel_ns.restype = ctypes.c_double
     L.t2sp_release.restype = None
     L.t2sp_device_count.restype = i32
+    for name, args in (("t2sp_gemm_grouped", [i32, i32, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i64, i64, i64, i64]),
+                       ("t2sp_gemm_grouped_wgrad", [i32, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i64, i64, i64, i64])):
+        getattr(L, name).argtypes = args + [vp, sz, vp]
+    L.t2sp_gemm_grouped_workspace_bytes.argtypes = [i32, i32, vp, vp, i32, i32, i32, i32, i64, i64, i64]
+    L.t2sp_gemm_grouped_workspace_bytes.restype = sz
+    L.t2sp_gemm_grouped_wgrad_workspace_bytes.argtypes = [i32, vp, vp, i32, i32, i32, i32, i64, i64]
+    L.t2sp_gemm_grouped_wgrad_workspace_bytes.restype = sz

@@ -1,0 +1,393 @@
+// grouped.hip — matrix products grouped by expert, with ragged group sizes.
+//
+//   forward   Y[r, :]  = X[r, :] * op(W[e])          for the rows offsets[e] <= r < offsets[e + 1] of group e
+//   wgrad     dW[e]    = X_e^T * dY_e                (the rows of group e; zeros for an empty group)
+//
+// op(W[e]) is K x N, stored so or (opb) as N x K; the gradient of the rows is the forward product of dY with the other
+// op.  The group sizes are on the device only, so the launch covers the largest number of row tiles they can make,
+//   sum_e ceil(m_e / BM) <= floor(T / BM) + min(E, T),
+// and every workgroup finds its group and tile by itself: the waves add up the tile counts of 64 groups at a time
+// (a scan over the lanes); workgroups beyond the actual number end at once.  The tiles are then dealt to the dies in
+// contiguous runs, since each die has an L2 of its own: neighbouring tiles read the same columns of one matrix.
+//
+// Offsets are clamped to 0 .. T and to be non-decreasing before use, so no value of theirs leads outside X or Y.
+#include "product_core.hpp"
+#include "product_host.hpp"
+
+namespace t2sp {
+
+struct GroupedArgs {
+    const char *X, *W;
+    char *Y;
+    const void *offsets;
+    int off64;                           // the offsets are 64-bit (else 32-bit) integers
+    int T, E, K, N;
+    int64_t ldx, ldw, sw, ldy;           // in elements; sw: between matrices
+    int col_tiles, xcds;
+    int vec_out;                         // rows of Y may be written 16 bytes at a time
+};
+
+__device__ __forceinline__ int group_edge(const GroupedArgs &g, int e) {
+    const int64_t v = g.off64 ? static_cast<const int64_t *>(g.offsets)[e] : (int64_t) static_cast<const int32_t *>(g.offsets)[e];
+    return (int)(v < 0 ? 0 : v > g.T ? g.T : v);
+}
+
+struct GroupTile {
+    int group, row0, rows, col_tile;     // rows: of the group from row0 on
+};
+
+// The output tile of workgroup `block`, false when there is none.  Every wave does the same work; the results are
+// uniform over the wave.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, GroupTile *out) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int e, int *start, int *rows) {
+        int a = 0, b = 0;
+        if (e < g.E) { a = group_edge(g, e); b = group_edge(g, e + 1); }
+        *start = a;
+        *rows = b > a ? b - a : 0;
+        return (*rows + BM - 1) / BM;
+    };
+    auto scan = [&](int v) {                         // inclusive prefix sum over the wave
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(v, d, 64);
+            if (lane >= d) v += o;
+        }
+        return v;
+    };
+    int start, rows, n = tiles_of(lane, &start, &rows), sum = scan(n);
+    int64_t total = __builtin_amdgcn_readlane(sum, 63);
+    for (int e0 = 64; e0 < g.E; e0 += 64) {
+        int s, r;
+        total += __builtin_amdgcn_readlane(scan(tiles_of(e0 + lane, &s, &r)), 63);
+    }
+    total *= g.col_tiles;
+    const int64_t run = (total + g.xcds - 1) / g.xcds;
+    const int64_t at = block / g.xcds, w = (block % g.xcds) * run + at;
+    if (at >= run || w >= total) return false;
+    int64_t before = 0;                              // tiles of the groups in front of this chunk of 64
+    for (int e0 = 0; e0 < g.E;) {
+        const int64_t end = (before + sum) * g.col_tiles;
+        const uint64_t past = __ballot(end > w);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            const int mine = __builtin_amdgcn_readlane(n, l);
+            const int64_t local = w - (before + __builtin_amdgcn_readlane(sum, l) - mine) * g.col_tiles;
+            constexpr int PANEL = 8;                 // row tiles that are walked together down the columns
+            const int64_t panel = local / ((int64_t)PANEL * g.col_tiles), rest = local % ((int64_t)PANEL * g.col_tiles);
+            const int high = mine - (int)panel * PANEL < PANEL ? mine - (int)panel * PANEL : PANEL;
+            const int m = (int)panel * PANEL + (int)(rest % high);
+            out->group = e0 + l;
+            out->col_tile = (int)(rest / high);
+            out->row0 = __builtin_amdgcn_readlane(start, l) + m * BM;
+            out->rows = __builtin_amdgcn_readlane(rows, l) - m * BM;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+        e0 += 64;
+        n = tiles_of(e0 + lane, &start, &rows);
+        sum = scan(n);
+    }
+    return false;
+}
+
+// A lane's 4 NT consecutive columns of one row, rounded to the output's type.
+template <class P, class O>
+__device__ __forceinline__ void store_row(char *row, int n, int n_end, const pv4f (&acc)[P::NT], bool vec) {
+    O *p = reinterpret_cast<O *>(row) + n;
+    typedef O chunk __attribute__((ext_vector_type(16 / sizeof(O))));
+    constexpr int CE = 16 / sizeof(O);
+    if (vec) {
+#pragma unroll
+        for (int c = 0; c < P::LANE_N / CE; c++) {
+            if (n + c * CE >= n_end) break;
+            chunk v;
+#pragma unroll
+            for (int i = 0; i < CE; i++) v[i] = (O)acc[(c * CE + i) / 4][(c * CE + i) % 4];
+            *reinterpret_cast<chunk *>(p + c * CE) = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P::LANE_N; i++)
+            if (n + i < n_end) p[i] = (O)acc[i / 4][i % 4];
+    }
+}
+
+template <class P>
+__device__ __forceinline__ void clear(pv4f (&acc)[P::MT][P::NT]) {
+#pragma unroll
+    for (int i = 0; i < P::MT; i++)
+#pragma unroll
+        for (int j = 0; j < P::NT; j++) acc[i][j] = pv4f{0.f, 0.f, 0.f, 0.f};
+}
+
+template <class P, class O>
+__global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    GroupTile t;
+    if (!find_tile<P::BM>(g, blockIdx.x, &t)) return;
+    const int n0 = t.col_tile * P::BN;
+    TileSource a, b;
+    a.p = g.X + t.row0 * g.ldx * P::SZ;
+    a.ld = (uint32_t)(g.ldx * P::SZ);
+    a.count = t.rows;
+    b.p = g.W + t.group * g.sw * P::SZ + (P::BS == KMAJOR ? n0 * g.ldw : (int64_t)n0) * P::SZ;
+    b.ld = (uint32_t)(g.ldw * P::SZ);
+    b.count = g.N - n0;
+    pv4f acc[P::MT][P::NT];
+    clear<P>(acc);
+    product_run<P>(a, b, g.K, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < P::MT; i++) {
+        const int m = (wave / P::WN) * P::TM + 16 * i + (lane & 15);
+        if (m < t.rows) store_row<P, O>(g.Y + (t.row0 + m) * g.ldy * sizeof(O), n, g.N, acc[i], g.vec_out);
+    }
+}
+
+// dW[e] tile: rows of the tile are K (contiguous in X), columns N (contiguous in dY), the reduction runs over the
+// rows of the group.  Here W is dY (ldw its row stride), Y is dW (ldy, sw its row and matrix strides).
+template <class P, class O>
+__global__ void __launch_bounds__(P::THREADS) grouped_wgrad_kernel(const GroupedArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int row_tiles = (g.K + P::BM - 1) / P::BM;
+    const unsigned total = gridDim.x, run = (total + g.xcds - 1) / g.xcds;
+    // contiguous runs of tiles per die; the last dies' runs are short when the dies do not divide the tiles
+    const unsigned whole = total / g.xcds, extra = total % g.xcds, die = blockIdx.x % g.xcds;
+    const unsigned w = run == whole ? die * run + blockIdx.x / g.xcds
+                                    : die * whole + (die < extra ? die : extra) + blockIdx.x / g.xcds;
+    const unsigned per_group = (unsigned)row_tiles * g.col_tiles;
+    const int e = w / per_group, local = w % per_group;
+    constexpr int PANEL = 8;
+    const int panel = local / (PANEL * g.col_tiles), rest = local % (PANEL * g.col_tiles);
+    const int high = row_tiles - panel * PANEL < PANEL ? row_tiles - panel * PANEL : PANEL;
+    const int k0 = (panel * PANEL + rest % high) * P::BM, n0 = rest / high * P::BN;
+    const int first = group_edge(g, e), last = group_edge(g, e + 1);
+    const int rows = last > first ? last - first : 0;
+    TileSource a, b;
+    a.p = g.X + (first * g.ldx + k0) * P::SZ;
+    a.ld = (uint32_t)(g.ldx * P::SZ);
+    a.count = g.K - k0;
+    b.p = g.W + (first * g.ldw + n0) * P::SZ;
+    b.ld = (uint32_t)(g.ldw * P::SZ);
+    b.count = g.N - n0;
+    pv4f acc[P::MT][P::NT];
+    clear<P>(acc);
+    if (rows) product_run<P>(a, b, rows, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < P::MT; i++) {
+        const int k = k0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
+        if (k < g.K) store_row<P, O>(g.Y + (e * g.sw + k * g.ldy) * (int64_t)sizeof(O), n, g.N, acc[i], g.vec_out);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ padded copies
+template <class T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T *src, T *dst, int64_t rows, int64_t cols, int64_t ld, int64_t batch_stride,
+                                                       int64_t chunks_per_row, int64_t chunks) {
+    constexpr int CE = 16 / sizeof(T);
+    typedef T chunk __attribute__((ext_vector_type(CE)));
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / chunks_per_row, c = (i % chunks_per_row) * CE;
+        const T *s = src + (row / rows) * batch_stride + (row % rows) * ld + c;
+        chunk v;
+#pragma unroll
+        for (int j = 0; j < CE; j++) v[j] = c + j < cols ? s[j] : (T)0;
+        *reinterpret_cast<chunk *>(dst + i * CE) = v;
+    }
+}
+
+int launch_pad_rows(const void *src, void *dst, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t batch_stride, int size,
+                    hipStream_t stream) {
+    const int64_t per_row = padded_cols(cols, size) * size / 16, chunks = batch * rows * per_row;
+    if (chunks == 0) return T2SP_OK;
+    const int64_t blocks = (chunks + 255) / 256 < 65536 ? (chunks + 255) / 256 : 65536;
+    if (size == 4)
+        hipLaunchKernelGGL(pad_rows_kernel<uint32_t>, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const uint32_t *>(src),
+                           static_cast<uint32_t *>(dst), rows, cols, ld, batch_stride, per_row, chunks);
+    else
+        hipLaunchKernelGGL(pad_rows_kernel<uint16_t>, dim3((unsigned)blocks), dim3(256), 0, stream, static_cast<const uint16_t *>(src),
+                           static_cast<uint16_t *>(dst), rows, cols, ld, batch_stride, per_row, chunks);
+    return launched();
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+// Tile shapes.  256 x 256 has the most arithmetic per byte from LDS and one workgroup per CU; 128 x 128 (two per CU)
+// and 64 x 128 (three per CU) fill the chip when there are few rows per group.
+template <class T, int AS, int BS> using Tile256 = ProductTile<T, 256, 256, 2, 4, AS, BS, 4>;
+template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, 2, AS, BS, 4>;
+template <class T, int BS> using Tile64 = ProductTile<T, 64, 128, 1, 4, KMAJOR, BS, 4>;
+
+// The number of row tiles of `bm` rows that T rows in at most E groups can make.
+static int64_t most_row_tiles(int T, int E, int bm) { return T / bm + (E < T ? E : T); }
+
+template <class P, class O>
+static int launch_forward(GroupedArgs g, hipStream_t stream) {
+    g.col_tiles = (g.N + P::BN - 1) / P::BN;
+    const int64_t blocks = (most_row_tiles(g.T, g.E, P::BM) * g.col_tiles + g.xcds - 1) / g.xcds * g.xcds;
+    if (blocks > 0x7fffffff / P::THREADS) return T2SP_ERR_SHAPE;
+    auto kern = grouped_kernel<P, O>;
+    if (allow_lds(kern, P::LDS)) return T2SP_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(P::THREADS), P::LDS, stream, g);
+    return launched();
+}
+
+template <class P, class O>
+static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
+    g.col_tiles = (g.N + P::BN - 1) / P::BN;
+    const int64_t blocks = (int64_t)g.E * ((g.K + P::BM - 1) / P::BM) * g.col_tiles;
+    if (blocks > 0x7fffffff / P::THREADS) return T2SP_ERR_SHAPE;
+    auto kern = grouped_wgrad_kernel<P, O>;
+    if (allow_lds(kern, P::LDS)) return T2SP_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(P::THREADS), P::LDS, stream, g);
+    return launched();
+}
+
+// Rounds of workgroups x time of one: the tile whose product ends first.  Groups are taken as equally large.
+static double rounds_cost(int64_t tiles, int per_cu, double tile_time) {
+    const int64_t slots = (int64_t)machine().cus * per_cu;
+    return (double)((tiles + slots - 1) / slots) * per_cu * tile_time;
+}
+
+template <class T, class O, int BS>
+static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
+    const int64_t groups = g.E < g.T ? g.E : g.T, per = (g.T + groups - 1) / groups;
+    auto tiles = [&](int bm, int bn) { return groups * ((per + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
+    const double c256 = rounds_cost(tiles(256, 256), 1, 1.0), c128 = rounds_cost(tiles(128, 128), 2, 0.31),
+                 c64 = rounds_cost(tiles(64, 128), 3, 0.2);
+    if (c256 <= c128 && c256 <= c64) return launch_forward<Tile256<T, KMAJOR, BS>, O>(g, stream);
+    if (c128 <= c64) return launch_forward<Tile128<T, KMAJOR, BS>, O>(g, stream);
+    return launch_forward<Tile64<T, BS>, O>(g, stream);
+}
+
+template <class T, class O>
+static int wgrad_tiles(const GroupedArgs &g, hipStream_t stream) {
+    auto tiles = [&](int b) { return (int64_t)g.E * ((g.K + b - 1) / b) * ((g.N + b - 1) / b); };
+    if (rounds_cost(tiles(256), 1, 1.0) <= rounds_cost(tiles(128), 2, 0.31)) return launch_wgrad<Tile256<T, KROWS, KROWS>, O>(g, stream);
+    return launch_wgrad<Tile128<T, KROWS, KROWS>, O>(g, stream);
+}
+
+template <class F>
+static int with_types(int type, int out_type, F f) {
+    if (type == T2SP_TYPE_F32) return f((float *)nullptr, (float *)nullptr);
+    if (type == T2SP_TYPE_F16) return out_type == type ? f((_Float16 *)nullptr, (_Float16 *)nullptr) : f((_Float16 *)nullptr, (float *)nullptr);
+    return out_type == type ? f((__bf16 *)nullptr, (__bf16 *)nullptr) : f((__bf16 *)nullptr, (float *)nullptr);
+}
+
+static bool writable_in_chunks(const void *p, int64_t ld, int64_t cols, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0;
+}
+
+}  // namespace t2sp
+
+using namespace t2sp;
+
+extern "C" size_t t2sp_gemm_grouped_workspace_bytes(int type, int opb, const void *X, const void *W, int T, int E, int K, int N,
+                                                    int64_t ldx, int64_t ldw, int64_t sw) {
+    const int size = type_bytes(type);
+    if (!size || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) || !extent_ok(K) || !extent_ok(N) || !stride_ok(ldx) || !stride_ok(ldw) ||
+        !stride_ok(sw) || (int64_t)E * (opb ? N : K) > T2SP_MAX_EXTENT)
+        return 0;
+    const int64_t wr = opb ? N : K, wc = opb ? K : N;
+    size_t n = 0;
+    if (!loadable(X, ldx, K, size)) n += round_up((size_t)T * padded_cols(K, size) * size, 16);
+    if (!loadable(W, ldw, wc, size) || sw * size % 16) n += (size_t)E * wr * padded_cols(wc, size) * size;
+    return n;
+}
+
+extern "C" int t2sp_gemm_grouped(int type, int out_type, int opb, const void *X, const void *W, const void *offsets, int offset_bits,
+                                 void *Y, int T, int E, int K, int N, int64_t ldx, int64_t ldw, int64_t sw, int64_t ldy,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
+    const int size = type_bytes(type);
+    const int64_t wr = opb ? N : K, wc = opb ? K : N;
+    if (!size || !out_type_ok(type, out_type) || (offset_bits != 32 && offset_bits != 64) || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) ||
+        !extent_ok(K) || !extent_ok(N) || !stride_ok(ldx) || !stride_ok(ldw) || !stride_ok(sw) || !stride_ok(ldy) || ldx < K || ldw < wc ||
+        ldy < N || (int64_t)E * wr > T2SP_MAX_EXTENT)
+        return T2SP_ERR_SHAPE;
+    if (T == 0) return T2SP_OK;
+    if (!X || !W || !offsets || !Y) return T2SP_ERR_SHAPE;
+    const size_t need = t2sp_gemm_grouped_workspace_bytes(type, opb, X, W, T, E, K, N, ldx, ldw, sw);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return T2SP_ERR_SHAPE;
+    const hipStream_t st = (hipStream_t)stream;
+    char *room = static_cast<char *>(workspace);
+    if (!loadable(X, ldx, K, size)) {
+        const int64_t pc = padded_cols(K, size);
+        if (int err = launch_pad_rows(X, room, 1, T, K, ldx, 0, size, st)) return err;
+        X = room;
+        ldx = pc;
+        room += round_up((size_t)T * pc * size, 16);
+    }
+    if (!loadable(W, ldw, wc, size) || sw * size % 16) {
+        const int64_t pc = padded_cols(wc, size);
+        if (int err = launch_pad_rows(W, room, E, wr, wc, ldw, sw, size, st)) return err;
+        W = room;
+        ldw = pc;
+        sw = wr * pc;
+    }
+    // (a copy's padding is zeros, so the reduction may run over it; columns of Y stop at N)
+    GroupedArgs g{};
+    g.X = static_cast<const char *>(X); g.W = static_cast<const char *>(W); g.Y = static_cast<char *>(Y);
+    g.offsets = offsets; g.off64 = offset_bits == 64;
+    g.T = T; g.E = E; g.K = K; g.N = N;
+    g.ldx = ldx; g.ldw = ldw; g.sw = sw; g.ldy = ldy;
+    g.xcds = machine().xcds;
+    g.vec_out = writable_in_chunks(Y, ldy, N, out_type == T2SP_TYPE_F32 ? 4 : 2);
+    return with_types(type, out_type, [&](auto *t, auto *o) {
+        using TT = std::remove_pointer_t<decltype(t)>;
+        using OO = std::remove_pointer_t<decltype(o)>;
+        return opb ? forward_tiles<TT, OO, KMAJOR>(g, st) : forward_tiles<TT, OO, KROWS>(g, st);
+    });
+}
+
+extern "C" size_t t2sp_gemm_grouped_wgrad_workspace_bytes(int type, const void *X, const void *dY, int T, int E, int K, int N, int64_t ldx,
+                                                          int64_t ldy) {
+    const int size = type_bytes(type);
+    if (!size || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) || !extent_ok(K) || !extent_ok(N) || !stride_ok(ldx) || !stride_ok(ldy)) return 0;
+    size_t n = 0;
+    if (!loadable(X, ldx, K, size)) n += round_up((size_t)T * padded_cols(K, size) * size, 16);
+    if (!loadable(dY, ldy, N, size)) n += (size_t)T * padded_cols(N, size) * size;
+    return n;
+}
+
+extern "C" int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, const void *dY, const void *offsets, int offset_bits, void *dW,
+                                       int T, int E, int K, int N, int64_t ldx, int64_t ldy, int64_t ldw, int64_t sw, void *workspace,
+                                       size_t workspace_bytes, void *stream) {
+    const int size = type_bytes(type);
+    if (!size || !out_type_ok(type, out_type) || (offset_bits != 32 && offset_bits != 64) || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) ||
+        !extent_ok(K) || !extent_ok(N) || !stride_ok(ldx) || !stride_ok(ldy) || !stride_ok(ldw) || !stride_ok(sw) || ldx < K || ldy < N || ldw < N ||
+        (E > 1 && sw < (K - 1) * ldw + N))
+        return T2SP_ERR_SHAPE;
+    if (!offsets || !dW || (T && (!X || !dY))) return T2SP_ERR_SHAPE;
+    const size_t need = t2sp_gemm_grouped_wgrad_workspace_bytes(type, X, dY, T, E, K, N, ldx, ldy);
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return T2SP_ERR_SHAPE;
+    const hipStream_t st = (hipStream_t)stream;
+    char *room = static_cast<char *>(workspace);
+    if (!loadable(X, ldx, K, size) && T) {
+        const int64_t pc = padded_cols(K, size);
+        if (int err = launch_pad_rows(X, room, 1, T, K, ldx, 0, size, st)) return err;
+        X = room;
+        ldx = pc;
+        room += round_up((size_t)T * pc * size, 16);
+    }
+    if (!loadable(dY, ldy, N, size) && T) {
+        const int64_t pc = padded_cols(N, size);
+        if (int err = launch_pad_rows(dY, room, 1, T, N, ldy, 0, size, st)) return err;
+        dY = room;
+        ldy = pc;
+    }
+    GroupedArgs g{};
+    g.X = static_cast<const char *>(X); g.W = static_cast<const char *>(dY); g.Y = static_cast<char *>(dW);
+    g.offsets = offsets; g.off64 = offset_bits == 64;
+    g.T = T; g.E = E; g.K = K; g.N = N;
+    g.ldx = ldx; g.ldw = ldy; g.sw = sw; g.ldy = ldw;
+    g.xcds = machine().xcds;
+    const int os = out_type == T2SP_TYPE_F32 ? 4 : 2;
+    g.vec_out = writable_in_chunks(dW, ldw, N, os) && sw * os % 16 == 0;
+    return with_types(type, out_type, [&](auto *t, auto *o) {
+        return wgrad_tiles<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, st);
+    });
+}

@@ -1,0 +1,39 @@
+// product_host.hpp — what the launchers of the 16/32-bit product operators (grouped.hip, xent.hip, gemv_w4.hip) share:
+// element types, checks of arguments, and the padded copies of operands that the 16-byte loaders cannot take.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "machine.hpp"
+#include "t2sp_hip.h"
+
+namespace t2sp {
+
+inline int type_bytes(int type) {
+    return type == T2SP_TYPE_F32 ? 4 : type == T2SP_TYPE_F16 || type == T2SP_TYPE_BF16 ? 2 : 0;
+}
+inline bool out_type_ok(int type, int out_type) { return out_type == type || out_type == T2SP_TYPE_F32; }
+inline bool extent_ok(int64_t e) { return e >= 1 && e <= T2SP_MAX_EXTENT; }
+inline bool stride_ok(int64_t s) { return s >= 0 && stride_in_range(s); }
+
+// Rows of a matrix the loaders of product_core.hpp can read where they lie: 16-byte chunks along the contiguous
+// dimension, lane offsets of up to 255 rows inside 31 bits.
+inline bool loadable(const void *p, int64_t ld, int64_t cols, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0 && ld * size <= (1 << 23);
+}
+// Elements per row of a padded copy.
+inline int64_t padded_cols(int64_t cols, int size) { return (cols * size + 15) / 16 * 16 / size; }
+inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
+
+// dst[b][r][0 .. padded) = src[b][r][0 .. cols), zeros behind: dense rows of whole 16-byte chunks.
+int launch_pad_rows(const void *src, void *dst, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t batch_stride,
+                    int size, hipStream_t stream);
+
+template <class K> int allow_lds(K kern, int bytes) {
+    if (bytes <= 64 * 1024) return T2SP_OK;
+    return hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? T2SP_OK
+                                                                                                               : T2SP_ERR_LAUNCH;
+}
+inline int launched() { return hipGetLastError() == hipSuccess ? T2SP_OK : T2SP_ERR_LAUNCH; }
+
+}  // namespace t2sp

@@ -1,0 +1,158 @@
+"""Python mirror of the products of a language model's layers (include/t2sp_hip.h, second half): products
+grouped by expert, cross entropy over a vocabulary, products with 4-bit weights.
+
+torch CUDA tensors go to the thin layer: kernels are enqueued on the current stream of the tensors' device and
+the call returns without waiting, so it can be captured into a HIP graph; workspaces and fresh results come from
+torch's allocator, which keeps them apart between streams and captured graphs.  Element types are float32, float16
+and bfloat16.  numpy arrays (float32 or float16, host memory) go through the operator entries
+(include/gemm_grouped-interface.h, xent-interface.h, gemv_w4-interface.h), which stage them through the device.
+Misuse raises T2spError with the Halide error code that the entry would return."""
+import ctypes
+
+import numpy as np
+
+from ._lib import lib
+from .buffer import HalideBuffer
+from .ops import T2spError, _check, _is_torch, host_empty
+
+BAD_TYPE, SHAPE, BAD_DIMENSIONS, OUT_OF_BOUNDS, NULL_BUFFER = -3, -8, -43, -4, -12
+_codes = None
+
+
+def _type_codes():
+    global _codes
+    if _codes is None:
+        import torch
+        _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    return _codes
+
+
+def _need(op, ok, code=SHAPE):
+    if not ok:
+        raise T2spError(op, code)
+
+
+def _tensors(op, dims, *tensors):
+    """Common checks of floating-point CUDA tensors: one element type, one device, the stated ranks, unit stride along
+    the last axis.  Returns the T2SP_TYPE_* code."""
+    first = tensors[0]
+    code = _type_codes().get(first.dtype)
+    _need(op, code is not None, BAD_TYPE)
+    for t, d in zip(tensors, dims):
+        _need(op, t.dtype == first.dtype, BAD_TYPE)
+        _need(op, t.dim() == d, BAD_DIMENSIONS)
+        _need(op, t.is_cuda and t.device == first.device)
+        _need(op, t.shape[-1] <= 1 or t.stride(-1) == 1)
+    return code
+
+
+def _integers(op, t, like, n):
+    """Bits of a contiguous vector of n integers on the device of `like`."""
+    import torch
+    _need(op, t.dtype in (torch.int32, torch.int64), BAD_TYPE)
+    _need(op, t.dim() == 1, BAD_DIMENSIONS)
+    _need(op, t.device == like.device and t.shape[0] == n and (n <= 1 or t.stride(0) == 1))
+    return 32 if t.dtype == torch.int32 else 64
+
+
+def _result(op, out, shape, like, dtype, types):
+    import torch
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _need(op, out.dtype in types, BAD_TYPE)
+    _need(op, out.dim() == len(shape), BAD_DIMENSIONS)
+    _need(op, tuple(out.shape) == tuple(shape) and out.device == like.device and (shape[-1] <= 1 or out.stride(-1) == 1))
+    return out
+
+
+def _row(t):
+    """Elements between rows (a single row's stride carries no information)."""
+    return t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), t.shape[-1])
+
+
+def _matrix(t):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * _row(t))
+
+
+class _On:
+    """Makes the tensors' device current around a call."""
+
+    def __init__(self, t):
+        import torch
+        self.index = t.device.index
+        self.back = torch.cuda.current_device()
+        self.set = torch.cuda.set_device
+
+    def __enter__(self):
+        if self.index != self.back:
+            self.set(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.back:
+            self.set(self.back)
+
+
+def _stream(t):
+    import torch
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _room(nbytes, like):
+    """(pointer, bytes, owner) of a workspace.  The owner may be dropped after the call: torch's allocator hands the memory
+    out again only to work that is ordered behind it."""
+    if not nbytes:
+        return None, 0, None
+    import torch
+    t = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return t.data_ptr(), nbytes, t
+
+
+def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
+    """Y[r] = X[r] @ op(W[e]) for the rows offsets[e] <= r < offsets[e + 1] of group e.
+
+    X: (T, K) rows sorted by group; W: (E, K, N), or (E, N, K) when opb; offsets: E + 1 int32 or int64 on the device,
+    not decreasing (they are clamped to 0 .. T).  Y: (T, N) of X's type, or float32 (out_dtype, or the type of `out`).
+    Rows outside every group are left as they were (in a fresh result: whatever its memory held).  The gradient of X is
+    gemm_grouped(dY, W, offsets, opb=1 - opb)."""
+    op = "gemm_grouped"
+    if not _is_torch(X):
+        return _host_grouped(op, X, W, offsets, opb, out)
+    import torch
+    code = _tensors(op, (2, 3), X, W)
+    T, K = X.shape
+    E, N = W.shape[0], W.shape[1] if opb else W.shape[2]
+    _need(op, (W.shape[2] if opb else W.shape[1]) == K and E >= 1 and K >= 1 and N >= 1)
+    bits = _integers(op, offsets, X, E + 1)
+    Y = _result(op, out, (T, N), X, out_dtype or X.dtype, (X.dtype, torch.float32))
+    _need(op, Y.dtype in (X.dtype, torch.float32), BAD_TYPE)
+    L = lib()
+    x, w, ldx, ldw, sw = X.data_ptr(), W.data_ptr(), _row(X), _row(W), _matrix(W)
+    with _On(X):
+        ws, nbytes, owner = _room(L.t2sp_gemm_grouped_workspace_bytes(code, opb, x, w, T, E, K, N, ldx, ldw, sw), X)
+        _check(op, L.t2sp_gemm_grouped(code, _type_codes()[Y.dtype], opb, x, w, offsets.data_ptr(), bits, Y.data_ptr(), T, E, K, N,
+                                       ldx, ldw, sw, _row(Y), ws, nbytes, _stream(X)))
+    return Y
+
+
+def gemm_grouped_wgrad(X, dY, offsets, out=None, out_dtype=None):
+    """dW[e] = X_e.T @ dY_e over the rows offsets[e] <= r < offsets[e + 1] of each group, zeros for an empty one.
+
+    X: (T, K), dY: (T, N), offsets as in gemm_grouped.  dW: (E, K, N) of X's type, or float32."""
+    op = "gemm_grouped_wgrad"
+    if not _is_torch(X):
+        return _host_wgrad(op, X, dY, offsets, out)
+    import torch
+    code = _tensors(op, (2, 2), X, dY)
+    T, K = X.shape
+    N, E = dY.shape[1], offsets.shape[0] - 1
+    _need(op, dY.shape[0] == T and E >= 1 and K >= 1 and N >= 1)
+    bits = _integers(op, offsets, X, E + 1)
+    dW = _result(op, out, (E, K, N), X, out_dtype or X.dtype, (X.dtype, torch.float32))
+    _need(op, dW.dtype in (X.dtype, torch.float32), BAD_TYPE)
+    L = lib()
+    x, dy, ldx, ldy = X.data_ptr(), dY.data_ptr(), _row(X), _row(dY)
+    with _On(X):
+        ws, nbytes, owner = _room(L.t2sp_gemm_grouped_wgrad_workspace_bytes(code, x, dy, T, E, K, N, ldx, ldy), X)
+        _check(op, L.t2sp_gemm_grouped_wgrad(code, _type_codes()[dW.dtype], x, dy, offsets.data_ptr(), bits, dW.data_ptr(), T, E, K,
+                                             N, ldx, ldy, _row(dW), _matrix(dW), ws, nbytes, _stream(X)))
+    return dW
