@@ -304,6 +304,8 @@ int t2sp_capsule_packed_f32(const float *P2, int64_t ldp, const float *W2, int64
 #define T2SP_TYPE_F32 0
 #define T2SP_TYPE_F16 1
 #define T2SP_TYPE_BF16 2
+/* Longest row (extent along which the elements of an operand are contiguous) of these products. */
+#define T2SP_MAX_ROW_BYTES (1 << 23)
 
 /* Products grouped by expert, with ragged group sizes.  The T rows of X are sorted by group; group e is
  * the rows offsets[e] <= r < offsets[e+1] (E + 1 integers of `offset_bits` = 32 or 64 in device memory,
@@ -327,6 +329,26 @@ size_t t2sp_gemm_grouped_wgrad_workspace_bytes(int type, const void *X, const vo
 int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, const void *dY, const void *offsets,
                             int offset_bits, void *dW, int T, int E, int K, int N, int64_t ldx, int64_t ldy,
                             int64_t ldw, int64_t sw, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Cross entropy of a softmax over a vocabulary, from hidden states H (T x D) and the output matrix W
+ * (V x D), without keeping the T x V logits z = H W^T:
+ *   t2sp_xent       loss[t] = lse[t] - z[t, label[t]],  lse[t] = log sum_v exp z[t, v] (lse may be NULL)
+ *   t2sp_xent_grad  with g[t, v] = (exp(z[t, v] - lse[t]) - [v == label[t]]) * dloss[t]:
+ *                   dH = g W (T x D),  dW = g^T H (V x D); either may be NULL
+ * `labels` are integers of `label_bits` = 32 or 64.  A token whose label is outside 0 .. V - 1 (padding, a
+ * prompt) has loss 0, a row of zeros in dH and no part in dW, whatever its rows of H and dloss hold.
+ * loss, lse and dloss are float, one per token; a mean's gradient is dloss = 1 / number of tokens.
+ * The gradient works through the vocabulary in pieces: p - [label] of one piece, rounded to `type`, passes
+ * through the workspace (16-byte aligned, t2sp_xent*_workspace_bytes, required), as do padded copies of
+ * operands whose rows are not whole 16-byte chunks.  Sums are in float and in a fixed order. */
+size_t t2sp_xent_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw);
+int t2sp_xent(int type, const void *H, const void *W, const void *labels, int label_bits, float *loss, float *lse,
+              int T, int V, int D, int64_t ldh, int64_t ldw, void *workspace, size_t workspace_bytes, void *stream);
+size_t t2sp_xent_grad_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh,
+                                      int64_t ldw);
+int t2sp_xent_grad(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits,
+                   const float *lse, const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh,
+                   int64_t ldw, int64_t lddh, int64_t lddw, void *workspace, size_t workspace_bytes, void *stream);
 
 /* dst[sum_d c_d*dst_strides[d]] = src[sum_d c_d*src_strides[d]] for every coordinate c of the
  * box `extents` (nd <= T2SP_MAX_DIMS, dimension 0 fastest).  Device-side replacement of the

@@ -124,3 +124,8 @@ def _declare(L):
     L.t2sp_gemm_grouped_workspace_bytes.restype = sz
     L.t2sp_gemm_grouped_wgrad_workspace_bytes.argtypes = [i32, vp, vp, i32, i32, i32, i32, i64, i64]
     L.t2sp_gemm_grouped_wgrad_workspace_bytes.restype = sz
+    for name in ("t2sp_xent_workspace_bytes", "t2sp_xent_grad_workspace_bytes"):
+        getattr(L, name).argtypes = [i32, vp, vp, i32, i32, i32, i64, i64]
+        getattr(L, name).restype = sz
+    L.t2sp_xent.argtypes = [i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, i64, i64, vp, sz, vp]
+    L.t2sp_xent_grad.argtypes = [i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, vp, sz, vp]

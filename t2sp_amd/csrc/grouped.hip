@@ -74,12 +74,9 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
             const int l = __ffsll((unsigned long long)past) - 1;
             const int mine = __builtin_amdgcn_readlane(n, l);
             const int64_t local = w - (before + __builtin_amdgcn_readlane(sum, l) - mine) * g.col_tiles;
-            constexpr int PANEL = 8;                 // row tiles that are walked together down the columns
-            const int64_t panel = local / ((int64_t)PANEL * g.col_tiles), rest = local % ((int64_t)PANEL * g.col_tiles);
-            const int high = mine - (int)panel * PANEL < PANEL ? mine - (int)panel * PANEL : PANEL;
-            const int m = (int)panel * PANEL + (int)(rest % high);
+            int m;
+            panel_tile(local, mine, g.col_tiles, &m, &out->col_tile);
             out->group = e0 + l;
-            out->col_tile = (int)(rest / high);
             out->row0 = __builtin_amdgcn_readlane(start, l) + m * BM;
             out->rows = __builtin_amdgcn_readlane(rows, l) - m * BM;
             return true;
@@ -90,36 +87,6 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
         sum = scan(n);
     }
     return false;
-}
-
-// A lane's 4 NT consecutive columns of one row, rounded to the output's type.
-template <class P, class O>
-__device__ __forceinline__ void store_row(char *row, int n, int n_end, const pv4f (&acc)[P::NT], bool vec) {
-    O *p = reinterpret_cast<O *>(row) + n;
-    typedef O chunk __attribute__((ext_vector_type(16 / sizeof(O))));
-    constexpr int CE = 16 / sizeof(O);
-    if (vec) {
-#pragma unroll
-        for (int c = 0; c < P::LANE_N / CE; c++) {
-            if (n + c * CE >= n_end) break;
-            chunk v;
-#pragma unroll
-            for (int i = 0; i < CE; i++) v[i] = (O)acc[(c * CE + i) / 4][(c * CE + i) % 4];
-            *reinterpret_cast<chunk *>(p + c * CE) = v;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < P::LANE_N; i++)
-            if (n + i < n_end) p[i] = (O)acc[i / 4][i % 4];
-    }
-}
-
-template <class P>
-__device__ __forceinline__ void clear(pv4f (&acc)[P::MT][P::NT]) {
-#pragma unroll
-    for (int i = 0; i < P::MT; i++)
-#pragma unroll
-        for (int j = 0; j < P::NT; j++) acc[i][j] = pv4f{0.f, 0.f, 0.f, 0.f};
 }
 
 template <class P, class O>
@@ -153,17 +120,12 @@ template <class P, class O>
 __global__ void __launch_bounds__(P::THREADS) grouped_wgrad_kernel(const GroupedArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int row_tiles = (g.K + P::BM - 1) / P::BM;
-    const unsigned total = gridDim.x, run = (total + g.xcds - 1) / g.xcds;
-    // contiguous runs of tiles per die; the last dies' runs are short when the dies do not divide the tiles
-    const unsigned whole = total / g.xcds, extra = total % g.xcds, die = blockIdx.x % g.xcds;
-    const unsigned w = run == whole ? die * run + blockIdx.x / g.xcds
-                                    : die * whole + (die < extra ? die : extra) + blockIdx.x / g.xcds;
-    const unsigned per_group = (unsigned)row_tiles * g.col_tiles;
-    const int e = w / per_group, local = w % per_group;
-    constexpr int PANEL = 8;
-    const int panel = local / (PANEL * g.col_tiles), rest = local % (PANEL * g.col_tiles);
-    const int high = row_tiles - panel * PANEL < PANEL ? row_tiles - panel * PANEL : PANEL;
-    const int k0 = (panel * PANEL + rest % high) * P::BM, n0 = rest / high * P::BN;
+    const unsigned w = die_run(blockIdx.x, gridDim.x, g.xcds), per_group = (unsigned)row_tiles * g.col_tiles;
+    const int e = w / per_group;
+    int k0, n0;
+    panel_tile(w % per_group, row_tiles, g.col_tiles, &k0, &n0);
+    k0 *= P::BM;
+    n0 *= P::BN;
     const int first = group_edge(g, e), last = group_edge(g, e + 1);
     const int rows = last > first ? last - first : 0;
     TileSource a, b;
@@ -216,12 +178,6 @@ int launch_pad_rows(const void *src, void *dst, int64_t batch, int64_t rows, int
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-// Tile shapes.  256 x 256 has the most arithmetic per byte from LDS and one workgroup per CU; 128 x 128 (two per CU)
-// and 64 x 128 (three per CU) fill the chip when there are few rows per group.
-template <class T, int AS, int BS> using Tile256 = ProductTile<T, 256, 256, 2, 4, AS, BS, 4>;
-template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, 2, AS, BS, 4>;
-template <class T, int BS> using Tile64 = ProductTile<T, 64, 128, 1, 4, KMAJOR, BS, 4>;
-
 // The number of row tiles of `bm` rows that T rows in at most E groups can make.
 static int64_t most_row_tiles(int T, int E, int bm) { return T / bm + (E < T ? E : T); }
 
@@ -247,12 +203,6 @@ static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
     return launched();
 }
 
-// Rounds of workgroups x time of one: the tile whose product ends first.  Groups are taken as equally large.
-static double rounds_cost(int64_t tiles, int per_cu, double tile_time) {
-    const int64_t slots = (int64_t)machine().cus * per_cu;
-    return (double)((tiles + slots - 1) / slots) * per_cu * tile_time;
-}
-
 template <class T, class O, int BS>
 static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
     const int64_t groups = g.E < g.T ? g.E : g.T, per = (g.T + groups - 1) / groups;
@@ -269,17 +219,6 @@ static int wgrad_tiles(const GroupedArgs &g, hipStream_t stream) {
     auto tiles = [&](int b) { return (int64_t)g.E * ((g.K + b - 1) / b) * ((g.N + b - 1) / b); };
     if (rounds_cost(tiles(256), 1, 1.0) <= rounds_cost(tiles(128), 2, 0.31)) return launch_wgrad<Tile256<T, KROWS, KROWS>, O>(g, stream);
     return launch_wgrad<Tile128<T, KROWS, KROWS>, O>(g, stream);
-}
-
-template <class F>
-static int with_types(int type, int out_type, F f) {
-    if (type == T2SP_TYPE_F32) return f((float *)nullptr, (float *)nullptr);
-    if (type == T2SP_TYPE_F16) return out_type == type ? f((_Float16 *)nullptr, (_Float16 *)nullptr) : f((_Float16 *)nullptr, (float *)nullptr);
-    return out_type == type ? f((__bf16 *)nullptr, (__bf16 *)nullptr) : f((__bf16 *)nullptr, (float *)nullptr);
-}
-
-static bool writable_in_chunks(const void *p, int64_t ld, int64_t cols, int size) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0;
 }
 
 }  // namespace t2sp
@@ -305,7 +244,7 @@ extern "C" int t2sp_gemm_grouped(int type, int out_type, int opb, const void *X,
     const int size = type_bytes(type);
     const int64_t wr = opb ? N : K, wc = opb ? K : N;
     if (!size || !out_type_ok(type, out_type) || (offset_bits != 32 && offset_bits != 64) || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) ||
-        !extent_ok(K) || !extent_ok(N) || !stride_ok(ldx) || !stride_ok(ldw) || !stride_ok(sw) || !stride_ok(ldy) || ldx < K || ldw < wc ||
+        !row_ok(K, size) || !extent_ok(N) || !row_ok(wc, size) || !stride_ok(ldx) || !stride_ok(ldw) || !stride_ok(sw) || !stride_ok(ldy) || ldx < K || ldw < wc ||
         ldy < N || (int64_t)E * wr > T2SP_MAX_EXTENT)
         return T2SP_ERR_SHAPE;
     if (T == 0) return T2SP_OK;
@@ -358,7 +297,7 @@ extern "C" int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, co
                                        size_t workspace_bytes, void *stream) {
     const int size = type_bytes(type);
     if (!size || !out_type_ok(type, out_type) || (offset_bits != 32 && offset_bits != 64) || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) ||
-        !extent_ok(K) || !extent_ok(N) || !stride_ok(ldx) || !stride_ok(ldy) || !stride_ok(ldw) || !stride_ok(sw) || ldx < K || ldy < N || ldw < N ||
+        !row_ok(K, size) || !row_ok(N, size) || !stride_ok(ldx) || !stride_ok(ldy) || !stride_ok(ldw) || !stride_ok(sw) || ldx < K || ldy < N || ldw < N ||
         (E > 1 && sw < (K - 1) * ldw + N))
         return T2SP_ERR_SHAPE;
     if (!offsets || !dW || (T && (!X || !dY))) return T2SP_ERR_SHAPE;

@@ -280,4 +280,58 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
     __builtin_amdgcn_s_barrier();
 }
 
+// The position that workgroup `block` of `total` takes when every die works on a contiguous run of positions (workgroup
+// ids are dealt to the dies in turn): neighbouring tiles share operands, and each die has an L2 of its own.
+__device__ __forceinline__ unsigned die_run(unsigned block, unsigned total, unsigned dies) {
+    const unsigned whole = total / dies, extra = total % dies, die = block % dies;
+    return die * whole + (die < extra ? die : extra) + block / dies;
+}
+
+// Tile `at` of a row_tiles x col_tiles grid, walked in panels of eight rows of tiles, down the rows first: a die's 32
+// tiles in flight are then 8 x 4, which read the least (12 panels of operands) among the shapes that cover 32.
+__device__ __forceinline__ void panel_tile(int64_t at, int row_tiles, int col_tiles, int *row, int *col) {
+    constexpr int PANEL = 8;
+    const int panel = (int)(at / ((int64_t)PANEL * col_tiles)), rest = (int)(at % ((int64_t)PANEL * col_tiles));
+    const int high = row_tiles - panel * PANEL < PANEL ? row_tiles - panel * PANEL : PANEL;
+    *row = panel * PANEL + rest % high;
+    *col = rest / high;
+}
+
+// A lane's 4 NT consecutive columns of one row, rounded to the output's type.
+template <class P, class O>
+__device__ __forceinline__ void store_row(char *row, int n, int n_end, const pv4f (&acc)[P::NT], bool vec) {
+    O *p = reinterpret_cast<O *>(row) + n;
+    typedef O chunk __attribute__((ext_vector_type(16 / sizeof(O))));
+    constexpr int CE = 16 / sizeof(O);
+    if (vec) {
+#pragma unroll
+        for (int c = 0; c < P::LANE_N / CE; c++) {
+            if (n + c * CE >= n_end) break;
+            chunk v;
+#pragma unroll
+            for (int i = 0; i < CE; i++) v[i] = (O)acc[(c * CE + i) / 4][(c * CE + i) % 4];
+            *reinterpret_cast<chunk *>(p + c * CE) = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P::LANE_N; i++)
+            if (n + i < n_end) p[i] = (O)acc[i / 4][i % 4];
+    }
+}
+
+template <class P>
+__device__ __forceinline__ void clear(pv4f (&acc)[P::MT][P::NT]) {
+#pragma unroll
+    for (int i = 0; i < P::MT; i++)
+#pragma unroll
+        for (int j = 0; j < P::NT; j++) acc[i][j] = pv4f{0.f, 0.f, 0.f, 0.f};
+}
+
+
+// Tile shapes.  256 x 256 has the most arithmetic per byte from LDS and one workgroup per CU; 128 x 128 (two per CU)
+// and 64 x 128 (three per CU) fill the chip when there are few rows per group.
+template <class T, int AS, int BS> using Tile256 = ProductTile<T, 256, 256, 2, 4, AS, BS, 4>;
+template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, 2, AS, BS, 4>;
+template <class T, int BS> using Tile64 = ProductTile<T, 64, 128, 1, 4, KMAJOR, BS, 4>;
+
 }  // namespace t2sp

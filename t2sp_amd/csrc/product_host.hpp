@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "machine.hpp"
 #include "t2sp_hip.h"
 
@@ -19,8 +21,10 @@ inline bool stride_ok(int64_t s) { return s >= 0 && stride_in_range(s); }
 // Rows of a matrix the loaders of product_core.hpp can read where they lie: 16-byte chunks along the contiguous
 // dimension, lane offsets of up to 255 rows inside 31 bits.
 inline bool loadable(const void *p, int64_t ld, int64_t cols, int size) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0 && ld * size <= (1 << 23);
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0 && ld * size <= T2SP_MAX_ROW_BYTES;
 }
+// Extents along which elements are contiguous: a (padded) row within the loaders' reach.
+inline bool row_ok(int64_t e, int size) { return e >= 1 && e * size <= T2SP_MAX_ROW_BYTES; }
 // Elements per row of a padded copy.
 inline int64_t padded_cols(int64_t cols, int size) { return (cols * size + 15) / 16 * 16 / size; }
 inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
@@ -34,6 +38,24 @@ template <class K> int allow_lds(K kern, int bytes) {
     return hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? T2SP_OK
                                                                                                                : T2SP_ERR_LAUNCH;
 }
+inline bool writable_in_chunks(const void *p, int64_t ld, int64_t cols, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0;
+}
+
+// Rounds of workgroups x time of one: the tile whose product ends first.  Groups are taken as equally large.
+inline double rounds_cost(int64_t tiles, int per_cu, double tile_time) {
+    const int64_t slots = (int64_t)machine().cus * per_cu;
+    return (double)((tiles + slots - 1) / slots) * per_cu * tile_time;
+}
+
+// f(element type, result type) as null pointers, for a pair that out_type_ok accepts.
+template <class F>
+int with_types(int type, int out_type, F f) {
+    if (type == T2SP_TYPE_F32) return f((float *)nullptr, (float *)nullptr);
+    if (type == T2SP_TYPE_F16) return out_type == type ? f((_Float16 *)nullptr, (_Float16 *)nullptr) : f((_Float16 *)nullptr, (float *)nullptr);
+    return out_type == type ? f((__bf16 *)nullptr, (__bf16 *)nullptr) : f((__bf16 *)nullptr, (float *)nullptr);
+}
+
 inline int launched() { return hipGetLastError() == hipSuccess ? T2SP_OK : T2SP_ERR_LAUNCH; }
 
 }  // namespace t2sp

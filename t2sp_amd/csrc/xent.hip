@@ -1,0 +1,580 @@
+// xent.hip — cross entropy of a softmax over a vocabulary, from hidden states, without keeping the logits.
+//
+//   z[t, v] = sum_d H[t, d] W[v, d]                         (T tokens, V words, D wide)
+//   lse[t]  = log sum_v exp z[t, v],    loss[t] = lse[t] - z[t, label[t]]
+//   g[t, v] = (exp(z[t, v] - lse[t]) - [v == label[t]]) * dloss[t]
+//   dH = g W,   dW = g^T H
+// A token whose label is outside 0 .. V - 1 has loss zero, no gradient and no part in dW.
+//
+// Forward: a 256 x 256 tile of z stays in the accumulators; its rows' maxima and sums of exponentials (both float) go
+// to the workspace, 8 bytes per row and tile instead of 1024, and a second kernel joins them.
+//
+// Backward, for one piece of the vocabulary after the other: the tile of z is computed again, its epilogue writes
+// p - [label] rounded to the operands' type (the one rounding besides the results': it enters two matrix products on
+// the 16-bit matrix cores, and its relative error of at most half a step averages out over V or T terms); then the
+// piece's rows of dW (complete) and its part of dH (added up in float) are two more products.  8 T D V operations in
+// all, of which 2 T D V pay for not holding T x V logits.
+//
+// Scales.  dloss is kept out of the rounded matrix: dH's rows are multiplied by it at the end, and for dW it goes into
+// the rows of H, as dloss[t] / max |dloss| (exactly 1 in the usual case of equal weights: then the copy of H is exact).
+// half has no room below 2^-24 for the probabilities of a large vocabulary: p - [label] is stored times 2^15 there
+// (at most 32768 in magnitude) and the products are scaled back in float.
+// The copy of H also holds zeros for tokens without a label: what their rows hold (padding may be anything) reaches
+// no sum.
+#include "product_core.hpp"
+#include "product_host.hpp"
+
+namespace t2sp {
+
+struct XentArgs {
+    const char *H, *W;
+    const void *labels;
+    int lab64;
+    int T, V, D;
+    int64_t ldh, ldw;                    // elements
+    int row_tiles, col_tiles, xcds;
+    float2 *part;                        // [col_tiles][T]: maximum of z over the tile's columns, sum of exp(z - maximum)
+    float *hit;                          // [T]: z at the label
+    // backward
+    const float *lse, *dloss;
+    char *G;                             // [T][ldg] p - [label] of the piece, zeros from vp to ldg
+    int64_t ldg;
+    int v0, vp;                          // the piece: words v0 .. v0 + vp - 1
+};
+
+__device__ __forceinline__ int64_t label_of(const void *labels, int lab64, int t) {
+    return lab64 ? static_cast<const int64_t *>(labels)[t] : (int64_t) static_cast<const int32_t *>(labels)[t];
+}
+
+constexpr float LOG2E = 1.44269504088896340736f;
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+
+// The tile of logits of rows m0.., words v0 + n0..
+template <class P>
+__device__ __forceinline__ void logits_tile(const XentArgs &g, int m0, int n0, char *smem, pv4f (&acc)[P::MT][P::NT]) {
+    TileSource a, b;
+    a.p = g.H + m0 * g.ldh * P::SZ;
+    a.ld = (uint32_t)(g.ldh * P::SZ);
+    a.count = g.T - m0;
+    b.p = g.W + (g.v0 + n0) * g.ldw * P::SZ;
+    b.ld = (uint32_t)(g.ldw * P::SZ);
+    b.count = g.vp - n0;
+    clear<P>(acc);
+    product_run<P>(a, b, g.D, smem, acc);
+}
+
+template <class P>
+__global__ void __launch_bounds__(P::THREADS) xent_stats_kernel(const XentArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int m0, n0;
+    panel_tile(die_run(blockIdx.x, gridDim.x, g.xcds), g.row_tiles, g.col_tiles, &m0, &n0);
+    const int tile = n0;
+    m0 *= P::BM;
+    n0 *= P::BN;
+    pv4f acc[P::MT][P::NT];
+    logits_tile<P>(g, m0, n0, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int first_m = (wave / P::WN) * P::TM, n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    float2 *joint = reinterpret_cast<float2 *>(smem);        // [WN][BM]; the product is done with its LDS
+#pragma unroll
+    for (int i = 0; i < P::MT; i++) {
+        const int m = first_m + 16 * i + (lane & 15);
+        const bool row = m0 + m < g.T;
+        const int64_t hot = row ? label_of(g.labels, g.lab64, m0 + m) : -1;
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int c = 0; c < P::LANE_N; c++) {
+            const float z = acc[i][c / 4][c % 4];
+            if (n + c < g.V) top = fmaxf(top, z);
+            if (n + c == hot && n + c < g.V) g.hit[m0 + m] = z;
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float base = top == -__builtin_inff() ? 0.f : top;         // (no word of the tile, or all at -inf)
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < P::LANE_N; c++)
+            if (n + c < g.V) sum += exp_of(acc[i][c / 4][c % 4] - base);
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lane < 16) joint[(wave % P::WN) * P::BM + m] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int m = threadIdx.x; m < P::BM && m0 + m < g.T; m += P::THREADS) {
+        float2 v[P::WN];
+        float top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < P::WN; w++) {
+            v[w] = joint[w * P::BM + m];
+            top = fmaxf(top, v[w].x);
+        }
+        const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < P::WN; w++) sum += v[w].y * exp_of((v[w].x == -__builtin_inff() ? base : v[w].x) - base);
+        g.part[(int64_t)tile * g.T + m0 + m] = make_float2(top, sum);
+    }
+}
+
+// Joins the tiles' maxima and sums: 64 rows per workgroup, 16 waves that take every sixteenth tile.
+constexpr int JOIN_WAVES = 16;
+__global__ void __launch_bounds__(64 * JOIN_WAVES) xent_join_kernel(const float2 *part, const float *hit, const void *labels, int lab64, int T,
+                                                                    int V, int tiles, float *loss, float *lse) {
+    __shared__ float2 joint[JOIN_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x * 64 + lane;
+    float top = -__builtin_inff(), sum = 0.f;
+    auto add = [&](float m, float s) {
+        const float to = fmaxf(top, m), base = to == -__builtin_inff() ? 0.f : to;
+        sum = sum * exp_of((top == -__builtin_inff() ? base : top) - base) + s * exp_of((m == -__builtin_inff() ? base : m) - base);
+        top = to;
+    };
+    if (t < T) {
+#pragma unroll 8
+        for (int c = wave; c < tiles; c += JOIN_WAVES) {
+            const float2 v = part[(int64_t)c * T + t];
+            add(v.x, v.y);
+        }
+    }
+    joint[wave][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (wave == 0 && t < T) {
+#pragma unroll
+        for (int w = 1; w < JOIN_WAVES; w++) add(joint[w][lane].x, joint[w][lane].y);
+        const float l = top + logf(sum);
+        const int64_t label = label_of(labels, lab64, t);
+        const bool valid = label >= 0 && label < V;
+        if (lse) lse[t] = l;
+        loss[t] = valid ? l - hit[t] : 0.f;
+    }
+}
+
+// max |dloss| over the tokens with a label.
+__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *dloss, const void *labels, int lab64, int T, int V, float *scale) {
+    __shared__ float joint[16];
+    float top = 0.f;
+    bool bad = false;
+    for (int t = threadIdx.x; t < T; t += 1024) {
+        const int64_t label = label_of(labels, lab64, t);
+        if (label >= 0 && label < V) {
+            const float v = fabsf(dloss[t]);
+            bad |= !(v < __builtin_inff());
+            top = fmaxf(top, v);
+        }
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    if (__ballot(bad)) top = __builtin_nanf("");
+    if ((threadIdx.x & 63) == 0) joint[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float all = 0.f;
+        for (int w = 0; w < 16; w++) all = joint[w] != joint[w] || all != all ? __builtin_nanf("") : fmaxf(all, joint[w]);
+        *scale = all;
+    }
+}
+
+// Hz[t, :] = H[t, :] * (dloss[t] / max |dloss|) rounded to the type, zeros for tokens without a label and from D to ld.
+template <class T>
+__global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int64_t ldh, bool vec, const void *labels, int lab64, const float *dloss,
+                                                                 const float *scale, int rows, int V, int D, T *Hz, int64_t ld, int64_t chunks) {
+    constexpr int CE = 16 / sizeof(T);
+    typedef T chunk __attribute__((ext_vector_type(CE)));
+    const int64_t per = ld / CE;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int t = (int)(i / per), c = (int)(i % per) * CE;
+        const int64_t label = label_of(labels, lab64, t);
+        chunk v;
+        if (label >= 0 && label < V) {
+            const float by = *scale == 0.f ? 0.f : dloss[t] / *scale;
+            const T *s = H + t * ldh + c;
+            if (vec) v = *reinterpret_cast<const chunk *>(s);
+#pragma unroll
+            for (int j = 0; j < CE; j++) v[j] = (T)((float)(vec ? v[j] : c + j < D ? s[j] : (T)0) * by);
+        } else {
+#pragma unroll
+            for (int j = 0; j < CE; j++) v[j] = (T)0.f;
+        }
+        *reinterpret_cast<chunk *>(Hz + i * CE) = v;
+    }
+}
+
+template <class T> struct GradientScale { static constexpr float value = 1.f; };
+template <> struct GradientScale<_Float16> { static constexpr float value = 32768.f; };
+
+template <class P>
+__global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const XentArgs g) {
+    using T = typename P::T;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int m0, n0;
+    panel_tile(die_run(blockIdx.x, gridDim.x, g.xcds), g.row_tiles, g.col_tiles, &m0, &n0);
+    m0 *= P::BM;
+    n0 *= P::BN;
+    pv4f acc[P::MT][P::NT];
+    logits_tile<P>(g, m0, n0, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < P::MT; i++) {
+        const int t = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
+        if (t >= g.T) continue;
+        const int64_t label = label_of(g.labels, g.lab64, t);
+        const bool valid = label >= 0 && label < g.V;
+        const float lse = g.lse[t];
+        const int64_t hot = label - g.v0;
+#pragma unroll
+        for (int c = 0; c < P::LANE_N; c++) {
+            const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (n + c == hot ? 1.f : 0.f);
+            acc[i][c / 4][c % 4] = valid && n + c < g.vp ? p * GradientScale<T>::value : 0.f;
+        }
+        store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n, (int)g.ldg, acc[i], true);
+    }
+}
+
+struct XentProductArgs {
+    const char *A, *B;
+    char *out;
+    int64_t lda, ldb, ldo;               // elements
+    int rows, cols, k;                   // of the result; the reduction
+    int a_cols, b_cols;                  // elements in a row of A (dW) and B, whole 16-byte chunks
+    int row_tiles, col_tiles, xcds;
+    const float *scale;                  // dW: max |dloss|
+    float by;
+    int vec_out;
+    int splits;                          // dH: the reduction in this many parts, each with a plane of floats
+    int64_t plane;
+    int add;                             // dH: add to the planes (a later piece of the vocabulary)
+};
+
+// dW[v0 + m, n] = scale * sum_t G[t, m] Hz[t, n]
+template <class P, class O>
+__global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int m0, n0;
+    panel_tile(die_run(blockIdx.x, gridDim.x, g.xcds), g.row_tiles, g.col_tiles, &m0, &n0);
+    m0 *= P::BM;
+    n0 *= P::BN;
+    const TileSource a{g.A + m0 * P::SZ, (uint32_t)(g.lda * P::SZ), g.a_cols - m0}, b{g.B + n0 * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
+    pv4f acc[P::MT][P::NT];
+    clear<P>(acc);
+    product_run<P>(a, b, g.k, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const float by = *g.scale * g.by;
+#pragma unroll
+    for (int i = 0; i < P::MT; i++) {
+        const int m = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
+        if (m >= g.rows) continue;
+#pragma unroll
+        for (int j = 0; j < P::NT; j++) acc[i][j] *= by;
+        store_row<P, O>(g.out + m * g.ldo * (int64_t)sizeof(O), n, g.cols, acc[i], g.vec_out);
+    }
+}
+
+// plane[s][t, n] (+)= sum over part s of the piece's words: G[t, v] W[v0 + v, n]
+template <class P>
+__global__ void __launch_bounds__(P::THREADS) xent_dh_kernel(const XentProductArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const unsigned at = die_run(blockIdx.x, gridDim.x, g.xcds), tiles = (unsigned)g.row_tiles * g.col_tiles, s = at / tiles;
+    int m0, n0;
+    panel_tile(at % tiles, g.row_tiles, g.col_tiles, &m0, &n0);
+    m0 *= P::BM;
+    n0 *= P::BN;
+    const int stages = (g.k + P::KS - 1) / P::KS, per = (stages + g.splits - 1) / g.splits * P::KS;
+    const int k0 = (int64_t)s * per < g.k ? (int)s * per : g.k, k = g.k - k0 < per ? g.k - k0 : per;
+    const TileSource a{g.A + (m0 * g.lda + k0) * P::SZ, (uint32_t)(g.lda * P::SZ), g.rows - m0},
+        b{g.B + (k0 * g.ldb + n0) * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
+    pv4f acc[P::MT][P::NT];
+    clear<P>(acc);
+    if (k > 0) product_run<P>(a, b, k, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < P::MT; i++) {
+        const int m = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
+        if (m >= g.rows) continue;
+        float *row = reinterpret_cast<float *>(g.out) + s * g.plane + m * g.ldo + n;
+#pragma unroll
+        for (int j = 0; j < P::NT; j++) {
+            if (n + 4 * j >= g.ldo) break;               // (planes have rows of whole 16-byte chunks)
+            pv4f *p = reinterpret_cast<pv4f *>(row + 4 * j);
+            *p = g.add ? *p + acc[i][j] : acc[i][j];
+        }
+    }
+}
+
+// dH[t, n] = dloss[t] * by * sum_s plane[s][t, n], zeros for tokens without a label.
+template <class O>
+__global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, int splits, int64_t plane, int64_t ld, const void *labels, int lab64,
+                                                           const float *dloss, float by, int V, int D, O *dH, int64_t ldo, bool vec, int64_t chunks) {
+    const int64_t per = ld / 4;
+    typedef O chunk __attribute__((ext_vector_type(4)));
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int t = (int)(i / per), n = (int)(i % per) * 4;
+        const int64_t label = label_of(labels, lab64, t);
+        pv4f sum = pv4f{0.f, 0.f, 0.f, 0.f};
+        if (label >= 0 && label < V) {
+#pragma unroll 4
+            for (int s = 0; s < splits; s++) sum += *reinterpret_cast<const pv4f *>(planes + s * plane + t * ld + n);
+            sum *= dloss[t] * by;
+        }
+        O *o = dH + t * ldo + n;
+        if (vec) {
+            *reinterpret_cast<chunk *>(o) = __builtin_convertvector(sum, chunk);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (n + j < D) o[j] = (O)sum[j];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+// What a call passes through its workspace, in this order (every part starts on 256 bytes).
+struct XentRoom {
+    size_t h, w;                         // padded copies of H and W (0: read where they lie)
+    size_t part, hit;                    // forward
+    size_t scale, hz, g, planes;         // backward
+    size_t total;
+    int64_t ldd;                         // elements per row of hz and of the planes
+    int piece, splits;
+};
+
+constexpr size_t ROOM_ALIGN = 256;
+constexpr int64_t G_BYTES = 128 << 20;   // of the piece of p - [label]: it then stays in the 256 MB cache between its
+                                         // kernel and the two products that read it ...
+constexpr int MIN_PIECE = 4096;          // ... but a piece is long enough that adding up dH costs little beside it
+
+static int pick_tile(int64_t rows, int64_t cols) {
+    auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * ((cols + bn - 1) / bn); };
+    const double c256 = rounds_cost(tiles(256, 256), 1, 1.0), c128 = rounds_cost(tiles(128, 128), 2, 0.31), c64 = rounds_cost(tiles(64, 128), 3, 0.2);
+    return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+}
+
+// The tile of dH (the rows of T decide: its columns and the split fill the chip) and the parts of its reduction.
+static int dh_tile(int T) { return T > 128 ? 256 : T > 64 ? 128 : 64; }
+static int dh_splits(int T, int D, int piece) {
+    if (T == 0) return 1;
+    const int bm = dh_tile(T), bn = bm == 256 ? 256 : 128, per_cu = bm == 256 ? 1 : bm == 128 ? 2 : 3;
+    const int64_t tiles = (int64_t)((T + bm - 1) / bm) * ((D + bn - 1) / bn), slots = (int64_t)machine().cus * per_cu;
+    int64_t s = slots / tiles;
+    if (s > piece / 512) s = piece / 512;
+    return s < 1 ? 1 : (int)s;
+}
+
+static XentRoom xent_room(bool backward, int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
+    const int size = type_bytes(type);
+    XentRoom r{};
+    r.ldd = padded_cols(D, size);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += round_up(bytes, ROOM_ALIGN);
+        return here;
+    };
+    r.h = loadable(H, ldh, D, size) ? (size_t)-1 : take((size_t)T * r.ldd * size);
+    r.w = loadable(W, ldw, D, size) ? (size_t)-1 : take((size_t)V * r.ldd * size);
+    if (!backward) {
+        const int t = pick_tile(T, V);
+        r.part = take((size_t)((V + (t == 256 ? 255 : 127)) / (t == 256 ? 256 : 128)) * T * sizeof(float2));
+        r.hit = take((size_t)T * sizeof(float));
+    } else {
+        int64_t piece = G_BYTES / ((int64_t)(T > 0 ? T : 1) * size) / 256 * 256;
+        if (piece < MIN_PIECE) piece = MIN_PIECE;
+        if (piece >= V) piece = V;
+        else piece = round_up((V + (V + piece - 1) / piece - 1) / ((V + piece - 1) / piece), 256);     // equal pieces
+        r.piece = (int)piece;
+        r.splits = dh_splits(T, D, r.piece);
+        r.scale = take(sizeof(float));
+        r.hz = take((size_t)T * r.ldd * size);
+        r.g = take((size_t)T * padded_cols(piece, size) * size);
+        r.planes = take((size_t)r.splits * T * r.ldd * sizeof(float));
+    }
+    r.total = at;
+    return r;
+}
+
+static bool xent_args_ok(int type, int T, int V, int D, int64_t ldh, int64_t ldw) {
+    const int size = type_bytes(type);
+    return size && T >= 0 && T <= T2SP_MAX_EXTENT && extent_ok(V) && row_ok(D, size) && stride_ok(ldh) && stride_ok(ldw) && ldh >= D && ldw >= D;
+}
+
+// Padded copies of the operands that need one; sets the pointers and leading dimensions of g.
+static int xent_operands(XentArgs &g, const XentRoom &r, int size, char *room, const void *H, const void *W, int64_t ldh, int64_t ldw,
+                         hipStream_t st) {
+    g.H = static_cast<const char *>(H); g.W = static_cast<const char *>(W);
+    g.ldh = ldh; g.ldw = ldw;
+    if (r.h != (size_t)-1) {
+        if (int err = launch_pad_rows(H, room + r.h, 1, g.T, g.D, ldh, 0, size, st)) return err;
+        g.H = room + r.h; g.ldh = r.ldd;
+    }
+    if (r.w != (size_t)-1) {
+        if (int err = launch_pad_rows(W, room + r.w, 1, g.V, g.D, ldw, 0, size, st)) return err;
+        g.W = room + r.w; g.ldw = r.ldd;
+    }
+    return T2SP_OK;
+}
+
+#define T2SP_LAUNCH_TILES(P, kern, blocks, st, g)                                              \
+    do {                                                                                       \
+        const int64_t b_ = (blocks);                                                           \
+        if (b_ > 0x7fffffff / P::THREADS) return T2SP_ERR_SHAPE;                               \
+        auto k_ = kern;                                                                        \
+        if (allow_lds(k_, P::LDS)) return T2SP_ERR_LAUNCH;                                     \
+        hipLaunchKernelGGL(k_, dim3((unsigned)b_), dim3(P::THREADS), P::LDS, st, g);           \
+        return launched();                                                                     \
+    } while (0)
+
+template <class P> static int launch_stats(XentArgs g, hipStream_t st) {
+    g.row_tiles = (g.T + P::BM - 1) / P::BM;
+    g.col_tiles = (g.V + P::BN - 1) / P::BN;
+    T2SP_LAUNCH_TILES(P, xent_stats_kernel<P>, (int64_t)g.row_tiles * g.col_tiles, st, g);
+}
+template <class P> static int launch_probabilities(XentArgs g, hipStream_t st) {
+    g.row_tiles = (g.T + P::BM - 1) / P::BM;
+    g.col_tiles = (g.vp + P::BN - 1) / P::BN;
+    T2SP_LAUNCH_TILES(P, xent_probabilities_kernel<P>, (int64_t)g.row_tiles * g.col_tiles, st, g);
+}
+template <class P, class O> static int launch_dw(XentProductArgs g, hipStream_t st) {
+    g.row_tiles = (g.rows + P::BM - 1) / P::BM;
+    g.col_tiles = (g.cols + P::BN - 1) / P::BN;
+    T2SP_LAUNCH_TILES(P, (xent_dw_kernel<P, O>), (int64_t)g.row_tiles * g.col_tiles, st, g);
+}
+template <class P> static int launch_dh(XentProductArgs g, hipStream_t st) {
+    g.row_tiles = (g.rows + P::BM - 1) / P::BM;
+    g.col_tiles = (g.cols + P::BN - 1) / P::BN;
+    T2SP_LAUNCH_TILES(P, xent_dh_kernel<P>, (int64_t)g.row_tiles * g.col_tiles * g.splits, st, g);
+}
+#undef T2SP_LAUNCH_TILES
+
+template <class T>
+static int xent_forward(XentArgs g, float *loss, float *lse, hipStream_t st) {
+    const int tile = pick_tile(g.T, g.V);
+    int err = tile == 256 ? launch_stats<Tile256<T, KMAJOR, KMAJOR>>(g, st)
+                          : tile == 128 ? launch_stats<Tile128<T, KMAJOR, KMAJOR>>(g, st) : launch_stats<Tile64<T, KMAJOR>>(g, st);
+    if (err) return err;
+    const int tiles = tile == 256 ? (g.V + 255) / 256 : (g.V + 127) / 128;
+    hipLaunchKernelGGL(xent_join_kernel, dim3((g.T + 63) / 64), dim3(64 * JOIN_WAVES), 0, st, g.part, g.hit, g.labels, g.lab64, g.T, g.V, tiles,
+                       loss, lse);
+    return launched();
+}
+
+template <class T, class O>
+static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *H, int64_t ldh, void *dH, void *dW, int64_t lddh, int64_t lddw,
+                         hipStream_t st) {
+    constexpr int size = sizeof(T);
+    const float by = 1.f / GradientScale<T>::value;
+    float *scale = reinterpret_cast<float *>(room + r.scale), *planes = reinterpret_cast<float *>(room + r.planes);
+    int err;
+    if (dW) {
+        hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, g.dloss, g.labels, g.lab64, g.T, g.V, scale);
+        if ((err = launched())) return err;
+        const int64_t chunks = (int64_t)g.T * r.ldd * size / 16;
+        if (chunks) {
+            hipLaunchKernelGGL(xent_weighted_rows_kernel<T>, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
+                               static_cast<const T *>(H), ldh, r.h == (size_t)-1, g.labels, g.lab64, g.dloss, scale, g.T, g.V, g.D,
+                               reinterpret_cast<T *>(room + r.hz), r.ldd, chunks);
+            if ((err = launched())) return err;
+        }
+    }
+    for (int v0 = 0; v0 < g.V; v0 += r.piece) {
+        g.v0 = v0;
+        g.vp = g.V - v0 < r.piece ? g.V - v0 : r.piece;
+        g.G = room + r.g;
+        g.ldg = padded_cols(g.vp, size);
+        if (g.T) {
+            const int tile = pick_tile(g.T, g.vp);
+            err = tile == 256 ? launch_probabilities<Tile256<T, KMAJOR, KMAJOR>>(g, st)
+                              : tile == 128 ? launch_probabilities<Tile128<T, KMAJOR, KMAJOR>>(g, st) : launch_probabilities<Tile64<T, KMAJOR>>(g, st);
+            if (err) return err;
+        }
+        XentProductArgs p{};
+        p.xcds = g.xcds;
+        if (dW) {
+            p.A = g.G; p.lda = g.ldg; p.a_cols = (int)g.ldg;
+            p.B = room + r.hz; p.ldb = r.ldd; p.b_cols = (int)r.ldd;
+            p.out = static_cast<char *>(dW) + v0 * lddw * (int64_t)sizeof(O); p.ldo = lddw;
+            p.rows = g.vp; p.cols = g.D; p.k = g.T;
+            p.scale = scale; p.by = by;
+            p.vec_out = writable_in_chunks(dW, lddw, g.D, sizeof(O));
+            auto tiles = [&](int b) { return (int64_t)((p.rows + b - 1) / b) * ((p.cols + b - 1) / b); };
+            err = rounds_cost(tiles(256), 1, 1.0) <= rounds_cost(tiles(128), 2, 0.31) ? launch_dw<Tile256<T, KROWS, KROWS>, O>(p, st)
+                                                                                      : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
+            if (err) return err;
+        }
+        if (dH && g.T) {
+            p.A = g.G; p.lda = g.ldg;
+            p.B = g.W + v0 * g.ldw * size; p.ldb = g.ldw; p.b_cols = (int)r.ldd;
+            p.out = reinterpret_cast<char *>(planes); p.ldo = r.ldd; p.plane = (int64_t)g.T * r.ldd;
+            p.rows = g.T; p.cols = g.D; p.k = g.vp;
+            p.splits = r.splits; p.add = v0 > 0;
+            const int tile = dh_tile(g.T);
+            err = tile == 256 ? launch_dh<Tile256<T, KMAJOR, KROWS>>(p, st)
+                              : tile == 128 ? launch_dh<Tile128<T, KMAJOR, KROWS>>(p, st) : launch_dh<Tile64<T, KROWS>>(p, st);
+            if (err) return err;
+        }
+    }
+    if (dH && g.T) {
+        const int64_t chunks = (int64_t)g.T * r.ldd / 4;
+        const bool vec = reinterpret_cast<uintptr_t>(dH) % (4 * sizeof(O)) == 0 && lddh % 4 == 0 && g.D % 4 == 0 && r.ldd == g.D;
+        hipLaunchKernelGGL(xent_dh_join_kernel<O>, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st, planes,
+                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, by, g.V, g.D, static_cast<O *>(dH), lddh, vec, chunks);
+        return launched();
+    }
+    return T2SP_OK;
+}
+
+}  // namespace t2sp
+
+using namespace t2sp;
+
+extern "C" size_t t2sp_xent_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
+    if (!xent_args_ok(type, T, V, D, ldh, ldw)) return 0;
+    return xent_room(false, type, H, W, T, V, D, ldh, ldw).total;
+}
+
+extern "C" int t2sp_xent(int type, const void *H, const void *W, const void *labels, int label_bits, float *loss, float *lse, int T, int V, int D,
+                         int64_t ldh, int64_t ldw, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!xent_args_ok(type, T, V, D, ldh, ldw) || (label_bits != 32 && label_bits != 64)) return T2SP_ERR_SHAPE;
+    if (T == 0) return T2SP_OK;
+    if (!H || !W || !labels || !loss) return T2SP_ERR_SHAPE;
+    const XentRoom r = xent_room(false, type, H, W, T, V, D, ldh, ldw);
+    if (!workspace || workspace_bytes < r.total || reinterpret_cast<uintptr_t>(workspace) % 16) return T2SP_ERR_SHAPE;
+    const hipStream_t st = (hipStream_t)stream;
+    char *room = static_cast<char *>(workspace);
+    XentArgs g{};
+    g.labels = labels; g.lab64 = label_bits == 64;
+    g.T = T; g.V = V; g.D = D; g.vp = V;
+    g.xcds = machine().xcds;
+    g.part = reinterpret_cast<float2 *>(room + r.part);
+    g.hit = reinterpret_cast<float *>(room + r.hit);
+    if (int err = xent_operands(g, r, type_bytes(type), room, H, W, ldh, ldw, st)) return err;
+    return with_types(type, type, [&](auto *t, auto *) { return xent_forward<std::remove_pointer_t<decltype(t)>>(g, loss, lse, st); });
+}
+
+extern "C" size_t t2sp_xent_grad_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
+    if (!xent_args_ok(type, T, V, D, ldh, ldw)) return 0;
+    return xent_room(true, type, H, W, T, V, D, ldh, ldw).total;
+}
+
+extern "C" int t2sp_xent_grad(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits, const float *lse,
+                              const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    if (!xent_args_ok(type, T, V, D, ldh, ldw) || !out_type_ok(type, out_type) || (label_bits != 32 && label_bits != 64) || !stride_ok(lddh) ||
+        !stride_ok(lddw) || (dH && lddh < D) || (dW && lddw < D))
+        return T2SP_ERR_SHAPE;
+    if ((!dH && !dW) || (T == 0 && !dW)) return T2SP_OK;
+    if (T && (!H || !W || !labels || !lse || !dloss)) return T2SP_ERR_SHAPE;
+    const XentRoom r = xent_room(true, type, H, W, T, V, D, ldh, ldw);
+    if (!workspace || workspace_bytes < r.total || reinterpret_cast<uintptr_t>(workspace) % 16) return T2SP_ERR_SHAPE;
+    const hipStream_t st = (hipStream_t)stream;
+    char *room = static_cast<char *>(workspace);
+    XentArgs g{};
+    g.labels = labels; g.lab64 = label_bits == 64;
+    g.T = T; g.V = V; g.D = D;
+    g.xcds = machine().xcds;
+    g.lse = lse; g.dloss = dloss;
+    if (T)
+        if (int err = xent_operands(g, r, type_bytes(type), room, H, W, ldh, ldw, st)) return err;
+    return with_types(type, out_type, [&](auto *t, auto *o) {
+        return xent_backward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, r, room, H, ldh, dH, dW, lddh, lddw, st);
+    });
+}

@@ -156,3 +156,67 @@ def gemm_grouped_wgrad(X, dY, offsets, out=None, out_dtype=None):
         _check(op, L.t2sp_gemm_grouped_wgrad(code, _type_codes()[dW.dtype], x, dy, offsets.data_ptr(), bits, dW.data_ptr(), T, E, K,
                                              N, ldx, ldy, _row(dW), _matrix(dW), ws, nbytes, _stream(X)))
     return dW
+
+
+def _xent_args(op, H, W, labels):
+    code = _tensors(op, (2, 2), H, W)
+    T, D = H.shape
+    V = W.shape[0]
+    _need(op, W.shape[1] == D and D >= 1 and V >= 1)
+    return code, T, V, D, _integers(op, labels, H, T)
+
+
+def _floats(op, t, like, n):
+    import torch
+    _need(op, t.dtype == torch.float32, BAD_TYPE)
+    _need(op, t.dim() == 1, BAD_DIMENSIONS)
+    _need(op, t.device == like.device and t.shape[0] == n and (n <= 1 or t.stride(0) == 1))
+    return t
+
+
+def xent(H, W, labels, loss=None, lse=None):
+    """Cross entropy of a softmax over a vocabulary, from hidden states: (loss, lse), float32 vectors of one value per token.
+
+    H: (T, D), W: (V, D), labels: T int32 or int64; z = H @ W.T is not kept.  lse[t] = log sum exp z[t],
+    loss[t] = lse[t] - z[t, labels[t]], 0 where the label is outside 0 .. V - 1."""
+    op = "xent"
+    if not _is_torch(H):
+        return _host_xent(op, H, W, labels, loss, lse)
+    import torch
+    code, T, V, D, bits = _xent_args(op, H, W, labels)
+    loss = torch.empty(T, dtype=torch.float32, device=H.device) if loss is None else _floats(op, loss, H, T)
+    lse = torch.empty(T, dtype=torch.float32, device=H.device) if lse is None else _floats(op, lse, H, T)
+    L = lib()
+    h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
+    with _On(H):
+        ws, nbytes, owner = _room(L.t2sp_xent_workspace_bytes(code, h, w, T, V, D, ldh, ldw), H)
+        _check(op, L.t2sp_xent(code, h, w, labels.data_ptr(), bits, loss.data_ptr(), lse.data_ptr(), T, V, D, ldh, ldw, ws, nbytes, _stream(H)))
+    return loss, lse
+
+
+def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted=(True, True)):
+    """Gradients (dH, dW) of sum_t dloss[t] * loss[t] (see xent): dH = g @ W, dW = g.T @ H with
+    g[t, v] = (exp(z[t, v] - lse[t]) - [v == labels[t]]) * dloss[t]; tokens without a label take no part.
+
+    lse: what xent returned; dloss: T float32.  The results have H's type, or float32 (out_dtype, or the type of dH / dW).
+    `wanted` leaves one out (its place in the result is None)."""
+    op = "xent_grad"
+    if not _is_torch(H):
+        return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW, wanted)
+    import torch
+    code, T, V, D, bits = _xent_args(op, H, W, labels)
+    _floats(op, lse, H, T)
+    _floats(op, dloss, H, T)
+    types = (H.dtype, torch.float32)
+    dtype = out_dtype or (dH.dtype if dH is not None else dW.dtype if dW is not None else H.dtype)
+    dH = _result(op, dH, (T, D), H, dtype, types) if wanted[0] or dH is not None else None
+    dW = _result(op, dW, (V, D), H, dtype, types) if wanted[1] or dW is not None else None
+    _need(op, dtype in types and all(t is None or t.dtype == dtype for t in (dH, dW)), BAD_TYPE)
+    L = lib()
+    h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
+    with _On(H):
+        ws, nbytes, owner = _room(L.t2sp_xent_grad_workspace_bytes(code, h, w, T, V, D, ldh, ldw), H)
+        _check(op, L.t2sp_xent_grad(code, _type_codes()[dtype], h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
+                                    dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None, T, V, D, ldh, ldw,
+                                    _row(dH) if dH is not None else D, _row(dW) if dW is not None else D, ws, nbytes, _stream(H)))
+    return dH, dW
