@@ -350,6 +350,22 @@ int t2sp_xent_grad(int type, int out_type, const void *H, const void *W, const v
                    const float *lse, const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh,
                    int64_t ldw, int64_t lddh, int64_t lddw, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Products with 4-bit weights and group scales, for the few rows of tokens being decoded:
+ *   y[m,n] = sum_k x[m,k] * (q[n,k] - z[n,k/group]) * s[n,k/group],  q in 0 .. 15, z = 8 without zero points
+ * group: 32, 64, 128, ... (a power of two; at least K for one scale per row).  x, y, scales and zero points
+ * are of `type`; sums in float.  E matrices, of which row m takes matrix ids[m] (E = 1 and ids = NULL: all rows
+ * take the one); an id outside 0 .. E - 1 gives a row of zeros.  With ids at most 65535 rows.
+ * The kernel reads a layout of its own that t2sp_w4_pack makes once, on the device, from plain arrays:
+ * q one number per byte (its low four bits), N x K with row stride ldq and sq between matrices; scales and
+ * zeros (may be NULL) N x ceil(K / group).  Per matrix, t2sp_w4_sizes gives the bytes of Q and the
+ * elements of S and of Z; Q, S and Z start on 16 bytes. */
+int t2sp_w4_sizes(int N, int K, int group, int64_t *q_bytes, int64_t *scale_elements);
+int t2sp_w4_pack(int type, const uint8_t *q, const void *scales, const void *zeros, int E, int N, int K, int group,
+                 int64_t ldq, int64_t sq, int64_t lds, int64_t ss, int64_t ldz, int64_t sz, void *Q, void *S, void *Z,
+                 void *stream);
+int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *S, const void *Z, const int *ids, void *y, int M,
+                 int N, int K, int E, int group, int64_t ldx, int64_t ldy, void *stream);
+
 /* dst[sum_d c_d*dst_strides[d]] = src[sum_d c_d*src_strides[d]] for every coordinate c of the
  * box `extents` (nd <= T2SP_MAX_DIMS, dimension 0 fastest).  Device-side replacement of the
  * host serializer/deserializer loops the reference's generated interface runs around its

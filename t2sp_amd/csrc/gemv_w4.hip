@@ -1,0 +1,312 @@
+// gemv_w4.hip — a few rows times a matrix of 4-bit numbers with a scale (and maybe a zero point) per group of inputs.
+//
+//   y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / G]) * s[n, k / G],   q in 0 .. 15, z = 8 when there are none
+//
+// A token being decoded reads every weight once: the bound is HBM, N K / 2 bytes.  What has to be cheap is taking
+// the numbers apart: at 6.5 TB/s a CU unpacks 21 of them per cycle.
+//
+// Numbers stay integers on their way into the matrix cores.  16 + q is a bfloat16 (and a half) whose upper bits are
+// constant and whose mantissa holds q in place: 0x4180 | q << 3 (half: 0x4c00 | q << 6), so two numbers cost a shift
+// and one v_and_or.  The 16 x 16 x 32 MFMA then sums x (16 + q) exactly but for float addition, over 32 inputs of 16
+// rows of the matrix, for up to 16 rows of x at once, and a group ends with
+//   y += s * (sum x (16 + q) - (16 + z) * sum x),
+// the last sum from one more MFMA with ones.  Scales and zero points are thus applied in float, once per group.
+// float rows of x go in as three bfloat16 pieces (24 bits together), each with its own MFMAs.
+//
+// Layout (t2sp_w4_pack, made once from plain numbers): blocks of 16 rows x 128 inputs, 1 KB, in which the 16 bytes of
+// lane l are what that lane feeds to four MFMAs: row l % 16, inputs 32 f + 8 (l / 16) + 0..7 for f = 0..3; in a word the
+// inputs 2 p and 2 p + 1 lie at bits 4 p and 4 p + 16.  A wave reads a block with one 16-byte load per lane, and any N
+// and K become whole blocks (numbers behind K meet zeros of x).  Scales and zero points: [group][row], rows padded to 16.
+//
+// One workgroup owns 16 * NT rows of the matrix and up to 16 * MT rows of x; its waves take the blocks of K in turn and
+// are joined through LDS in a fixed order.
+#include "product_core.hpp"
+#include "product_host.hpp"
+
+namespace t2sp {
+
+struct W4Args {
+    const char *x;
+    const uint8_t *Q;
+    const char *S, *Z;                   // of x's type; Z may be NULL
+    const int *ids;                      // row m takes matrix ids[m]; NULL: one matrix
+    char *y;
+    int M, N, K, E;
+    int64_t ldx, ldy;                    // elements
+    int blocks_k, tiles_n;               // of 128 inputs, of 16 rows
+    int group_shift;                     // G = 32 << group_shift
+    int groups;
+    int vec_x;                           // rows of x may be read 16 bytes at a time
+};
+
+// Pieces of x that go through the matrix cores, and 16 + q.
+template <class T> struct W4Type;
+template <> struct W4Type<__bf16> {
+    using M = __bf16;
+    static constexpr int PIECES = 1;
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, int p) {      // numbers at bits 4 p and 4 p + 16
+        return ((p == 0 ? w << 3 : w >> (4 * p - 3)) & 0x00780078u) | 0x41804180u;
+    }
+    static constexpr uint32_t ONES = 0x3f803f80u;
+};
+template <> struct W4Type<_Float16> {
+    using M = _Float16;
+    static constexpr int PIECES = 1;
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, int p) {
+        return ((p == 0 ? w << 6 : p == 1 ? w << 2 : w >> (4 * p - 6)) & 0x03c003c0u) | 0x4c004c00u;
+    }
+    static constexpr uint32_t ONES = 0x3c003c00u;
+};
+template <> struct W4Type<float> {
+    using M = __bf16;
+    static constexpr int PIECES = 3;
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, int p) { return W4Type<__bf16>::pair(w, p); }
+    static constexpr uint32_t ONES = W4Type<__bf16>::ONES;
+};
+
+// Eight inputs of a row of x from k on, zeros behind K and for rows that do not exist, as MFMA operands.
+template <class T>
+__device__ __forceinline__ void load_x(const T *row, bool exists, int k, int K, bool vec, pv4u (&out)[W4Type<T>::PIECES]) {
+    T v[8];
+    typedef T chunk __attribute__((ext_vector_type(16 / sizeof(T))));
+    if (exists && vec && k + 8 <= K) {
+#pragma unroll
+        for (int c = 0; c < 8; c += 16 / sizeof(T)) {
+            const chunk u = *reinterpret_cast<const chunk *>(row + k + c);
+#pragma unroll
+            for (int j = 0; j < (int)(16 / sizeof(T)); j++) v[c + j] = u[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = exists && k + j < K ? row[k + j] : (T)0.f;
+    }
+    typedef typename W4Type<T>::M m8 __attribute__((ext_vector_type(8)));
+    if constexpr (W4Type<T>::PIECES == 1) {
+        m8 u;
+#pragma unroll
+        for (int j = 0; j < 8; j++) u[j] = v[j];
+        out[0] = __builtin_bit_cast(pv4u, u);
+    } else {
+        m8 a, b, c;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            a[j] = (__bf16)v[j];
+            const float r = v[j] - (float)a[j];
+            b[j] = (__bf16)r;
+            c[j] = (__bf16)(r - (float)b[j]);
+        }
+        out[0] = __builtin_bit_cast(pv4u, a);
+        out[1] = __builtin_bit_cast(pv4u, b);
+        out[2] = __builtin_bit_cast(pv4u, c);
+    }
+}
+
+// MT: tiles of 16 rows of x.  WAVES take the blocks of K in turn.  SHIFT: a group has 32 << SHIFT of a block's inputs
+// (the whole block for groups of 128 and more).
+template <class T, int MT, int WAVES, int SHIFT>
+__global__ void __launch_bounds__(64 * WAVES) gemv_w4_kernel(const W4Args g) {
+    using Op = MatrixOp<typename W4Type<T>::M>;
+    constexpr int PIECES = W4Type<T>::PIECES;
+    __shared__ __attribute__((aligned(16))) pv4f joint[WAVES > 1 ? WAVES - 1 : 1][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, kg = lane >> 4;
+    const int tile = blockIdx.x, n0 = tile * 16 + 4 * kg;              // this lane ends with rows n0 .. n0 + 3 of x row r
+    int m0 = blockIdx.y * 16 * MT, m_end = g.M;
+    const uint8_t *Q = g.Q;
+    const T *S = reinterpret_cast<const T *>(g.S), *Z = reinterpret_cast<const T *>(g.Z);
+    const int64_t padded_n = (int64_t)g.tiles_n * 16;
+    bool matrix = true;
+    if (g.ids) {                                                        // one row of x per workgroup
+        m0 = blockIdx.y;
+        m_end = m0 + 1;
+        const int e = g.ids[m0];
+        matrix = e >= 0 && e < g.E;
+        const int64_t at = matrix ? e : 0;
+        Q += at * g.tiles_n * g.blocks_k * 1024;
+        S += at * g.groups * padded_n;
+        if (Z) Z += at * g.groups * padded_n;
+    }
+    Q += (int64_t)tile * g.blocks_k * 1024 + lane * 16;
+    pv4f y[MT], acc[MT], sum[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) y[i] = pv4f{0.f, 0.f, 0.f, 0.f};
+    typedef T quad __attribute__((ext_vector_type(4)));
+    const pv4u ones = pv4u{W4Type<T>::ONES, W4Type<T>::ONES, W4Type<T>::ONES, W4Type<T>::ONES};
+
+    if (matrix)
+        for (int b = wave; b < g.blocks_k; b += WAVES) {
+            const pv4u q = *reinterpret_cast<const pv4u *>(Q + (int64_t)b * 1024);
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const int step = b * 4 + f;                             // of 32 inputs
+                constexpr int LAST = (1 << SHIFT) - 1;
+                if ((f & LAST) == 0)
+#pragma unroll
+                    for (int i = 0; i < MT; i++) acc[i] = sum[i] = pv4f{0.f, 0.f, 0.f, 0.f};
+                const pv4u w = pv4u{W4Type<T>::pair(q[f], 0), W4Type<T>::pair(q[f], 1), W4Type<T>::pair(q[f], 2), W4Type<T>::pair(q[f], 3)};
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const int m = m0 + 16 * i + r;
+                    pv4u xs[PIECES];
+                    load_x<T>(reinterpret_cast<const T *>(g.x) + m * g.ldx, m < m_end, step * 32 + kg * 8, g.K, g.vec_x, xs);
+#pragma unroll
+                    for (int p = 0; p < PIECES; p++) {
+                        acc[i] = Op::mul(w, xs[p], acc[i]);
+                        sum[i] = Op::mul(ones, xs[p], sum[i]);
+                    }
+                }
+                const int group = step >> g.group_shift;
+                if ((f & LAST) == LAST && group < g.groups) {             // (steps behind K belong to no group)
+                    const quad s = *reinterpret_cast<const quad *>(S + group * padded_n + n0);
+                    pv4f z = pv4f{24.f, 24.f, 24.f, 24.f};
+                    if (Z) {
+                        const quad zz = *reinterpret_cast<const quad *>(Z + group * padded_n + n0);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) z[j] = 16.f + (float)zz[j];
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) y[i][j] += (float)s[j] * (acc[i][j] - z[j] * sum[i][j]);
+                }
+            }
+        }
+    if (WAVES > 1) {
+        if (wave > 0)
+#pragma unroll
+            for (int i = 0; i < MT; i++) joint[wave - 1][i][lane] = y[i];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; w++)
+#pragma unroll
+            for (int i = 0; i < MT; i++) y[i] += joint[w][i][lane];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = m0 + 16 * i + r;
+        if (m >= m_end || (g.ids && r)) continue;
+        T *row = reinterpret_cast<T *>(g.y) + m * g.ldy;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (n0 + j < g.N) row[n0 + j] = (T)y[i][j];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ packing
+__global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t *q, int N, int K, int64_t ldq, int64_t sq, int blocks_k, int tiles_n, int64_t words,
+                                                      uint32_t *Q) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
+        const int f = (int)(i & 3), lane = (int)(i >> 2) & 63;
+        const int64_t block = i >> 8, b = block % blocks_k, t = block / blocks_k % tiles_n, e = block / blocks_k / tiles_n;
+        const int64_t n = t * 16 + (lane & 15), k = b * 128 + f * 32 + (lane >> 4) * 8;
+        uint32_t w = 0;
+        if (n < N)
+            for (int j = 0; j < 8; j++)
+                if (k + j < K) w |= (uint32_t)(q[e * sq + n * ldq + k + j] & 15) << (4 * (j >> 1) + 16 * (j & 1));
+        Q[i] = w;
+    }
+}
+
+// dst[e][g][n] = src[e][n][g], zeros for n from N to the padded rows.
+template <class T>
+__global__ void __launch_bounds__(256) w4_scales_kernel(const T *src, int N, int groups, int64_t ld, int64_t stride, int64_t padded_n, int64_t total, T *dst) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t n = i % padded_n, g = i / padded_n % groups, e = i / padded_n / groups;
+        dst[i] = n < N ? src[e * stride + n * ld + g] : (T)0;
+    }
+}
+
+static int group_shift_of(int group) {
+    for (int s = 0; s <= 25; s++)
+        if (group == 32 << s) return s;
+    return -1;
+}
+
+static unsigned blocks_for(int64_t n) { return (unsigned)(n < 256 * 65536 ? (n + 255) / 256 : 65536); }
+
+}  // namespace t2sp
+
+using namespace t2sp;
+
+extern "C" int t2sp_w4_sizes(int N, int K, int group, int64_t *q_bytes, int64_t *scale_elements) {
+    if (!extent_ok(N) || !extent_ok(K) || group_shift_of(group) < 0 || !q_bytes || !scale_elements) return T2SP_ERR_SHAPE;
+    const int64_t tiles_n = ((int64_t)N + 15) / 16, blocks_k = ((int64_t)K + 127) / 128;
+    *q_bytes = tiles_n * blocks_k * 1024;
+    *scale_elements = ((int64_t)K + group - 1) / group * tiles_n * 16;
+    return T2SP_OK;
+}
+
+extern "C" int t2sp_w4_pack(int type, const uint8_t *q, const void *scales, const void *zeros, int E, int N, int K, int group, int64_t ldq, int64_t sq,
+                            int64_t lds, int64_t ss, int64_t ldz, int64_t sz, void *Q, void *S, void *Z, void *stream) {
+    int64_t qb, se;
+    const int size = type_bytes(type);
+    if (!size || !extent_ok(E) || t2sp_w4_sizes(N, K, group, &qb, &se)) return T2SP_ERR_SHAPE;
+    const int groups = (K + group - 1) / group;
+    if (!q || !scales || !Q || !S || (zeros && !Z) || !stride_ok(ldq) || !stride_ok(sq) || !stride_ok(lds) || !stride_ok(ss) || ldq < K || lds < groups ||
+        (zeros && (!stride_ok(ldz) || !stride_ok(sz) || ldz < groups)))
+        return T2SP_ERR_SHAPE;
+    const hipStream_t st = (hipStream_t)stream;
+    const int64_t words = qb / 4 * E, total = se * E;
+    const int64_t padded_n = ((int64_t)N + 15) / 16 * 16;
+    hipLaunchKernelGGL(w4_pack_kernel, dim3(blocks_for(words)), dim3(256), 0, st, q, N, K, ldq, sq, (int)(((int64_t)K + 127) / 128), (int)(padded_n / 16),
+                       words, static_cast<uint32_t *>(Q));
+    if (int err = launched()) return err;
+    for (int i = 0; i < (zeros ? 2 : 1); i++) {
+        const void *from = i ? zeros : scales;
+        void *to = i ? Z : S;
+        const int64_t ld = i ? ldz : lds, stride = i ? sz : ss;
+        if (size == 4)
+            hipLaunchKernelGGL(w4_scales_kernel<uint32_t>, dim3(blocks_for(total)), dim3(256), 0, st, static_cast<const uint32_t *>(from), N, groups, ld,
+                               stride, padded_n, total, static_cast<uint32_t *>(to));
+        else
+            hipLaunchKernelGGL(w4_scales_kernel<uint16_t>, dim3(blocks_for(total)), dim3(256), 0, st, static_cast<const uint16_t *>(from), N, groups, ld,
+                               stride, padded_n, total, static_cast<uint16_t *>(to));
+        if (int err = launched()) return err;
+    }
+    return T2SP_OK;
+}
+
+namespace t2sp {
+template <class T, int MT, int SHIFT>
+static int launch_w4(const W4Args &g, hipStream_t st) {
+    const int64_t rows = g.ids ? g.M : (g.M + 16 * MT - 1) / (16 * MT);
+    if (rows > 65535) return T2SP_ERR_SHAPE;
+    const dim3 grid((unsigned)g.tiles_n, (unsigned)rows);
+    if (g.blocks_k >= 16) hipLaunchKernelGGL((gemv_w4_kernel<T, MT, 8, SHIFT>), grid, dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((gemv_w4_kernel<T, MT, 4, SHIFT>), grid, dim3(256), 0, st, g);
+    return launched();
+}
+template <class T, int MT>
+static int launch_w4(const W4Args &g, hipStream_t st) {
+    return g.group_shift == 0 ? launch_w4<T, MT, 0>(g, st) : g.group_shift == 1 ? launch_w4<T, MT, 1>(g, st) : launch_w4<T, MT, 2>(g, st);
+}
+}  // namespace t2sp
+
+extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *S, const void *Z, const int *ids, void *y, int M, int N, int K, int E,
+                            int group, int64_t ldx, int64_t ldy, void *stream) {
+    const int size = type_bytes(type);
+    int64_t qb, se;
+    if (!size || M < 0 || M > T2SP_MAX_EXTENT || !extent_ok(E) || t2sp_w4_sizes(N, K, group, &qb, &se) || !stride_ok(ldx) || !stride_ok(ldy) || ldx < K ||
+        ldy < N)
+        return T2SP_ERR_SHAPE;
+    if (M == 0) return T2SP_OK;
+    if (!x || !Q || !S || !y || (!ids && E != 1)) return T2SP_ERR_SHAPE;
+    if (reinterpret_cast<uintptr_t>(Q) % 16 || reinterpret_cast<uintptr_t>(S) % 16 || reinterpret_cast<uintptr_t>(Z) % 16) return T2SP_ERR_SHAPE;
+    W4Args g{};
+    g.x = static_cast<const char *>(x); g.Q = static_cast<const uint8_t *>(Q);
+    g.S = static_cast<const char *>(S); g.Z = static_cast<const char *>(Z);
+    g.ids = ids; g.y = static_cast<char *>(y);
+    g.M = M; g.N = N; g.K = K; g.E = E;
+    g.ldx = ldx; g.ldy = ldy;
+    g.blocks_k = (int)(((int64_t)K + 127) / 128); g.tiles_n = (int)(((int64_t)N + 15) / 16);
+    g.group_shift = group_shift_of(group);
+    g.groups = (K + group - 1) / group;
+    g.vec_x = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0;
+    const hipStream_t st = (hipStream_t)stream;
+    return with_types(type, type, [&](auto *t, auto *) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (ids || M <= 16) return launch_w4<T, 1>(g, st);
+        return M <= 32 ? launch_w4<T, 2>(g, st) : launch_w4<T, 4>(g, st);
+    });
+}

@@ -220,3 +220,65 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
                                     dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None, T, V, D, ldh, ldw,
                                     _row(dH) if dH is not None else D, _row(dW) if dW is not None else D, ws, nbytes, _stream(H)))
     return dH, dW
+
+
+class W4:
+    """Matrices of 4-bit numbers in the layout of the kernels (pack_w4): E matrices of N x K, or one (E is None)."""
+
+    def __init__(self, E, N, K, group, Q, S, Z):
+        self.E, self.N, self.K, self.group, self.Q, self.S, self.Z = E, N, K, group, Q, S, Z
+        self.code = _type_codes()[S.dtype]
+
+
+def pack_w4(q, scales, zeros=None, group=128):
+    """Lays 4-bit numbers out for gemv_w4, once: W[n, k] = (q[n, k] - zeros[n, k // group]) * scales[n, k // group], with
+    zeros = 8 when there are none.
+
+    q: uint8 (N, K), or (E, N, K) for E matrices, one number in the low four bits of each byte; scales, zeros:
+    (..., N, ceil(K / group)) of the type of the rows they will meet (float32, float16 or bfloat16).  group: a power of two
+    from 32 on; at least K for one scale per row."""
+    import torch
+    op = "pack_w4"
+    _need(op, q.dtype == torch.uint8, BAD_TYPE)
+    _need(op, q.dim() in (2, 3), BAD_DIMENSIONS)
+    _need(op, q.is_cuda and (q.shape[-1] <= 1 or q.stride(-1) == 1))
+    code = _tensors(op, (q.dim(),) * 2, *((scales,) if zeros is None else (scales, zeros)))
+    N, K = q.shape[-2:]
+    group = int(group)
+    qb, se = ctypes.c_int64(), ctypes.c_int64()
+    L = lib()
+    _check(op, L.t2sp_w4_sizes(N, K, group, ctypes.byref(qb), ctypes.byref(se)))
+    E = q.shape[0] if q.dim() == 3 else 1
+    want = tuple(q.shape[:-1]) + (-(-K // group),)
+    _need(op, E >= 1 and tuple(scales.shape) == want and (zeros is None or tuple(zeros.shape) == want) and scales.device == q.device)
+    Q = torch.empty(E * qb.value, dtype=torch.uint8, device=q.device)
+    S = torch.empty(E * se.value, dtype=scales.dtype, device=q.device)
+    Z = torch.empty_like(S) if zeros is not None else None
+    each = lambda t: _matrix(t) if t.dim() == 3 else 0
+    with _On(q):
+        _check(op, L.t2sp_w4_pack(code, q.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, E, N, K, group,
+                                  _row(q), each(q), _row(scales), each(scales), _row(zeros) if zeros is not None else 0,
+                                  each(zeros) if zeros is not None else 0, Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None,
+                                  _stream(q)))
+    return W4(E if q.dim() == 3 else None, N, K, group, Q, S, Z)
+
+
+def gemv_w4(x, w, ids=None, out=None):
+    """y = x @ W.T for a few rows x (M, K) and 4-bit weights w (pack_w4), y (M, N) of x's type.
+
+    With matrices for E experts, ids (M int32) picks the matrix of each row; a row whose id is outside 0 .. E - 1 is zeros."""
+    import torch
+    op = "gemv_w4"
+    _need(op, x.dtype == w.S.dtype, BAD_TYPE)
+    _need(op, x.dim() == 2, BAD_DIMENSIONS)
+    M, K = x.shape
+    _need(op, K == w.K and x.is_cuda and x.device == w.Q.device and (K <= 1 or x.stride(1) == 1) and (ids is None) == (w.E is None))
+    if ids is not None:
+        _need(op, ids.dtype == torch.int32, BAD_TYPE)
+        _integers(op, ids, x, M)
+    y = _result(op, out, (M, w.N), x, x.dtype, (x.dtype,))
+    with _On(x):
+        _check(op, lib().t2sp_gemv_w4(w.code, x.data_ptr(), w.Q.data_ptr(), w.S.data_ptr(), w.Z.data_ptr() if w.Z is not None else None,
+                                      ids.data_ptr() if ids is not None else None, y.data_ptr(), M, w.N, K, w.E or 1, w.group, _row(x), _row(y),
+                                      _stream(x)))
+    return y
