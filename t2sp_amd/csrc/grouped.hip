@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g
     clear<P>(acc);
     product_run<P>(a, b, g.K, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const int n = n0 + (wave % P::WN) * P::TN;
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int m = (wave / P::WN) * P::TM + 16 * i + (lane & 15);
@@ -114,16 +114,34 @@ __global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g
     }
 }
 
+// The group that is `rank`-th in size (ties: the lower index first); the first 64 groups among themselves, as the
+// groups behind them, which keep their places.
+__device__ __forceinline__ int group_of_rank(const GroupedArgs &g, int rank) {
+    if (rank >= 64) return rank;
+    const int lane = threadIdx.x & 63, among = g.E < 64 ? g.E : 64;
+    int size = -1;
+    if (lane < among) size = group_edge(g, lane + 1) - group_edge(g, lane);
+    int place = 0;
+    for (int j = 0; j < among; j++) {
+        const int other = __builtin_amdgcn_readlane(size, j);
+        place += other > size || (other == size && j < lane);
+    }
+    return __ffsll((unsigned long long)__ballot(lane < among && place == rank)) - 1;
+}
+
 // dW[e] tile: rows of the tile are K (contiguous in X), columns N (contiguous in dY), the reduction runs over the
 // rows of the group.  Here W is dY (ldw its row stride), Y is dW (ldy, sw its row and matrix strides).
 template <class P, class O>
 __global__ void __launch_bounds__(P::THREADS) grouped_wgrad_kernel(const GroupedArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    // Every die takes its share of every group's tiles (dies that took whole groups would end with the largest one), the
+    // workgroups of a die go through the groups from the largest to the smallest, so that short tiles come last.
     const int row_tiles = (g.K + P::BM - 1) / P::BM;
-    const unsigned w = die_run(blockIdx.x, gridDim.x, g.xcds), per_group = (unsigned)row_tiles * g.col_tiles;
-    const int e = w / per_group;
-    int k0, n0;
-    panel_tile(w % per_group, row_tiles, g.col_tiles, &k0, &n0);
+    const unsigned per_group = (unsigned)row_tiles * g.col_tiles;
+    int e, k0, n0;
+    const unsigned rank = blockIdx.x / per_group;
+    panel_tile(die_run(blockIdx.x % per_group, per_group, g.xcds), row_tiles, g.col_tiles, &k0, &n0);
+    e = group_of_rank(g, rank);
     k0 *= P::BM;
     n0 *= P::BN;
     const int first = group_edge(g, e), last = group_edge(g, e + 1);
@@ -139,7 +157,7 @@ __global__ void __launch_bounds__(P::THREADS) grouped_wgrad_kernel(const Grouped
     clear<P>(acc);
     if (rows) product_run<P>(a, b, rows, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const int n = n0 + (wave % P::WN) * P::TN;
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int k = k0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);

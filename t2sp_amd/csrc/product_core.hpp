@@ -107,7 +107,7 @@ struct ProductTile {
     static_assert(B_LOADS >= 1 && B_LOADS * NW * 16 == BN, "the waves share B's loads evenly");
     static_assert(AS == KMAJOR || BM * SZ >= 256, "a KROWS tile row holds at least the sixteen chunks a key permutes");
     static_assert(BS == KMAJOR || BN * SZ >= 256, "a KROWS tile row holds at least the sixteen chunks a key permutes");
-    static_assert(NT == 2 || NT == 4, "the B keys below are worked out for these");
+    static_assert(NT == 2 || NT == 4 || (NT == 8 && SZ == 2), "the B keys below are worked out for these");
     static_assert(S >= 3 && (S - 1) * LOADS < 63, "the wait counter has six bits");
 
     // key of a KMAJOR row: the sixteen rows a read touches take four to each of the four chunk positions, rows
@@ -119,7 +119,7 @@ struct ProductTile {
     static __device__ __forceinline__ int key_krows(bool b, int k) {
         if (SZ == 2) {
             if (!b) return 2 * ((k & 3) | ((k >> 3) & 1) << 2);
-            return NT == 4 ? (k & 1) | ((k >> 1) & 1) << 3 : (k & 3) << 2;
+            return NT == 8 ? k & 3 : NT == 4 ? (k & 1) | ((k >> 1) & 1) << 3 : (k & 3) << 2;
         }
         const int q = (k >> 2) & 3;
         if (!b) return q << 2;
@@ -297,26 +297,66 @@ __device__ __forceinline__ void panel_tile(int64_t at, int row_tiles, int col_ti
     *col = rest / high;
 }
 
-// A lane's 4 NT consecutive columns of one row, rounded to the output's type.
+// Lane sixteens a, b of `x` and c, d of `y` change places: x = {x0, y0, x2, y2}, y = {x1, y1, x3, y3} (16) or
+// x = {x0, x1, y0, y1}, y = {x2, x3, y2, y3} (32), indices counting sixteens.
+template <int LANES>
+__device__ __forceinline__ void swap_sixteens(pv4u &x, pv4u &y) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const auto r = LANES == 16 ? __builtin_amdgcn_permlane16_swap(x[i], y[i], false, false) : __builtin_amdgcn_permlane32_swap(x[i], y[i], false, false);
+        x[i] = r[0];
+        y[i] = r[1];
+    }
+}
+
+// Calls f(column, 16 bytes of the row from that column on, rounded to O) for a lane's share of row lane % 16 of
+// accumulator row i, whose first column of the wave is n.  The four lanes of a row hold LANE_N consecutive columns each;
+// they exchange 16-byte chunks first such that one store (or load) of the wave covers 64 consecutive bytes of each row:
+// chunks 64 bytes apart, as they lie in the accumulators, cost a memory request each (268 MB of float results of an
+// 8192 x 8192 x 4096 product: 695 us stored so, 430 us exchanged).
+template <class P, class O, class F>
+__device__ __forceinline__ void row_chunks(int n, const pv4f (&acc)[P::NT], F f) {
+    constexpr int CE = 16 / sizeof(O), C = P::LANE_N / CE;
+    typedef O chunk __attribute__((ext_vector_type(CE)));
+    static_assert(C == 1 || C == 2 || C == 4, "chunks per lane");
+    pv4u v[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        chunk u;
+#pragma unroll
+        for (int i = 0; i < CE; i++) u[i] = (O)acc[(c * CE + i) / 4][(c * CE + i) % 4];
+        v[c] = __builtin_bit_cast(pv4u, u);
+    }
+    const int kg = (threadIdx.x >> 4) & 3;
+    if constexpr (C == 2) {                          // v[0]: the chunks of sixteens 0 and 1 in order, v[1]: of 2 and 3
+        swap_sixteens<16>(v[0], v[1]);
+        swap_sixteens<32>(v[0], v[1]);
+    } else if constexpr (C == 4) {                   // v[c]: the four chunks of sixteen c
+        swap_sixteens<32>(v[0], v[2]);
+        swap_sixteens<32>(v[1], v[3]);
+        swap_sixteens<16>(v[0], v[1]);
+        swap_sixteens<16>(v[2], v[3]);
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++) f(n + (c * 4 + kg) * CE, __builtin_bit_cast(chunk, v[c]));
+}
+
+// Row lane % 16 of accumulator row i to memory, columns below n_end, rounded to the output's type; `row` is the row's first
+// element, n the wave's first column.  `vec`: 16-byte stores are possible (n_end is then a whole number of chunks).
 template <class P, class O>
 __device__ __forceinline__ void store_row(char *row, int n, int n_end, const pv4f (&acc)[P::NT], bool vec) {
-    O *p = reinterpret_cast<O *>(row) + n;
-    typedef O chunk __attribute__((ext_vector_type(16 / sizeof(O))));
     constexpr int CE = 16 / sizeof(O);
-    if (vec) {
+    typedef O chunk __attribute__((ext_vector_type(CE)));
+    O *p = reinterpret_cast<O *>(row);
+    row_chunks<P, O>(n, acc, [&](int col, chunk v) {
+        if (vec) {
+            if (col < n_end) *reinterpret_cast<chunk *>(p + col) = v;
+        } else {
 #pragma unroll
-        for (int c = 0; c < P::LANE_N / CE; c++) {
-            if (n + c * CE >= n_end) break;
-            chunk v;
-#pragma unroll
-            for (int i = 0; i < CE; i++) v[i] = (O)acc[(c * CE + i) / 4][(c * CE + i) % 4];
-            *reinterpret_cast<chunk *>(p + c * CE) = v;
+            for (int i = 0; i < CE; i++)
+                if (col + i < n_end) p[col + i] = v[i];
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < P::LANE_N; i++)
-            if (n + i < n_end) p[i] = (O)acc[i / 4][i % 4];
-    }
+    });
 }
 
 template <class P>
@@ -328,10 +368,12 @@ __device__ __forceinline__ void clear(pv4f (&acc)[P::MT][P::NT]) {
 }
 
 
-// Tile shapes.  256 x 256 has the most arithmetic per byte from LDS and one workgroup per CU; 128 x 128 (two per CU)
-// and 64 x 128 (three per CU) fill the chip when there are few rows per group.
-template <class T, int AS, int BS> using Tile256 = ProductTile<T, 256, 256, 2, 4, AS, BS, 4>;
-template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, 2, AS, BS, 4>;
+// Tile shapes.  256 x 256 has the most arithmetic per byte from LDS and one workgroup per CU, whose 160 KB hold five
+// stages (8192 x 8192 x 2048, bfloat16, both operands k-contiguous: 282 us with four stages, 215 with five; k = 8192
+// with rows contiguous: 763 / 770 us, 1.43 PFLOP/s); 128 x 128 (two per CU) and 64 x 128 (three per CU) fill the chip
+// when there are few rows.
+template <class T, int AS, int BS> using Tile256 = ProductTile<T, 256, 256, 2, 4, AS, BS, 5>;
+template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, 2, AS, BS, 5>;
 template <class T, int BS> using Tile64 = ProductTile<T, 64, 128, 1, 4, KMAJOR, BS, 4>;
 
 }  // namespace t2sp

@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
             const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (n + c == hot ? 1.f : 0.f);
             acc[i][c / 4][c % 4] = valid && n + c < g.vp ? p * GradientScale<T>::value : 0.f;
         }
-        store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n, (int)g.ldg, acc[i], true);
+        store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n0 + (wave % P::WN) * P::TN, (int)g.ldg, acc[i], true);
     }
 }
 
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
     clear<P>(acc);
     product_run<P>(a, b, g.k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const int n = n0 + (wave % P::WN) * P::TN;
     const float by = *g.scale * g.by;
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
@@ -286,18 +286,17 @@ __global__ void __launch_bounds__(P::THREADS) xent_dh_kernel(const XentProductAr
     clear<P>(acc);
     if (k > 0) product_run<P>(a, b, k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const int n = n0 + (wave % P::WN) * P::TN;
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int m = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
         if (m >= g.rows) continue;
-        float *row = reinterpret_cast<float *>(g.out) + s * g.plane + m * g.ldo + n;
-#pragma unroll
-        for (int j = 0; j < P::NT; j++) {
-            if (n + 4 * j >= g.ldo) break;               // (planes have rows of whole 16-byte chunks)
-            pv4f *p = reinterpret_cast<pv4f *>(row + 4 * j);
-            *p = g.add ? *p + acc[i][j] : acc[i][j];
-        }
+        float *row = reinterpret_cast<float *>(g.out) + s * g.plane + m * g.ldo;
+        row_chunks<P, float>(n, acc[i], [&](int col, pv4f v) {
+            if (col >= g.ldo) return;                    // (planes have rows of whole 16-byte chunks)
+            pv4f *p = reinterpret_cast<pv4f *>(row + col);
+            *p = g.add ? *p + v : v;
+        });
     }
 }
 
