@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_stats_kernel(const XentArgs g
     pv4f acc[P::MT][P::NT];
     logits_tile<P>(g, m0, n0, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int first_m = (wave / P::WN) * P::TM, n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const int first_m = (wave / P::WN) * P::TM, n = n0 + (wave % P::WN) * P::TN + P::lane_column(lane);
     float2 *joint = reinterpret_cast<float2 *>(smem);        // [WN][BM]; the product is done with its LDS
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
@@ -85,8 +85,9 @@ __global__ void __launch_bounds__(P::THREADS) xent_stats_kernel(const XentArgs g
 #pragma unroll
         for (int c = 0; c < P::LANE_N; c++) {
             const float z = acc[i][c / 4][c % 4];
-            if (n + c < g.V) top = fmaxf(top, z);
-            if (n + c == hot && n + c < g.V) g.hit[m0 + m] = z;
+            const int v = n + 8 * (c / 4) + c % 4;
+            if (v < g.V) top = fmaxf(top, z);
+            if (v == hot && v < g.V) g.hit[m0 + m] = z;
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_stats_kernel(const XentArgs g
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < P::LANE_N; c++)
-            if (n + c < g.V) sum += exp_of(acc[i][c / 4][c % 4] - base);
+            if (n + 8 * (c / 4) + c % 4 < g.V) sum += exp_of(acc[i][c / 4][c % 4] - base);
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
         if (lane < 16) joint[(wave % P::WN) * P::BM + m] = make_float2(top, sum);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
     pv4f acc[P::MT][P::NT];
     logits_tile<P>(g, m0, n0, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = n0 + (wave % P::WN) * P::TN + P::LANE_N * (lane >> 4);
+    const int n = n0 + (wave % P::WN) * P::TN + P::lane_column(lane);
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int t = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
@@ -222,8 +223,9 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
         const int64_t hot = label - g.v0;
 #pragma unroll
         for (int c = 0; c < P::LANE_N; c++) {
-            const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (n + c == hot ? 1.f : 0.f);
-            acc[i][c / 4][c % 4] = valid && n + c < g.vp ? p * GradientScale<T>::value : 0.f;
+            const int v = n + 8 * (c / 4) + c % 4;
+            const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (v == hot ? 1.f : 0.f);
+            acc[i][c / 4][c % 4] = valid && v < g.vp ? p * GradientScale<T>::value : 0.f;
         }
         store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n0 + (wave % P::WN) * P::TN, (int)g.ldg, acc[i], true);
     }
