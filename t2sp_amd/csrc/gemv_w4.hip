@@ -36,7 +36,7 @@ struct W4Args {
     int blocks_k, tiles_n;               // of 128 inputs, of 16 rows
     int group_shift;                     // G = 32 << group_shift
     int groups;
-    int vec_x;                           // rows of x may be read 16 bytes at a time
+    int vec_x;                           // rows of x are whole 16-byte chunks
 };
 
 // Pieces of x that go through the matrix cores, and 16 + q.
@@ -64,34 +64,39 @@ template <> struct W4Type<float> {
     static constexpr uint32_t ONES = W4Type<__bf16>::ONES;
 };
 
-// Eight inputs of a row of x from k on, zeros behind K and for rows that do not exist, as MFMA operands.
-template <class T>
-__device__ __forceinline__ void load_x(const T *row, bool exists, int k, int K, bool vec, pv4u (&out)[W4Type<T>::PIECES]) {
-    T v[8];
-    typedef T chunk __attribute__((ext_vector_type(16 / sizeof(T))));
-    if (exists && vec && k + 8 <= K) {
+// Eight inputs of a row of x at `k`, as MFMA operands: zeros behind K and for rows that do not exist.  VEC: rows are whole
+// 16-byte chunks (the loads outside go past the descriptor's end and read zeros without memory traffic).
+template <class T, bool VEC>
+__device__ __forceinline__ void load_x(__amdgpu_buffer_rsrc_t rsrc, const T *x, uint32_t row, bool exists, int k, int K, pv4u (&raw)[sizeof(T) / 2]) {
+    if (VEC) {
+        const uint32_t off = exists && k < K ? row * (uint32_t)sizeof(T) + (uint32_t)k * (uint32_t)sizeof(T) : OUT_OF_RANGE;
 #pragma unroll
-        for (int c = 0; c < 8; c += 16 / sizeof(T)) {
-            const chunk u = *reinterpret_cast<const chunk *>(row + k + c);
+        for (int c = 0; c < (int)sizeof(T) / 2; c++) raw[c] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(off + 16 * c), 0, 0);
+    } else {
+        T v[8];
 #pragma unroll
-            for (int j = 0; j < (int)(16 / sizeof(T)); j++) v[c + j] = u[j];
+        for (int j = 0; j < 8; j++) v[j] = exists && k + j < K ? x[row + k + j] : (T)0.f;
+#pragma unroll
+        for (int c = 0; c < (int)sizeof(T) / 2; c++) {
+            typename Chunk<T>::type u;
+#pragma unroll
+            for (int j = 0; j < 16 / (int)sizeof(T); j++) u[j] = v[c * (16 / sizeof(T)) + j];
+            raw[c] = __builtin_bit_cast(pv4u, u);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = exists && k + j < K ? row[k + j] : (T)0.f;
     }
-    typedef typename W4Type<T>::M m8 __attribute__((ext_vector_type(8)));
-    if constexpr (W4Type<T>::PIECES == 1) {
-        m8 u;
-#pragma unroll
-        for (int j = 0; j < 8; j++) u[j] = v[j];
-        out[0] = __builtin_bit_cast(pv4u, u);
+}
+template <class T>
+__device__ __forceinline__ void pieces_of(const pv4u (&raw)[sizeof(T) / 2], pv4u (&out)[W4Type<T>::PIECES]) {
+    if constexpr (sizeof(T) == 2) {
+        out[0] = raw[0];
     } else {
-        m8 a, b, c;
+        typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+        b8 a, b, c;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            a[j] = (__bf16)v[j];
-            const float r = v[j] - (float)a[j];
+            const float v = __builtin_bit_cast(pv4f, raw[j / 4])[j % 4];
+            a[j] = (__bf16)v;
+            const float r = v - (float)a[j];
             b[j] = (__bf16)r;
             c[j] = (__bf16)(r - (float)b[j]);
         }
@@ -101,13 +106,16 @@ __device__ __forceinline__ void load_x(const T *row, bool exists, int k, int K, 
     }
 }
 
-// MT: tiles of 16 rows of x.  WAVES take the blocks of K in turn.  SHIFT: a group has 32 << SHIFT of a block's inputs
-// (the whole block for groups of 128 and more).
-template <class T, int MT, int WAVES, int SHIFT>
-__global__ void __launch_bounds__(64 * WAVES) gemv_w4_kernel(const W4Args g) {
+// MT: tiles of 16 rows of x.  SHIFT: a group has 32 << SHIFT of a block's inputs (the whole block for groups of 128 and more).
+// A wave has DEEP blocks of the matrix, their scales and their part of x under way before it waits for the first.
+constexpr int W4_WAVES = 8;
+template <class T, int MT, int SHIFT, bool VEC>
+__global__ void __launch_bounds__(64 * W4_WAVES) gemv_w4_kernel(const W4Args g) {
     using Op = MatrixOp<typename W4Type<T>::M>;
-    constexpr int PIECES = W4Type<T>::PIECES;
-    __shared__ __attribute__((aligned(16))) pv4f joint[WAVES > 1 ? WAVES - 1 : 1][MT][64];
+    constexpr int PIECES = W4Type<T>::PIECES, DEEP = MT * sizeof(T) <= 2 ? 4 : MT * sizeof(T) <= 4 ? 2 : 1;
+    constexpr int GROUPS = SHIFT == 0 ? 4 : SHIFT == 1 ? 2 : 1;         // of a block
+    typedef T quad __attribute__((ext_vector_type(4)));
+    __shared__ __attribute__((aligned(16))) pv4f joint[W4_WAVES - 1][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, kg = lane >> 4;
     const int tile = blockIdx.x, n0 = tile * 16 + 4 * kg;              // this lane ends with rows n0 .. n0 + 3 of x row r
@@ -127,69 +135,92 @@ __global__ void __launch_bounds__(64 * WAVES) gemv_w4_kernel(const W4Args g) {
         if (Z) Z += at * g.groups * padded_n;
     }
     Q += (int64_t)tile * g.blocks_k * 1024 + lane * 16;
-    pv4f y[MT], acc[MT], sum[MT];
+    S += n0;
+    if (Z) Z += n0;
+    const T *x = reinterpret_cast<const T *>(g.x) + (int64_t)m0 * g.ldx;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x), 0, 0x7fffffff, 0x00020000);
+    pv4f y[MT];
 #pragma unroll
     for (int i = 0; i < MT; i++) y[i] = pv4f{0.f, 0.f, 0.f, 0.f};
-    typedef T quad __attribute__((ext_vector_type(4)));
     const pv4u ones = pv4u{W4Type<T>::ONES, W4Type<T>::ONES, W4Type<T>::ONES, W4Type<T>::ONES};
 
     if (matrix)
-        for (int b = wave; b < g.blocks_k; b += WAVES) {
-            const pv4u q = *reinterpret_cast<const pv4u *>(Q + (int64_t)b * 1024);
+        for (int b0 = wave; b0 < g.blocks_k; b0 += DEEP * W4_WAVES) {
+            pv4u q[DEEP], xs[DEEP][4][MT][sizeof(T) / 2];
+            quad s[DEEP][GROUPS], z[DEEP][GROUPS];
 #pragma unroll
-            for (int f = 0; f < 4; f++) {
-                const int step = b * 4 + f;                             // of 32 inputs
-                constexpr int LAST = (1 << SHIFT) - 1;
-                if ((f & LAST) == 0)
+            for (int d = 0; d < DEEP; d++) {                            // (blocks behind the last one repeat it against zeros)
+                const int b = b0 + d * W4_WAVES, read = b < g.blocks_k ? b : g.blocks_k - 1;
+                q[d] = __builtin_nontemporal_load(reinterpret_cast<const pv4u *>(Q + (int64_t)read * 1024));
 #pragma unroll
-                    for (int i = 0; i < MT; i++) acc[i] = sum[i] = pv4f{0.f, 0.f, 0.f, 0.f};
-                const pv4u w = pv4u{W4Type<T>::pair(q[f], 0), W4Type<T>::pair(q[f], 1), W4Type<T>::pair(q[f], 2), W4Type<T>::pair(q[f], 3)};
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const int m = m0 + 16 * i + r;
-                    pv4u xs[PIECES];
-                    load_x<T>(reinterpret_cast<const T *>(g.x) + m * g.ldx, m < m_end, step * 32 + kg * 8, g.K, g.vec_x, xs);
-#pragma unroll
-                    for (int p = 0; p < PIECES; p++) {
-                        acc[i] = Op::mul(w, xs[p], acc[i]);
-                        sum[i] = Op::mul(ones, xs[p], sum[i]);
-                    }
+                for (int c = 0; c < GROUPS; c++) {
+                    int group = (read * 4 + c * (4 / GROUPS)) >> g.group_shift;
+                    if (group >= g.groups) group = g.groups - 1;        // (steps behind K, likewise)
+                    s[d][c] = *reinterpret_cast<const quad *>(S + group * padded_n);
+                    if (Z) z[d][c] = *reinterpret_cast<const quad *>(Z + group * padded_n);
                 }
-                const int group = step >> g.group_shift;
-                if ((f & LAST) == LAST && group < g.groups) {             // (steps behind K belong to no group)
-                    const quad s = *reinterpret_cast<const quad *>(S + group * padded_n + n0);
-                    pv4f z = pv4f{24.f, 24.f, 24.f, 24.f};
-                    if (Z) {
-                        const quad zz = *reinterpret_cast<const quad *>(Z + group * padded_n + n0);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) z[j] = 16.f + (float)zz[j];
-                    }
+                for (int f = 0; f < 4; f++)
 #pragma unroll
                     for (int i = 0; i < MT; i++)
+                        load_x<T, VEC>(xr, x, (uint32_t)(16 * i + r) * (uint32_t)g.ldx, m0 + 16 * i + r < m_end, (b * 4 + f) * 32 + kg * 8, g.K, xs[d][f][i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) y[i][j] += (float)s[j] * (acc[i][j] - z[j] * sum[i][j]);
+            for (int d = 0; d < DEEP; d++) {
+                pv4f acc[MT], sum[MT];
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    constexpr int LAST = 4 / GROUPS - 1;
+                    if ((f & LAST) == 0)
+#pragma unroll
+                        for (int i = 0; i < MT; i++) acc[i] = sum[i] = pv4f{0.f, 0.f, 0.f, 0.f};
+                    const uint32_t word = q[d][f];
+                    const pv4u w = pv4u{W4Type<T>::pair(word, 0), W4Type<T>::pair(word, 1), W4Type<T>::pair(word, 2), W4Type<T>::pair(word, 3)};
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        pv4u p[PIECES];
+                        pieces_of<T>(xs[d][f][i], p);
+#pragma unroll
+                        for (int c = 0; c < PIECES; c++) {
+                            acc[i] = Op::mul(w, p[c], acc[i]);
+                            sum[i] = Op::mul(ones, p[c], sum[i]);
+                        }
+                    }
+                    if ((f & LAST) == LAST) {
+                        const int c = f / (4 / GROUPS);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float zz = Z ? 16.f + (float)z[d][c][j] : 24.f;
+#pragma unroll
+                            for (int i = 0; i < MT; i++) y[i][j] += (float)s[d][c][j] * (acc[i][j] - zz * sum[i][j]);
+                        }
+                    }
                 }
             }
         }
-    if (WAVES > 1) {
-        if (wave > 0)
+    if (wave > 0)
 #pragma unroll
-            for (int i = 0; i < MT; i++) joint[wave - 1][i][lane] = y[i];
-        __syncthreads();
-        if (wave > 0) return;
+        for (int i = 0; i < MT; i++) joint[wave - 1][i][lane] = y[i];
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-        for (int w = 0; w < WAVES - 1; w++)
+    for (int w = 0; w < W4_WAVES - 1; w++)
 #pragma unroll
-            for (int i = 0; i < MT; i++) y[i] += joint[w][i][lane];
-    }
+        for (int i = 0; i < MT; i++) y[i] += joint[w][i][lane];
 #pragma unroll
     for (int i = 0; i < MT; i++) {
         const int m = m0 + 16 * i + r;
-        if (m >= m_end || (g.ids && r)) continue;
+        if (m >= m_end) continue;
         T *row = reinterpret_cast<T *>(g.y) + m * g.ldy;
+        typedef T quad_anywhere __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        if (n0 + 4 <= g.N) {
+            *reinterpret_cast<quad_anywhere *>(row + n0) = __builtin_convertvector(y[i], quad);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (n0 + j < g.N) row[n0 + j] = (T)y[i][j];
+            for (int j = 0; j < 4; j++)
+                if (n0 + j < g.N) row[n0 + j] = (T)y[i][j];
+        }
     }
 }
 
@@ -273,8 +304,8 @@ static int launch_w4(const W4Args &g, hipStream_t st) {
     const int64_t rows = g.ids ? g.M : (g.M + 16 * MT - 1) / (16 * MT);
     if (rows > 65535) return T2SP_ERR_SHAPE;
     const dim3 grid((unsigned)g.tiles_n, (unsigned)rows);
-    if (g.blocks_k >= 16) hipLaunchKernelGGL((gemv_w4_kernel<T, MT, 8, SHIFT>), grid, dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((gemv_w4_kernel<T, MT, 4, SHIFT>), grid, dim3(256), 0, st, g);
+    if (g.vec_x) hipLaunchKernelGGL((gemv_w4_kernel<T, MT, SHIFT, true>), grid, dim3(64 * W4_WAVES), 0, st, g);
+    else hipLaunchKernelGGL((gemv_w4_kernel<T, MT, SHIFT, false>), grid, dim3(64 * W4_WAVES), 0, st, g);
     return launched();
 }
 template <class T, int MT>
@@ -292,6 +323,7 @@ extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *
         return T2SP_ERR_SHAPE;
     if (M == 0) return T2SP_OK;
     if (!x || !Q || !S || !y || (!ids && E != 1)) return T2SP_ERR_SHAPE;
+    if (ldx * size > T2SP_MAX_ROW_BYTES) return T2SP_ERR_SHAPE;          // (64 rows of x within 31 bits)
     if (reinterpret_cast<uintptr_t>(Q) % 16 || reinterpret_cast<uintptr_t>(S) % 16 || reinterpret_cast<uintptr_t>(Z) % 16) return T2SP_ERR_SHAPE;
     W4Args g{};
     g.x = static_cast<const char *>(x); g.Q = static_cast<const uint8_t *>(Q);
@@ -302,11 +334,11 @@ extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *
     g.blocks_k = (int)(((int64_t)K + 127) / 128); g.tiles_n = (int)(((int64_t)N + 15) / 16);
     g.group_shift = group_shift_of(group);
     g.groups = (K + group - 1) / group;
-    g.vec_x = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0;
+    g.vec_x = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && (int64_t)K % 8 == 0;
     const hipStream_t st = (hipStream_t)stream;
     return with_types(type, type, [&](auto *t, auto *) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (ids || M <= 16) return launch_w4<T, 1>(g, st);
-        return M <= 32 ? launch_w4<T, 2>(g, st) : launch_w4<T, 4>(g, st);
+        return launch_w4<T, 4>(g, st);
     });
 }

@@ -14,6 +14,8 @@
 #include "product_core.hpp"
 #include "product_host.hpp"
 
+#include <algorithm>
+
 namespace t2sp {
 
 struct GroupedArgs {
@@ -24,7 +26,6 @@ struct GroupedArgs {
     int T, E, K, N;
     int64_t ldx, ldw, sw, ldy;           // in elements; sw: between matrices
     int col_tiles, xcds;
-    int vec_out;                         // rows of Y may be written 16 bytes at a time
 };
 
 __device__ __forceinline__ int group_edge(const GroupedArgs &g, int e) {
@@ -110,7 +111,142 @@ __global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int m = (wave / P::WN) * P::TM + 16 * i + (lane & 15);
-        if (m < t.rows) store_row<P, O>(g.Y + (t.row0 + m) * g.ldy * sizeof(O), n, g.N, acc[i], g.vec_out);
+        if (m < t.rows) store_row<P, O>(g.Y + (t.row0 + m) * g.ldy * sizeof(O), n, g.N, acc[i]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows per group
+// Decoding: a group has a handful of rows, and what takes time is reading its matrix once.  A workgroup owns up to 16 MT
+// rows of a group and a strip of columns; its eight waves take pieces of K in turn and are joined through LDS in a
+// fixed order.  The matrix goes from memory straight into MFMA operands, 8 loads of 16 bytes per lane in flight and two
+// or more workgroups per CU (a CU needs about 50 KB in flight to draw its share of HBM's rate):
+//   KMAJOR  32 columns; a lane's 16 bytes are k of its column, as the MFMA wants them; 256 bytes of a column per piece.
+//   KROWS   16 EPC columns (128 of 16 bits, 64 floats): lane l reads EPC columns of k rows EPC (l / 16) + 0 .. EPC - 1, a block
+//           that it transposes in its own registers (one v_perm per two elements; floats need none); accumulator tile j
+//           then has the columns congruent to j modulo EPC.
+// Rows that do not exist read as zeros without memory traffic, row tiles beyond the group's end are left out.
+// MEASURED_FEW_ROWS
+__device__ __forceinline__ pv4u load_or_zeros(__amdgpu_buffer_rsrc_t rsrc, uint32_t off, bool valid) {
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(valid ? off : OUT_OF_RANGE), 0, 0);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const char *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, 0x7fffffff, 0x00020000);
+}
+
+template <class T, int BS>
+struct FewRows {
+    static constexpr int SZ = sizeof(T), EPC = 16 / SZ, STEP = 64 / SZ;     // k per MFMA step
+    static constexpr int WAVES = 8, THREADS = 64 * WAVES;
+    static constexpr int NT = BS == KMAJOR ? 2 : EPC, COLS = 16 * NT;
+    static constexpr int STEPS = BS == KMAJOR ? 4 : SZ == 2 ? 1 : 2;        // per piece: 8 loads of the matrix
+    static constexpr int LDS = WAVES * 16 * COLS * 4;
+};
+
+template <class T, class O, int BS, int MT>
+__global__ void __launch_bounds__(512) grouped_few_rows_kernel(const GroupedArgs g) {
+    using F = FewRows<T, BS>;
+    constexpr int EPC = F::EPC, NT = F::NT, SZ = F::SZ;
+    __shared__ __attribute__((aligned(16))) float joint[F::WAVES][16][F::COLS];
+    GroupTile t;
+    if (!find_tile<16 * MT>(g, blockIdx.x, &t)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, kg = lane >> 4;
+    const int n0 = t.col_tile * F::COLS, rows = t.rows < 16 * MT ? t.rows : 16 * MT;
+    const char *x = g.X + t.row0 * g.ldx * SZ;
+    const char *w = g.W + t.group * g.sw * SZ + (BS == KMAJOR ? n0 * g.ldw : (int64_t)n0) * SZ;
+    const uint32_t ldx = (uint32_t)(g.ldx * SZ), ldw = (uint32_t)(g.ldw * SZ);
+    const __amdgpu_buffer_rsrc_t xr = buffer_at(x);
+    pv4f acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = pv4f{0.f, 0.f, 0.f, 0.f};
+    constexpr int PIECE = F::STEP * F::STEPS;
+    for (int k0 = wave * PIECE; k0 < g.K; k0 += F::WAVES * PIECE) {
+        pv4u b[F::STEPS][BS == KMAJOR ? NT : EPC], a[F::STEPS][MT];
+        if (BS == KMAJOR) {
+            const __amdgpu_buffer_rsrc_t wr = buffer_at(w + (int64_t)k0 * SZ);
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int s = 0; s < F::STEPS; s++)
+                    b[s][j] = load_or_zeros(wr, (uint32_t)(16 * j + r) * ldw + s * 64 + kg * 16, n0 + 16 * j + r < g.N && k0 + s * F::STEP + kg * EPC < g.K);
+        } else {
+            const __amdgpu_buffer_rsrc_t wr = buffer_at(w + (int64_t)k0 * ldw);
+#pragma unroll
+            for (int s = 0; s < F::STEPS; s++)
+#pragma unroll
+                for (int j = 0; j < EPC; j++) {
+                    const int k = s * F::STEP + kg * EPC + j;
+                    b[s][j] = load_or_zeros(wr, (uint32_t)k * ldw + r * 16, n0 + r * EPC < g.N && k0 + k < g.K);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int s = 0; s < F::STEPS; s++)
+                a[s][i] = load_or_zeros(xr, (uint32_t)(16 * i + r) * ldx + (uint32_t)k0 * SZ + s * 64 + kg * 16,
+                                        16 * i + r < rows && k0 + s * F::STEP + kg * EPC < g.K);
+        __builtin_amdgcn_sched_barrier(0);           // (every load is under way before the first is waited for)
+#pragma unroll
+        for (int s = 0; s < F::STEPS; s++) {
+            pv4u f[NT];
+            if constexpr (BS == KMAJOR) {
+#pragma unroll
+                for (int j = 0; j < NT; j++) f[j] = b[s][j];
+            } else if constexpr (SZ == 2) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+                        f[j][p] = __builtin_amdgcn_perm(b[s][2 * p + 1][j >> 1], b[s][2 * p][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int p = 0; p < 4; p++) f[j][p] = b[s][p][j];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                if (16 * i >= rows) break;
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[i][j] = MatrixOp<T>::mul(f[j], a[s][i], acc[i][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        if (16 * i >= rows) break;
+        if (i) __syncthreads();
+        // element e of tile j belongs to column 16 j + 4 kg + e (KMAJOR) or EPC (4 kg + e) + j (KROWS)
+        if (BS == KMAJOR) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) *reinterpret_cast<pv4f *>(&joint[wave][r][16 * j + 4 * kg]) = acc[i][j];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int j = 0; j < NT; j += 4)
+                    *reinterpret_cast<pv4f *>(&joint[wave][r][EPC * (4 * kg + e) + j]) = pv4f{acc[i][j][e], acc[i][j + 1 < NT ? j + 1 : 0][e],
+                                                                                              acc[i][j + 2 < NT ? j + 2 : 0][e], acc[i][j + 3 < NT ? j + 3 : 0][e]};
+        }
+        __syncthreads();
+        for (int q = threadIdx.x; q < 16 * F::COLS / 4; q += F::THREADS) {
+            const int row = q / (F::COLS / 4), c = q % (F::COLS / 4) * 4;
+            if (16 * i + row >= rows) continue;
+            pv4f sum = *reinterpret_cast<const pv4f *>(&joint[0][row][c]);
+#pragma unroll
+            for (int v = 1; v < F::WAVES; v++) sum += *reinterpret_cast<const pv4f *>(&joint[v][row][c]);
+            O *y = reinterpret_cast<O *>(g.Y + (t.row0 + 16 * i + row) * g.ldy * sizeof(O)) + n0 + c;
+            typedef O quad __attribute__((ext_vector_type(4)));
+            typedef O quad_anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
+            if (n0 + c + 4 <= g.N) {
+                *reinterpret_cast<quad_anywhere *>(y) = __builtin_convertvector(sum, quad);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (n0 + c + e < g.N) y[e] = (O)sum[e];
+            }
+        }
     }
 }
 
@@ -161,7 +297,7 @@ __global__ void __launch_bounds__(P::THREADS) grouped_wgrad_kernel(const Grouped
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int k = k0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
-        if (k < g.K) store_row<P, O>(g.Y + (e * g.sw + k * g.ldy) * (int64_t)sizeof(O), n, g.N, acc[i], g.vec_out);
+        if (k < g.K) store_row<P, O>(g.Y + (e * g.sw + k * g.ldy) * (int64_t)sizeof(O), n, g.N, acc[i]);
     }
 }
 
@@ -210,6 +346,15 @@ static int launch_forward(GroupedArgs g, hipStream_t stream) {
     return launched();
 }
 
+template <class T, class O, int BS, int MT>
+static int launch_few_rows(GroupedArgs g, hipStream_t stream) {
+    g.col_tiles = (g.N + FewRows<T, BS>::COLS - 1) / FewRows<T, BS>::COLS;
+    const int64_t blocks = (most_row_tiles(g.T, g.E, 16 * MT) * g.col_tiles + g.xcds - 1) / g.xcds * g.xcds;
+    if (blocks > 0x7fffffff / 512) return T2SP_ERR_SHAPE;
+    hipLaunchKernelGGL((grouped_few_rows_kernel<T, O, BS, MT>), dim3((unsigned)blocks), dim3(512), 0, stream, g);
+    return launched();
+}
+
 template <class P, class O>
 static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
     g.col_tiles = (g.N + P::BN - 1) / P::BN;
@@ -221,21 +366,39 @@ static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
     return launched();
 }
 
+// Groups are taken as equally large for these choices.  Beside the tiles' cost stands the time to read the matrices at the
+// rate each form reached on 0.5 GB of them (TB/s): the larger of the two and a quarter of the smaller.
 template <class T, class O, int BS>
 static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
-    const int64_t groups = g.E < g.T ? g.E : g.T, per = (g.T + groups - 1) / groups;
-    auto tiles = [&](int bm, int bn) { return groups * ((per + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
-    const double c256 = rounds_cost(tiles(256, 256), 1, 1.0), c128 = rounds_cost(tiles(128, 128), 2, 0.31),
-                 c64 = rounds_cost(tiles(64, 128), 3, 0.2);
-    if (c256 <= c128 && c256 <= c64) return launch_forward<Tile256<T, KMAJOR, BS>, O>(g, stream);
-    if (c128 <= c64) return launch_forward<Tile128<T, KMAJOR, BS>, O>(g, stream);
+    constexpr int size = sizeof(T), cols = FewRows<T, BS>::COLS;
+    constexpr bool kc = BS == KMAJOR;
+    const int64_t groups = g.E < g.T ? g.E : g.T, per = (g.T + groups - 1) / groups, k_bytes = (int64_t)g.K * size;
+    const double bytes = (double)groups * k_bytes * g.N;
+    auto cost = [&](const TileShape &s, double rate) {
+        const double c = tiles_cost(s, groups, per, g.N, k_bytes), h = bytes / (rate * 1e6);
+        return c > h ? c + 0.25 * h : h + 0.25 * c;
+    };
+    const double few1 = cost({16, cols, kc ? 0.06 : 0.14, kc ? 0.09 : 0.07}, kc ? 4.65 : 4.6),
+                 few2 = cost({32, cols, kc ? 0.06 : 0.14, kc ? 0.13 : 0.11}, kc ? 4.7 : 4.6),
+                 few4 = cost({64, cols, kc ? 0.06 : 0.14, kc ? 0.25 : 0.24}, kc ? 4.1 : 4.6);
+    const double c256 = size == 2 ? cost(SHAPE_256, kc ? 4.2 : 5.9) : 1e30, c128 = cost(size == 2 ? SHAPE_128 : SHAPE_128F, kc ? 4.7 : 5.6),
+                 c64 = cost(size == 2 ? SHAPE_64 : SHAPE_64F, kc ? 4.9 : 5.3);
+    const double best = std::min({few1, few2, few4, c256, c128, c64});
+    if (best == few1) return launch_few_rows<T, O, BS, 1>(g, stream);
+    if (best == few2) return launch_few_rows<T, O, BS, 2>(g, stream);
+    if (best == few4) return launch_few_rows<T, O, BS, 4>(g, stream);
+    if constexpr (size == 2)
+        if (best == c256) return launch_forward<Tile256<T, KMAJOR, BS>, O>(g, stream);
+    if (best == c128) return launch_forward<Tile128<T, KMAJOR, BS>, O>(g, stream);
     return launch_forward<Tile64<T, BS>, O>(g, stream);
 }
 
 template <class T, class O>
 static int wgrad_tiles(const GroupedArgs &g, hipStream_t stream) {
-    auto tiles = [&](int b) { return (int64_t)g.E * ((g.K + b - 1) / b) * ((g.N + b - 1) / b); };
-    if (rounds_cost(tiles(256), 1, 1.0) <= rounds_cost(tiles(128), 2, 0.31)) return launch_wgrad<Tile256<T, KROWS, KROWS>, O>(g, stream);
+    const int64_t per = (g.T + g.E - 1) / g.E;
+    const int tile = pick_tile(g.E, g.K, g.N, per, sizeof(T), false);
+    if constexpr (sizeof(T) == 2)
+        if (tile == 256) return launch_wgrad<Tile256<T, KROWS, KROWS>, O>(g, stream);
     return launch_wgrad<Tile128<T, KROWS, KROWS>, O>(g, stream);
 }
 
@@ -292,7 +455,6 @@ extern "C" int t2sp_gemm_grouped(int type, int out_type, int opb, const void *X,
     g.T = T; g.E = E; g.K = K; g.N = N;
     g.ldx = ldx; g.ldw = ldw; g.sw = sw; g.ldy = ldy;
     g.xcds = machine().xcds;
-    g.vec_out = writable_in_chunks(Y, ldy, N, out_type == T2SP_TYPE_F32 ? 4 : 2);
     return with_types(type, out_type, [&](auto *t, auto *o) {
         using TT = std::remove_pointer_t<decltype(t)>;
         using OO = std::remove_pointer_t<decltype(o)>;
@@ -342,8 +504,6 @@ extern "C" int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, co
     g.T = T; g.E = E; g.K = K; g.N = N;
     g.ldx = ldx; g.ldw = ldy; g.sw = sw; g.ldy = ldw;
     g.xcds = machine().xcds;
-    const int os = out_type == T2SP_TYPE_F32 ? 4 : 2;
-    g.vec_out = writable_in_chunks(dW, ldw, N, os) && sw * os % 16 == 0;
     return with_types(type, out_type, [&](auto *t, auto *o) {
         return wgrad_tiles<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, st);
     });

@@ -41,6 +41,12 @@ typedef short pv4s __attribute__((ext_vector_type(4)));
 
 enum : int { KMAJOR = 0, KROWS = 1 };
 
+// 16 bytes of elements, and the same for an address that is aligned to an element only.
+template <class O> struct Chunk {
+    typedef O type __attribute__((ext_vector_type(16 / sizeof(O))));
+    typedef O anywhere __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
+};
+
 template <class T> struct MatrixOp;
 template <> struct MatrixOp<__bf16> {
     typedef __bf16 frag __attribute__((ext_vector_type(8)));
@@ -109,6 +115,7 @@ struct ProductTile {
     static_assert(AS == KMAJOR || BM * SZ >= 256, "a KROWS tile row holds at least the sixteen chunks a key permutes");
     static_assert(BS == KMAJOR || BN * SZ >= 256, "a KROWS tile row holds at least the sixteen chunks a key permutes");
     static_assert(NT == 2 || NT == 4, "the B keys below are worked out for these");
+    static_assert(SZ == 2 || MT * NT <= 16, "floats keep two sets of sums in registers");
     static_assert(S >= 3 && (S - 1) * LOADS < 63, "the wait counter has six bits");
 
     // Column of B's operand row i in accumulator tile 0 (tile j: + 8 j).
@@ -274,7 +281,27 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
     typename P::Frags f0, f1;
     fetch(f0);
     const int stages = (k_len + P::KS - 1) / P::KS;
+    // Sums of floats are taken in runs of RUN stages (256 elements of k) that are added up on the vector units: the error of
+    // one running sum over k grows with sqrt(k), that of two levels with sqrt(256 + k / 256) (8192 of k: 1.0e-6 -> 3e-7
+    // of the result's norm).  Results of 16-bit operands are rounded far above that.
+    constexpr int RUN = 16;
+    constexpr bool TWO_LEVELS = P::SZ == 4;
+    pv4f whole[TWO_LEVELS ? P::MT : 1][TWO_LEVELS ? P::NT : 1];
+    if constexpr (TWO_LEVELS)
+#pragma unroll
+        for (int i = 0; i < P::MT; i++)
+#pragma unroll
+            for (int j = 0; j < P::NT; j++) whole[i][j] = pv4f{0.f, 0.f, 0.f, 0.f};
     for (int t = 0; t < stages; t += 2) {            // (an odd number of stages ends with one of zeros)
+        if constexpr (TWO_LEVELS)
+            if (t % RUN == 0)
+#pragma unroll
+                for (int i = 0; i < P::MT; i++)
+#pragma unroll
+                    for (int j = 0; j < P::NT; j++) {
+                        whole[i][j] += acc[i][j];
+                        acc[i][j] = pv4f{0.f, 0.f, 0.f, 0.f};
+                    }
         wait_loads<(P::S - 2) * P::LOADS>();          // stage t + 1 has landed
         wait_lds_reads();                             // this wave's operands of stage t are in registers:
         __builtin_amdgcn_s_barrier();                 // its buffer may be overwritten
@@ -286,6 +313,11 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
         issue();
         fetch_and_multiply(f0, f1);
     }
+    if constexpr (TWO_LEVELS)
+#pragma unroll
+        for (int i = 0; i < P::MT; i++)
+#pragma unroll
+            for (int j = 0; j < P::NT; j++) acc[i][j] += whole[i][j];
     wait_loads<0>();
     wait_lds_reads();
     __builtin_amdgcn_s_barrier();
@@ -326,7 +358,7 @@ __device__ __forceinline__ void swap_sixteens(pv4u &x, pv4u &y) {
 template <class P, class O, class F>
 __device__ __forceinline__ void row_chunks(int n, const pv4f (&acc)[P::NT], F f) {
     constexpr int CE = 16 / sizeof(O), C = P::LANE_N / CE;
-    typedef O chunk __attribute__((ext_vector_type(CE)));
+    typedef typename Chunk<O>::type chunk;
     pv4u v[C];
     const int kg = (threadIdx.x >> 4) & 3;
     if constexpr (sizeof(O) == 4) {                  // v[j]: chunks 2 j, 2 j + 1, 2 NT + 2 j, 2 NT + 2 j + 1 in the sixteens
@@ -353,22 +385,24 @@ __device__ __forceinline__ void row_chunks(int n, const pv4f (&acc)[P::NT], F f)
     }
 }
 
-// Row lane % 16 of accumulator row i to memory, columns below n_end, rounded to the output's type; `row` is the row's first
-// element, n the wave's first column.  `vec`: 16-byte stores are possible (n_end is then a whole number of chunks).
-template <class P, class O>
-__device__ __forceinline__ void store_row(char *row, int n, int n_end, const pv4f (&acc)[P::NT], bool vec) {
+// CE elements to p: one 16-byte store (memory takes it at any element's alignment), or those below n_end one by one.
+template <class O>
+__device__ __forceinline__ void store_chunk(O *p, int col, int n_end, typename Chunk<O>::type v) {
     constexpr int CE = 16 / sizeof(O);
-    typedef O chunk __attribute__((ext_vector_type(CE)));
-    O *p = reinterpret_cast<O *>(row);
-    row_chunks<P, O>(n, acc, [&](int col, chunk v) {
-        if (vec) {
-            if (col < n_end) *reinterpret_cast<chunk *>(p + col) = v;
-        } else {
+    if (col + CE <= n_end) {
+        *reinterpret_cast<typename Chunk<O>::anywhere *>(p + col) = v;
+    } else {
 #pragma unroll
-            for (int i = 0; i < CE; i++)
-                if (col + i < n_end) p[col + i] = v[i];
-        }
-    });
+        for (int i = 0; i < CE; i++)
+            if (col + i < n_end) p[col + i] = v[i];
+    }
+}
+
+// Row lane % 16 of accumulator row i to memory, columns below n_end, rounded to the output's type; `row` is the row's first
+// element, n the wave's first column.
+template <class P, class O>
+__device__ __forceinline__ void store_row(char *row, int n, int n_end, const pv4f (&acc)[P::NT]) {
+    row_chunks<P, O>(n, acc, [&](int col, typename Chunk<O>::type v) { store_chunk<O>(reinterpret_cast<O *>(row), col, n_end, v); });
 }
 
 template <class P>
@@ -380,12 +414,12 @@ __device__ __forceinline__ void clear(pv4f (&acc)[P::MT][P::NT]) {
 }
 
 
-// Tile shapes.  256 x 256 has the most arithmetic per byte from LDS and one workgroup per CU, whose 160 KB hold five
-// stages (8192 x 8192 x 2048, bfloat16, both operands k-contiguous: 282 us with four stages, 215 with five; k = 8192
-// with rows contiguous: 763 / 770 us, 1.43 PFLOP/s); 128 x 128 (two per CU) and 64 x 128 (three per CU) fill the chip
-// when there are few rows.
+// Tile shapes.  256 x 256 (16-bit) has the most arithmetic per byte from LDS and one workgroup per CU, whose 160 KB hold
+// five stages (8192 x 8192 x 2048, bfloat16, both operands k-contiguous: 282 us with four stages, 235 with five); the
+// smaller ones fill the chip when there are few rows or columns.  Floats, whose MFMAs are long, take two waves per SIMD
+// instead of large wave tiles (128 x 128 x 1024 alone on a CU: 77 us with four waves, 70 with eight), and a 64 x 64 tile.
 template <class T, int AS, int BS> using Tile256 = ProductTile<T, 256, 256, 2, 4, AS, BS, 5>;
-template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, 2, AS, BS, 5>;
-template <class T, int BS> using Tile64 = ProductTile<T, 64, 128, 1, 4, KMAJOR, BS, 4>;
+template <class T, int AS, int BS> using Tile128 = ProductTile<T, 128, 128, 2, sizeof(T) == 2 ? 2 : 4, AS, BS, 5>;
+template <class T, int BS> using Tile64 = ProductTile<T, 64, sizeof(T) == 2 ? 128 : 64, sizeof(T) == 2 ? 1 : 2, sizeof(T) == 2 ? 4 : 2, KMAJOR, BS, sizeof(T) == 2 ? 4 : 6>;
 
 }  // namespace t2sp

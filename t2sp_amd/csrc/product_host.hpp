@@ -38,14 +38,31 @@ template <class K> int allow_lds(K kern, int bytes) {
     return hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? T2SP_OK
                                                                                                                : T2SP_ERR_LAUNCH;
 }
-inline bool writable_in_chunks(const void *p, int64_t ld, int64_t cols, int size) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && cols * size % 16 == 0;
+// Time in microseconds of a product in tiles, for choosing among tile shapes: `tiles` workgroups share the CUs, n to a
+// CU, and a stage of 64 bytes of k then takes a + c n (fitted to sweeps of 1 to 1024 rows in 1 to 32 groups,
+// 2048 x 1024 to 4096 x 2048; what it picks is within a tenth of the best shape there but for a few sizes at the borders).
+struct TileShape {
+    int rows, cols;
+    double a, c;
+    int ends = 4;
+};
+constexpr TileShape SHAPE_256{256, 256, -0.2, 0.9, 10}, SHAPE_128{128, 128, 0.06, 0.335}, SHAPE_64{64, 128, 0.12, 0.21};
+constexpr TileShape SHAPE_128F{128, 128, 0.1, 1.02}, SHAPE_64F{64, 64, 0.12, 0.285};
+inline double tiles_cost(const TileShape &s, int64_t tiles, int64_t k_bytes) {
+    const int64_t cus = machine().cus, n = (tiles + cus - 1) / cus;
+    return (double)(k_bytes / 64 + s.ends) * (s.a + s.c * (double)n);
 }
-
-// Rounds of workgroups x time of one: the tile whose product ends first.  Groups are taken as equally large.
-inline double rounds_cost(int64_t tiles, int per_cu, double tile_time) {
-    const int64_t slots = (int64_t)machine().cus * per_cu;
-    return (double)((tiles + slots - 1) / slots) * per_cu * tile_time;
+inline double tiles_cost(const TileShape &s, int64_t groups, int64_t rows, int64_t cols, int64_t k_bytes) {
+    // (groups differ in size: a twentieth more row tiles than equal ones would make)
+    const int64_t row_tiles = groups * ((rows + s.rows - 1) / s.rows);
+    return tiles_cost(s, (row_tiles + (groups > 1 ? row_tiles / 20 + 1 : 0)) * ((cols + s.cols - 1) / s.cols), k_bytes);
+}
+// The tile edge for a product of `rows` x `cols`: 256, 128 or 64 (64 only where its operand layouts have that tile).
+inline int pick_tile(int64_t groups, int64_t rows, int64_t cols, int64_t k, int size, bool small = true) {
+    const double c256 = size == 2 ? tiles_cost(SHAPE_256, groups, rows, cols, k * size) : 1e30;
+    const double c128 = tiles_cost(size == 2 ? SHAPE_128 : SHAPE_128F, groups, rows, cols, k * size);
+    const double c64 = small ? tiles_cost(size == 2 ? SHAPE_64 : SHAPE_64F, groups, rows, cols, k * size) : 1e30;
+    return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
 }
 
 // f(element type, result type) as null pointers, for a pair that out_type_ok accepts.

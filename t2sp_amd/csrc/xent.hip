@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
             const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (v == hot ? 1.f : 0.f);
             acc[i][c / 4][c % 4] = valid && v < g.vp ? p * GradientScale<T>::value : 0.f;
         }
-        store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n0 + (wave % P::WN) * P::TN, (int)g.ldg, acc[i], true);
+        store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n0 + (wave % P::WN) * P::TN, (int)g.ldg, acc[i]);
     }
 }
 
@@ -240,7 +240,6 @@ struct XentProductArgs {
     int row_tiles, col_tiles, xcds;
     const float *scale;                  // dW: max |dloss|
     float by;
-    int vec_out;
     int splits;                          // dH: the reduction in this many parts, each with a plane of floats
     int64_t plane;
     int add;                             // dH: add to the planes (a later piece of the vocabulary)
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
         if (m >= g.rows) continue;
 #pragma unroll
         for (int j = 0; j < P::NT; j++) acc[i][j] *= by;
-        store_row<P, O>(g.out + m * g.ldo * (int64_t)sizeof(O), n, g.cols, acc[i], g.vec_out);
+        store_row<P, O>(g.out + m * g.ldo * (int64_t)sizeof(O), n, g.cols, acc[i]);
     }
 }
 
@@ -305,9 +304,10 @@ __global__ void __launch_bounds__(P::THREADS) xent_dh_kernel(const XentProductAr
 // dH[t, n] = dloss[t] * by * sum_s plane[s][t, n], zeros for tokens without a label.
 template <class O>
 __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, int splits, int64_t plane, int64_t ld, const void *labels, int lab64,
-                                                           const float *dloss, float by, int V, int D, O *dH, int64_t ldo, bool vec, int64_t chunks) {
+                                                           const float *dloss, float by, int V, int D, O *dH, int64_t ldo, int64_t chunks) {
     const int64_t per = ld / 4;
-    typedef O chunk __attribute__((ext_vector_type(4)));
+    typedef O quad __attribute__((ext_vector_type(4)));
+    typedef O quad_anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int t = (int)(i / per), n = (int)(i % per) * 4;
         const int64_t label = label_of(labels, lab64, t);
@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, 
             sum *= dloss[t] * by;
         }
         O *o = dH + t * ldo + n;
-        if (vec) {
-            *reinterpret_cast<chunk *>(o) = __builtin_convertvector(sum, chunk);
+        if (n + 4 <= D) {
+            *reinterpret_cast<quad_anywhere *>(o) = __builtin_convertvector(sum, quad);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -344,17 +344,14 @@ constexpr int64_t G_BYTES = 128 << 20;   // of the piece of p - [label]: it then
                                          // kernel and the two products that read it ...
 constexpr int MIN_PIECE = 4096;          // ... but a piece is long enough that adding up dH costs little beside it
 
-static int pick_tile(int64_t rows, int64_t cols) {
-    auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * ((cols + bn - 1) / bn); };
-    const double c256 = rounds_cost(tiles(256, 256), 1, 1.0), c128 = rounds_cost(tiles(128, 128), 2, 0.31), c64 = rounds_cost(tiles(64, 128), 3, 0.2);
-    return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
-}
+// Columns of the forward pass's tile.
+static int tile_cols(int tile, int size) { return tile == 64 && size == 2 ? 128 : tile; }
 
 // The tile of dH (the rows of T decide: its columns and the split fill the chip) and the parts of its reduction.
-static int dh_tile(int T) { return T > 128 ? 256 : T > 64 ? 128 : 64; }
-static int dh_splits(int T, int D, int piece) {
+static int dh_tile(int T, int size) { return T > 128 && size == 2 ? 256 : T > 64 ? 128 : 64; }
+static int dh_splits(int T, int D, int piece, int size) {
     if (T == 0) return 1;
-    const int bm = dh_tile(T), bn = bm == 256 ? 256 : 128, per_cu = bm == 256 ? 1 : bm == 128 ? 2 : 3;
+    const int bm = dh_tile(T, size), bn = tile_cols(bm, size), per_cu = bm == 256 ? 1 : bm == 128 ? 2 : 3;
     const int64_t tiles = (int64_t)((T + bm - 1) / bm) * ((D + bn - 1) / bn), slots = (int64_t)machine().cus * per_cu;
     int64_t s = slots / tiles;
     if (s > piece / 512) s = piece / 512;
@@ -374,8 +371,8 @@ static XentRoom xent_room(bool backward, int type, const void *H, const void *W,
     r.h = loadable(H, ldh, D, size) ? (size_t)-1 : take((size_t)T * r.ldd * size);
     r.w = loadable(W, ldw, D, size) ? (size_t)-1 : take((size_t)V * r.ldd * size);
     if (!backward) {
-        const int t = pick_tile(T, V);
-        r.part = take((size_t)((V + (t == 256 ? 255 : 127)) / (t == 256 ? 256 : 128)) * T * sizeof(float2));
+        const int cols = tile_cols(pick_tile(1, T, V, D, size), size);
+        r.part = take((size_t)((V + cols - 1) / cols) * T * sizeof(float2));
         r.hit = take((size_t)T * sizeof(float));
     } else {
         int64_t piece = G_BYTES / ((int64_t)(T > 0 ? T : 1) * size) / 256 * 256;
@@ -383,7 +380,7 @@ static XentRoom xent_room(bool backward, int type, const void *H, const void *W,
         if (piece >= V) piece = V;
         else piece = round_up((V + (V + piece - 1) / piece - 1) / ((V + piece - 1) / piece), 256);     // equal pieces
         r.piece = (int)piece;
-        r.splits = dh_splits(T, D, r.piece);
+        r.splits = dh_splits(T, D, r.piece, size);
         r.scale = take(sizeof(float));
         r.hz = take((size_t)T * r.ldd * size);
         r.g = take((size_t)T * padded_cols(piece, size) * size);
@@ -446,13 +443,16 @@ template <class P> static int launch_dh(XentProductArgs g, hipStream_t st) {
 }
 #undef T2SP_LAUNCH_TILES
 
+// The largest tile of a type (the choices above take 256 x 256 for 16-bit elements only).
+template <class T, int AS, int BS> using Large = std::conditional_t<sizeof(T) == 2, Tile256<T, AS, BS>, Tile128<T, AS, BS>>;
+
 template <class T>
 static int xent_forward(XentArgs g, float *loss, float *lse, hipStream_t st) {
-    const int tile = pick_tile(g.T, g.V);
-    int err = tile == 256 ? launch_stats<Tile256<T, KMAJOR, KMAJOR>>(g, st)
+    const int tile = pick_tile(1, g.T, g.V, g.D, sizeof(T)), cols = tile_cols(tile, sizeof(T));
+    int err = tile == 256 ? launch_stats<Large<T, KMAJOR, KMAJOR>>(g, st)
                           : tile == 128 ? launch_stats<Tile128<T, KMAJOR, KMAJOR>>(g, st) : launch_stats<Tile64<T, KMAJOR>>(g, st);
     if (err) return err;
-    const int tiles = tile == 256 ? (g.V + 255) / 256 : (g.V + 127) / 128;
+    const int tiles = (g.V + cols - 1) / cols;
     hipLaunchKernelGGL(xent_join_kernel, dim3((g.T + 63) / 64), dim3(64 * JOIN_WAVES), 0, st, g.part, g.hit, g.labels, g.lab64, g.T, g.V, tiles,
                        loss, lse);
     return launched();
@@ -482,8 +482,8 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
         g.G = room + r.g;
         g.ldg = padded_cols(g.vp, size);
         if (g.T) {
-            const int tile = pick_tile(g.T, g.vp);
-            err = tile == 256 ? launch_probabilities<Tile256<T, KMAJOR, KMAJOR>>(g, st)
+            const int tile = pick_tile(1, g.T, g.vp, g.D, size);
+            err = tile == 256 ? launch_probabilities<Large<T, KMAJOR, KMAJOR>>(g, st)
                               : tile == 128 ? launch_probabilities<Tile128<T, KMAJOR, KMAJOR>>(g, st) : launch_probabilities<Tile64<T, KMAJOR>>(g, st);
             if (err) return err;
         }
@@ -495,10 +495,8 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
             p.out = static_cast<char *>(dW) + v0 * lddw * (int64_t)sizeof(O); p.ldo = lddw;
             p.rows = g.vp; p.cols = g.D; p.k = g.T;
             p.scale = scale; p.by = by;
-            p.vec_out = writable_in_chunks(dW, lddw, g.D, sizeof(O));
-            auto tiles = [&](int b) { return (int64_t)((p.rows + b - 1) / b) * ((p.cols + b - 1) / b); };
-            err = rounds_cost(tiles(256), 1, 1.0) <= rounds_cost(tiles(128), 2, 0.31) ? launch_dw<Tile256<T, KROWS, KROWS>, O>(p, st)
-                                                                                      : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
+            err = pick_tile(1, p.rows, p.cols, p.k, size, false) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
+                                                                      : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
             if (err) return err;
         }
         if (dH && g.T) {
@@ -507,17 +505,16 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
             p.out = reinterpret_cast<char *>(planes); p.ldo = r.ldd; p.plane = (int64_t)g.T * r.ldd;
             p.rows = g.T; p.cols = g.D; p.k = g.vp;
             p.splits = r.splits; p.add = v0 > 0;
-            const int tile = dh_tile(g.T);
-            err = tile == 256 ? launch_dh<Tile256<T, KMAJOR, KROWS>>(p, st)
+            const int tile = dh_tile(g.T, size);
+            err = tile == 256 ? launch_dh<Large<T, KMAJOR, KROWS>>(p, st)
                               : tile == 128 ? launch_dh<Tile128<T, KMAJOR, KROWS>>(p, st) : launch_dh<Tile64<T, KROWS>>(p, st);
             if (err) return err;
         }
     }
     if (dH && g.T) {
         const int64_t chunks = (int64_t)g.T * r.ldd / 4;
-        const bool vec = reinterpret_cast<uintptr_t>(dH) % (4 * sizeof(O)) == 0 && lddh % 4 == 0 && g.D % 4 == 0 && r.ldd == g.D;
         hipLaunchKernelGGL(xent_dh_join_kernel<O>, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st, planes,
-                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, by, g.V, g.D, static_cast<O *>(dH), lddh, vec, chunks);
+                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, by, g.V, g.D, static_cast<O *>(dH), lddh, chunks);
         return launched();
     }
     return T2SP_OK;

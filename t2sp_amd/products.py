@@ -15,14 +15,23 @@ from ._lib import lib
 from .buffer import HalideBuffer
 from .ops import T2spError, _check, _is_torch, host_empty
 
-BAD_TYPE, SHAPE, BAD_DIMENSIONS, OUT_OF_BOUNDS, NULL_BUFFER = -3, -8, -43, -4, -12
-_codes = None
+BAD_TYPE, SHAPE, BAD_DIMENSIONS = -3, -8, -43
+_F32 = 0                                     # T2SP_TYPE_F32
+_codes = None                                # torch dtype -> T2SP_TYPE_*; set with the other torch names on first use
 
 
-def _type_codes():
-    global _codes
+def _torch():
+    """Names of torch that every call needs (the package itself imports without torch)."""
+    global _codes, _int_bits, _current_device, _set_device, _raw_stream, torch
     if _codes is None:
         import torch
+        _int_bits = {torch.int32: 32, torch.int64: 64}
+        # a call's cost on the host is a good part of a small product's: the plain numbers, where torch has them, save
+        # 2 us of the 4 that current_stream() and current_device() take
+        _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _set_device = torch.cuda.set_device
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        torch.cuda.init()
         _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     return _codes
 
@@ -34,35 +43,41 @@ def _need(op, ok, code=SHAPE):
 
 def _tensors(op, dims, *tensors):
     """Common checks of floating-point CUDA tensors: one element type, one device, the stated ranks, unit stride along
-    the last axis.  Returns the T2SP_TYPE_* code."""
+    the last axis.  Returns the T2SP_TYPE_* code and the device's index."""
     first = tensors[0]
-    code = _type_codes().get(first.dtype)
-    _need(op, code is not None, BAD_TYPE)
+    code, index = _torch().get(first.dtype), first.get_device()
+    if code is None:
+        raise T2spError(op, BAD_TYPE)
     for t, d in zip(tensors, dims):
-        _need(op, t.dtype == first.dtype, BAD_TYPE)
-        _need(op, t.dim() == d, BAD_DIMENSIONS)
-        _need(op, t.is_cuda and t.device == first.device)
-        _need(op, t.shape[-1] <= 1 or t.stride(-1) == 1)
-    return code
+        if t.dtype is not first.dtype:
+            raise T2spError(op, BAD_TYPE)
+        if t.dim() != d:
+            raise T2spError(op, BAD_DIMENSIONS)
+        if index < 0 or t.get_device() != index or (t.stride(-1) != 1 and t.shape[-1] > 1):
+            raise T2spError(op, SHAPE)
+    return code, index
 
 
-def _integers(op, t, like, n):
-    """Bits of a contiguous vector of n integers on the device of `like`."""
-    import torch
-    _need(op, t.dtype in (torch.int32, torch.int64), BAD_TYPE)
+def _vector(op, t, types, index, n):
+    """Checks a contiguous vector of n elements on the device; returns types[its dtype]."""
+    kind = types.get(t.dtype)
+    _need(op, kind is not None, BAD_TYPE)
     _need(op, t.dim() == 1, BAD_DIMENSIONS)
-    _need(op, t.device == like.device and t.shape[0] == n and (n <= 1 or t.stride(0) == 1))
-    return 32 if t.dtype == torch.int32 else 64
+    _need(op, t.get_device() == index and t.shape[0] == n and (n <= 1 or t.stride(0) == 1))
+    return kind
 
 
-def _result(op, out, shape, like, dtype, types):
-    import torch
+def _result(op, out, shape, like, dtype=None):
+    """(result, its T2SP_TYPE_*): `out` checked, or a fresh one of `dtype` (the type of `like`); that type or float32."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    _need(op, out.dtype in types, BAD_TYPE)
+        if dtype is None or dtype is like.dtype:
+            return like.new_empty(shape), _codes[like.dtype]
+        _need(op, dtype is torch.float32, BAD_TYPE)
+        return like.new_empty(shape, dtype=dtype), _F32
+    _need(op, out.dtype is like.dtype or out.dtype is torch.float32, BAD_TYPE)
     _need(op, out.dim() == len(shape), BAD_DIMENSIONS)
-    _need(op, tuple(out.shape) == tuple(shape) and out.device == like.device and (shape[-1] <= 1 or out.stride(-1) == 1))
-    return out
+    _need(op, tuple(out.shape) == shape and out.get_device() == like.get_device() and (shape[-1] <= 1 or out.stride(-1) == 1))
+    return out, _codes[out.dtype]
 
 
 def _row(t):
@@ -74,37 +89,22 @@ def _matrix(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * _row(t))
 
 
-class _On:
-    """Makes the tensors' device current around a call."""
-
-    def __init__(self, t):
-        import torch
-        self.index = t.device.index
-        self.back = torch.cuda.current_device()
-        self.set = torch.cuda.set_device
-
-    def __enter__(self):
-        if self.index != self.back:
-            self.set(self.index)
-
-    def __exit__(self, *exc):
-        if self.index != self.back:
-            self.set(self.back)
-
-
-def _stream(t):
-    import torch
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _room(nbytes, like):
-    """(pointer, bytes, owner) of a workspace.  The owner may be dropped after the call: torch's allocator hands the memory
-    out again only to work that is ordered behind it."""
-    if not nbytes:
-        return None, 0, None
-    import torch
-    t = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    return t.data_ptr(), nbytes, t
+def _enqueue(op, index, like, need, call):
+    """call(workspace, bytes, stream) on device `index`'s current stream, with `need` (a function, or None) bytes of
+    workspace.  The workspace's owner may be dropped after the call: torch's allocator hands the memory out again only to
+    work that is ordered behind it."""
+    back = _current_device()
+    if index != back:
+        _set_device(index)
+    try:
+        nbytes = need() if need else 0
+        room = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        code = call(room.data_ptr() if nbytes else None, nbytes, _raw_stream(index))
+    finally:
+        if index != back:
+            _set_device(back)
+    if code:
+        raise T2spError(op, code)
 
 
 def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
@@ -117,20 +117,22 @@ def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
     op = "gemm_grouped"
     if not _is_torch(X):
         return _host_grouped(op, X, W, offsets, opb, out)
-    import torch
-    code = _tensors(op, (2, 3), X, W)
-    T, K = X.shape
-    E, N = W.shape[0], W.shape[1] if opb else W.shape[2]
-    _need(op, (W.shape[2] if opb else W.shape[1]) == K and E >= 1 and K >= 1 and N >= 1)
-    bits = _integers(op, offsets, X, E + 1)
-    Y = _result(op, out, (T, N), X, out_dtype or X.dtype, (X.dtype, torch.float32))
-    _need(op, Y.dtype in (X.dtype, torch.float32), BAD_TYPE)
+    code, index = _tensors(op, (2, 3), X, W)
+    (T, K), (E, N) = X.shape, W.shape[:2]
+    opb = 1 if opb else 0
+    if opb:
+        _need(op, W.shape[2] == K)
+    else:
+        _need(op, N == K)
+        N = W.shape[2]
+    _need(op, E >= 1 and K >= 1 and N >= 1)
+    bits = _vector(op, offsets, _int_bits, index, E + 1)
+    Y, out_code = _result(op, out, (T, N), X, out_dtype)
     L = lib()
     x, w, ldx, ldw, sw = X.data_ptr(), W.data_ptr(), _row(X), _row(W), _matrix(W)
-    with _On(X):
-        ws, nbytes, owner = _room(L.t2sp_gemm_grouped_workspace_bytes(code, opb, x, w, T, E, K, N, ldx, ldw, sw), X)
-        _check(op, L.t2sp_gemm_grouped(code, _type_codes()[Y.dtype], opb, x, w, offsets.data_ptr(), bits, Y.data_ptr(), T, E, K, N,
-                                       ldx, ldw, sw, _row(Y), ws, nbytes, _stream(X)))
+    _enqueue(op, index, X, lambda: L.t2sp_gemm_grouped_workspace_bytes(code, opb, x, w, T, E, K, N, ldx, ldw, sw),
+             lambda ws, nbytes, stream: L.t2sp_gemm_grouped(code, out_code, opb, x, w, offsets.data_ptr(), bits, Y.data_ptr(), T, E, K, N,
+                                                            ldx, ldw, sw, _row(Y), ws, nbytes, stream))
     return Y
 
 
@@ -141,36 +143,30 @@ def gemm_grouped_wgrad(X, dY, offsets, out=None, out_dtype=None):
     op = "gemm_grouped_wgrad"
     if not _is_torch(X):
         return _host_wgrad(op, X, dY, offsets, out)
-    import torch
-    code = _tensors(op, (2, 2), X, dY)
+    code, index = _tensors(op, (2, 2), X, dY)
     T, K = X.shape
-    N, E = dY.shape[1], offsets.shape[0] - 1
+    N, E = dY.shape[1], offsets.shape[0] - 1 if offsets.dim() else 0
     _need(op, dY.shape[0] == T and E >= 1 and K >= 1 and N >= 1)
-    bits = _integers(op, offsets, X, E + 1)
-    dW = _result(op, out, (E, K, N), X, out_dtype or X.dtype, (X.dtype, torch.float32))
-    _need(op, dW.dtype in (X.dtype, torch.float32), BAD_TYPE)
+    bits = _vector(op, offsets, _int_bits, index, E + 1)
+    dW, out_code = _result(op, out, (E, K, N), X, out_dtype)
     L = lib()
     x, dy, ldx, ldy = X.data_ptr(), dY.data_ptr(), _row(X), _row(dY)
-    with _On(X):
-        ws, nbytes, owner = _room(L.t2sp_gemm_grouped_wgrad_workspace_bytes(code, x, dy, T, E, K, N, ldx, ldy), X)
-        _check(op, L.t2sp_gemm_grouped_wgrad(code, _type_codes()[dW.dtype], x, dy, offsets.data_ptr(), bits, dW.data_ptr(), T, E, K,
-                                             N, ldx, ldy, _row(dW), _matrix(dW), ws, nbytes, _stream(X)))
+    _enqueue(op, index, X, lambda: L.t2sp_gemm_grouped_wgrad_workspace_bytes(code, x, dy, T, E, K, N, ldx, ldy),
+             lambda ws, nbytes, stream: L.t2sp_gemm_grouped_wgrad(code, out_code, x, dy, offsets.data_ptr(), bits, dW.data_ptr(), T, E, K, N,
+                                                                  ldx, ldy, _row(dW), _matrix(dW), ws, nbytes, stream))
     return dW
 
 
 def _xent_args(op, H, W, labels):
-    code = _tensors(op, (2, 2), H, W)
+    code, index = _tensors(op, (2, 2), H, W)
     T, D = H.shape
     V = W.shape[0]
     _need(op, W.shape[1] == D and D >= 1 and V >= 1)
-    return code, T, V, D, _integers(op, labels, H, T)
+    return code, index, T, V, D, _vector(op, labels, _int_bits, index, T)
 
 
-def _floats(op, t, like, n):
-    import torch
-    _need(op, t.dtype == torch.float32, BAD_TYPE)
-    _need(op, t.dim() == 1, BAD_DIMENSIONS)
-    _need(op, t.device == like.device and t.shape[0] == n and (n <= 1 or t.stride(0) == 1))
+def _floats(op, t, index, n):
+    _vector(op, t, {torch.float32: 32}, index, n)
     return t
 
 
@@ -182,15 +178,14 @@ def xent(H, W, labels, loss=None, lse=None):
     op = "xent"
     if not _is_torch(H):
         return _host_xent(op, H, W, labels, loss, lse)
-    import torch
-    code, T, V, D, bits = _xent_args(op, H, W, labels)
-    loss = torch.empty(T, dtype=torch.float32, device=H.device) if loss is None else _floats(op, loss, H, T)
-    lse = torch.empty(T, dtype=torch.float32, device=H.device) if lse is None else _floats(op, lse, H, T)
+    code, index, T, V, D, bits = _xent_args(op, H, W, labels)
+    loss = H.new_empty(T, dtype=torch.float32) if loss is None else _floats(op, loss, index, T)
+    lse = H.new_empty(T, dtype=torch.float32) if lse is None else _floats(op, lse, index, T)
     L = lib()
     h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
-    with _On(H):
-        ws, nbytes, owner = _room(L.t2sp_xent_workspace_bytes(code, h, w, T, V, D, ldh, ldw), H)
-        _check(op, L.t2sp_xent(code, h, w, labels.data_ptr(), bits, loss.data_ptr(), lse.data_ptr(), T, V, D, ldh, ldw, ws, nbytes, _stream(H)))
+    _enqueue(op, index, H, lambda: L.t2sp_xent_workspace_bytes(code, h, w, T, V, D, ldh, ldw),
+             lambda ws, nbytes, stream: L.t2sp_xent(code, h, w, labels.data_ptr(), bits, loss.data_ptr(), lse.data_ptr(), T, V, D, ldh, ldw, ws,
+                                                    nbytes, stream))
     return loss, lse
 
 
@@ -203,22 +198,26 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
     op = "xent_grad"
     if not _is_torch(H):
         return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW, wanted)
-    import torch
-    code, T, V, D, bits = _xent_args(op, H, W, labels)
-    _floats(op, lse, H, T)
-    _floats(op, dloss, H, T)
-    types = (H.dtype, torch.float32)
-    dtype = out_dtype or (dH.dtype if dH is not None else dW.dtype if dW is not None else H.dtype)
-    dH = _result(op, dH, (T, D), H, dtype, types) if wanted[0] or dH is not None else None
-    dW = _result(op, dW, (V, D), H, dtype, types) if wanted[1] or dW is not None else None
-    _need(op, dtype in types and all(t is None or t.dtype == dtype for t in (dH, dW)), BAD_TYPE)
+    code, index, T, V, D, bits = _xent_args(op, H, W, labels)
+    _floats(op, lse, index, T)
+    _floats(op, dloss, index, T)
+    out_code = None
+    dtype = out_dtype or (dH.dtype if dH is not None else dW.dtype if dW is not None else None)
+    if wanted[0] or dH is not None:
+        dH, out_code = _result(op, dH, (T, D), H, dtype)
+    if wanted[1] or dW is not None:
+        dW, other = _result(op, dW, (V, D), H, dtype)
+        _need(op, out_code in (None, other), BAD_TYPE)
+        out_code = other
+    if out_code is None:
+        return None, None
     L = lib()
     h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
-    with _On(H):
-        ws, nbytes, owner = _room(L.t2sp_xent_grad_workspace_bytes(code, h, w, T, V, D, ldh, ldw), H)
-        _check(op, L.t2sp_xent_grad(code, _type_codes()[dtype], h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
-                                    dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None, T, V, D, ldh, ldw,
-                                    _row(dH) if dH is not None else D, _row(dW) if dW is not None else D, ws, nbytes, _stream(H)))
+    _enqueue(op, index, H, lambda: L.t2sp_xent_grad_workspace_bytes(code, h, w, T, V, D, ldh, ldw),
+             lambda ws, nbytes, stream: L.t2sp_xent_grad(code, out_code, h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
+                                                         dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None,
+                                                         T, V, D, ldh, ldw, _row(dH) if dH is not None else D, _row(dW) if dW is not None else D,
+                                                         ws, nbytes, stream))
     return dH, dW
 
 
@@ -227,7 +226,8 @@ class W4:
 
     def __init__(self, E, N, K, group, Q, S, Z):
         self.E, self.N, self.K, self.group, self.Q, self.S, self.Z = E, N, K, group, Q, S, Z
-        self.code = _type_codes()[S.dtype]
+        self.dtype, self.code, self.index = S.dtype, _torch()[S.dtype], S.get_device()
+        self.pointers = Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None
 
 
 def pack_w4(q, scales, zeros=None, group=128):
@@ -237,12 +237,11 @@ def pack_w4(q, scales, zeros=None, group=128):
     q: uint8 (N, K), or (E, N, K) for E matrices, one number in the low four bits of each byte; scales, zeros:
     (..., N, ceil(K / group)) of the type of the rows they will meet (float32, float16 or bfloat16).  group: a power of two
     from 32 on; at least K for one scale per row."""
-    import torch
     op = "pack_w4"
-    _need(op, q.dtype == torch.uint8, BAD_TYPE)
+    code, index = _tensors(op, (q.dim(),) * 2, *((scales,) if zeros is None else (scales, zeros)))
+    _need(op, q.dtype is torch.uint8, BAD_TYPE)
     _need(op, q.dim() in (2, 3), BAD_DIMENSIONS)
-    _need(op, q.is_cuda and (q.shape[-1] <= 1 or q.stride(-1) == 1))
-    code = _tensors(op, (q.dim(),) * 2, *((scales,) if zeros is None else (scales, zeros)))
+    _need(op, q.get_device() == index and (q.shape[-1] <= 1 or q.stride(-1) == 1))
     N, K = q.shape[-2:]
     group = int(group)
     qb, se = ctypes.c_int64(), ctypes.c_int64()
@@ -250,16 +249,16 @@ def pack_w4(q, scales, zeros=None, group=128):
     _check(op, L.t2sp_w4_sizes(N, K, group, ctypes.byref(qb), ctypes.byref(se)))
     E = q.shape[0] if q.dim() == 3 else 1
     want = tuple(q.shape[:-1]) + (-(-K // group),)
-    _need(op, E >= 1 and tuple(scales.shape) == want and (zeros is None or tuple(zeros.shape) == want) and scales.device == q.device)
-    Q = torch.empty(E * qb.value, dtype=torch.uint8, device=q.device)
-    S = torch.empty(E * se.value, dtype=scales.dtype, device=q.device)
+    _need(op, E >= 1 and tuple(scales.shape) == want and (zeros is None or tuple(zeros.shape) == want))
+    Q = q.new_empty(E * qb.value)
+    S = scales.new_empty(E * se.value)
     Z = torch.empty_like(S) if zeros is not None else None
     each = lambda t: _matrix(t) if t.dim() == 3 else 0
-    with _On(q):
-        _check(op, L.t2sp_w4_pack(code, q.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, E, N, K, group,
-                                  _row(q), each(q), _row(scales), each(scales), _row(zeros) if zeros is not None else 0,
-                                  each(zeros) if zeros is not None else 0, Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None,
-                                  _stream(q)))
+    _enqueue(op, index, q, None,
+             lambda ws, nbytes, stream: L.t2sp_w4_pack(code, q.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, E, N,
+                                                       K, group, _row(q), each(q), _row(scales), each(scales),
+                                                       _row(zeros) if zeros is not None else 0, each(zeros) if zeros is not None else 0,
+                                                       Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None, stream))
     return W4(E if q.dim() == 3 else None, N, K, group, Q, S, Z)
 
 
@@ -267,18 +266,22 @@ def gemv_w4(x, w, ids=None, out=None):
     """y = x @ W.T for a few rows x (M, K) and 4-bit weights w (pack_w4), y (M, N) of x's type.
 
     With matrices for E experts, ids (M int32) picks the matrix of each row; a row whose id is outside 0 .. E - 1 is zeros."""
-    import torch
     op = "gemv_w4"
-    _need(op, x.dtype == w.S.dtype, BAD_TYPE)
+    _need(op, x.dtype is w.dtype, BAD_TYPE)
     _need(op, x.dim() == 2, BAD_DIMENSIONS)
     M, K = x.shape
-    _need(op, K == w.K and x.is_cuda and x.device == w.Q.device and (K <= 1 or x.stride(1) == 1) and (ids is None) == (w.E is None))
+    index = w.index
+    _need(op, K == w.K and x.get_device() == index and (x.stride(1) == 1 or K <= 1) and (ids is None) == (w.E is None))
     if ids is not None:
-        _need(op, ids.dtype == torch.int32, BAD_TYPE)
-        _integers(op, ids, x, M)
-    y = _result(op, out, (M, w.N), x, x.dtype, (x.dtype,))
-    with _On(x):
-        _check(op, lib().t2sp_gemv_w4(w.code, x.data_ptr(), w.Q.data_ptr(), w.S.data_ptr(), w.Z.data_ptr() if w.Z is not None else None,
-                                      ids.data_ptr() if ids is not None else None, y.data_ptr(), M, w.N, K, w.E or 1, w.group, _row(x), _row(y),
-                                      _stream(x)))
+        _vector(op, ids, {torch.int32: 32}, index, M)
+    if out is None:
+        y, ldy = x.new_empty((M, w.N)), w.N
+    else:
+        _need(op, out.dtype is x.dtype, BAD_TYPE)
+        y, _ = _result(op, out, (M, w.N), x)
+        ldy = _row(y)
+    Q, S, Z = w.pointers
+    _enqueue(op, index, x, None,
+             lambda ws, nbytes, stream: lib().t2sp_gemv_w4(w.code, x.data_ptr(), Q, S, Z, ids.data_ptr() if ids is not None else None, y.data_ptr(),
+                                                           M, w.N, K, w.E or 1, w.group, _row(x), ldy, stream))
     return y
