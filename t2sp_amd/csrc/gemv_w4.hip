@@ -16,7 +16,9 @@
 // Layout (t2sp_w4_pack, made once from plain numbers): blocks of 16 rows x 128 inputs, 1 KB, in which the 16 bytes of
 // lane l are what that lane feeds to four MFMAs: row l % 16, inputs 32 f + 8 (l / 16) + 0..7 for f = 0..3; in a word the
 // inputs 2 p and 2 p + 1 lie at bits 4 p and 4 p + 16.  A wave reads a block with one 16-byte load per lane, and any N
-// and K become whole blocks (numbers behind K meet zeros of x).  Scales and zero points: [group][row], rows padded to 16.
+// and K become whole blocks (numbers behind K meet zeros of x).  Scales and zero points lie in the order in which a lane
+// needs them: [tile of 16 rows][block][rows by fours][group of the block][four rows], the block's 4, 2 or 1 groups together
+// (with [group][row] a block of 32-input groups took eight loads besides that of its numbers, and 8192 x 4096 13 us).
 //
 // One workgroup owns 16 * NT rows of the matrix and up to 16 * MT rows of x; its waves take the blocks of K in turn and
 // are joined through LDS in a fixed order.
@@ -35,7 +37,7 @@ struct W4Args {
     int64_t ldx, ldy;                    // elements
     int blocks_k, tiles_n;               // of 128 inputs, of 16 rows
     int group_shift;                     // G = 32 << group_shift
-    int groups;
+    int groups, group_blocks;            // in K; blocks of scales (of 4, 2 or 1 groups)
     int vec_x;                           // rows of x are whole 16-byte chunks
 };
 
@@ -106,23 +108,26 @@ __device__ __forceinline__ void pieces_of(const pv4u (&raw)[sizeof(T) / 2], pv4u
     }
 }
 
-// MT: tiles of 16 rows of x.  SHIFT: a group has 32 << SHIFT of a block's inputs (the whole block for groups of 128 and more).
+// MT: tiles of 16 rows of x, NT: of the matrix.  With many rows of x a workgroup takes several tiles of the matrix, which then
+// share what it reads of x (16 rows of 4096 halves are 128 KB, four times a 16-row tile's numbers: 16384 x 4096 with 16 rows takes
+// MEASURED_NT).  SHIFT: a group has 32 << SHIFT of a block's inputs (the whole block for groups of 128 and more).
 // A wave has DEEP blocks of the matrix, their scales and their part of x under way before it waits for the first.
 constexpr int W4_WAVES = 8;
-template <class T, int MT, int SHIFT, bool VEC>
+template <class T, int MT, int NT, int SHIFT, bool VEC>
 __global__ void __launch_bounds__(64 * W4_WAVES) gemv_w4_kernel(const W4Args g) {
     using Op = MatrixOp<typename W4Type<T>::M>;
-    constexpr int PIECES = W4Type<T>::PIECES, DEEP = MT * sizeof(T) <= 2 ? 4 : MT * sizeof(T) <= 4 ? 2 : 1;
+    constexpr int PIECES = W4Type<T>::PIECES, DEEP = MT * NT * sizeof(T) <= 2 ? 4 : MT * sizeof(T) <= 4 ? 2 : 1;
     constexpr int GROUPS = SHIFT == 0 ? 4 : SHIFT == 1 ? 2 : 1;         // of a block
     typedef T quad __attribute__((ext_vector_type(4)));
-    __shared__ __attribute__((aligned(16))) pv4f joint[W4_WAVES - 1][MT][64];
+    typedef T quads __attribute__((ext_vector_type(4 * GROUPS)));
+    __shared__ __attribute__((aligned(16))) pv4f joint[W4_WAVES - 1][MT * NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, kg = lane >> 4;
-    const int tile = blockIdx.x, n0 = tile * 16 + 4 * kg;              // this lane ends with rows n0 .. n0 + 3 of x row r
+    const int tile = blockIdx.x * NT, n0 = tile * 16 + 4 * kg;         // this lane ends with rows n0 .. n0 + 3 (+ 16 per tile) of x row r
     int m0 = blockIdx.y * 16 * MT, m_end = g.M;
     const uint8_t *Q = g.Q;
     const T *S = reinterpret_cast<const T *>(g.S), *Z = reinterpret_cast<const T *>(g.Z);
-    const int64_t padded_n = (int64_t)g.tiles_n * 16;
+    const int64_t side = (int64_t)g.tiles_n * 16 * g.group_blocks * GROUPS;       // elements of S and of Z per matrix
     bool matrix = true;
     if (g.ids) {                                                        // one row of x per workgroup
         m0 = blockIdx.y;
@@ -131,33 +136,39 @@ __global__ void __launch_bounds__(64 * W4_WAVES) gemv_w4_kernel(const W4Args g) 
         matrix = e >= 0 && e < g.E;
         const int64_t at = matrix ? e : 0;
         Q += at * g.tiles_n * g.blocks_k * 1024;
-        S += at * g.groups * padded_n;
-        if (Z) Z += at * g.groups * padded_n;
+        S += at * side;
+        if (Z) Z += at * side;
     }
-    Q += (int64_t)tile * g.blocks_k * 1024 + lane * 16;
-    S += n0;
-    if (Z) Z += n0;
+    Q += lane * 16;
+    S += kg * GROUPS * 4;
+    if (Z) Z += kg * GROUPS * 4;
+    int64_t tile_q[NT], tile_s[NT];                                     // (tiles behind the last one repeat it and are not stored)
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int own = tile + t < g.tiles_n ? tile + t : g.tiles_n - 1;
+        tile_q[t] = (int64_t)own * g.blocks_k * 1024;
+        tile_s[t] = (int64_t)own * g.group_blocks;
+    }
     const T *x = reinterpret_cast<const T *>(g.x) + (int64_t)m0 * g.ldx;
     const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(x), 0, 0x7fffffff, 0x00020000);
-    pv4f y[MT];
+    pv4f y[MT * NT];
 #pragma unroll
-    for (int i = 0; i < MT; i++) y[i] = pv4f{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MT * NT; i++) y[i] = pv4f{0.f, 0.f, 0.f, 0.f};
     const pv4u ones = pv4u{W4Type<T>::ONES, W4Type<T>::ONES, W4Type<T>::ONES, W4Type<T>::ONES};
 
     if (matrix)
         for (int b0 = wave; b0 < g.blocks_k; b0 += DEEP * W4_WAVES) {
-            pv4u q[DEEP], xs[DEEP][4][MT][sizeof(T) / 2];
-            quad s[DEEP][GROUPS], z[DEEP][GROUPS];
+            pv4u q[DEEP][NT], xs[DEEP][4][MT][sizeof(T) / 2];
+            quads s[DEEP][NT], z[DEEP][NT];
 #pragma unroll
             for (int d = 0; d < DEEP; d++) {                            // (blocks behind the last one repeat it against zeros)
                 const int b = b0 + d * W4_WAVES, read = b < g.blocks_k ? b : g.blocks_k - 1;
-                q[d] = __builtin_nontemporal_load(reinterpret_cast<const pv4u *>(Q + (int64_t)read * 1024));
 #pragma unroll
-                for (int c = 0; c < GROUPS; c++) {
-                    int group = (read * 4 + c * (4 / GROUPS)) >> g.group_shift;
-                    if (group >= g.groups) group = g.groups - 1;        // (steps behind K, likewise)
-                    s[d][c] = *reinterpret_cast<const quad *>(S + group * padded_n);
-                    if (Z) z[d][c] = *reinterpret_cast<const quad *>(Z + group * padded_n);
+                for (int t = 0; t < NT; t++) {
+                    q[d][t] = __builtin_nontemporal_load(reinterpret_cast<const pv4u *>(Q + tile_q[t] + (int64_t)read * 1024));
+                    const int64_t at = (tile_s[t] + (SHIFT == 2 ? (read * 4) >> g.group_shift : read)) * (16 * GROUPS);
+                    s[d][t] = *reinterpret_cast<const quads *>(S + at);
+                    if (Z) z[d][t] = *reinterpret_cast<const quads *>(Z + at);
                 }
 #pragma unroll
                 for (int f = 0; f < 4; f++)
@@ -168,58 +179,71 @@ __global__ void __launch_bounds__(64 * W4_WAVES) gemv_w4_kernel(const W4Args g) 
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int d = 0; d < DEEP; d++) {
-                pv4f acc[MT], sum[MT];
+                pv4f acc[MT * NT], sum[MT];
 #pragma unroll
                 for (int f = 0; f < 4; f++) {
                     constexpr int LAST = 4 / GROUPS - 1;
-                    if ((f & LAST) == 0)
+                    if ((f & LAST) == 0) {
 #pragma unroll
-                        for (int i = 0; i < MT; i++) acc[i] = sum[i] = pv4f{0.f, 0.f, 0.f, 0.f};
-                    const uint32_t word = q[d][f];
-                    const pv4u w = pv4u{W4Type<T>::pair(word, 0), W4Type<T>::pair(word, 1), W4Type<T>::pair(word, 2), W4Type<T>::pair(word, 3)};
+                        for (int i = 0; i < MT; i++) sum[i] = pv4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < MT * NT; i++) acc[i] = pv4f{0.f, 0.f, 0.f, 0.f};
+                    }
+                    pv4u p[MT][PIECES];
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
-                        pv4u p[PIECES];
-                        pieces_of<T>(xs[d][f][i], p);
+                        pieces_of<T>(xs[d][f][i], p[i]);
 #pragma unroll
-                        for (int c = 0; c < PIECES; c++) {
-                            acc[i] = Op::mul(w, p[c], acc[i]);
-                            sum[i] = Op::mul(ones, p[c], sum[i]);
-                        }
+                        for (int c = 0; c < PIECES; c++) sum[i] = Op::mul(ones, p[i][c], sum[i]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const uint32_t word = q[d][t][f];
+                        const pv4u w = pv4u{W4Type<T>::pair(word, 0), W4Type<T>::pair(word, 1), W4Type<T>::pair(word, 2), W4Type<T>::pair(word, 3)};
+#pragma unroll
+                        for (int i = 0; i < MT; i++)
+#pragma unroll
+                            for (int c = 0; c < PIECES; c++) acc[i * NT + t] = Op::mul(w, p[i][c], acc[i * NT + t]);
                     }
                     if ((f & LAST) == LAST) {
                         const int c = f / (4 / GROUPS);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float zz = Z ? 16.f + (float)z[d][c][j] : 24.f;
+                        for (int t = 0; t < NT; t++)
 #pragma unroll
-                            for (int i = 0; i < MT; i++) y[i][j] += (float)s[d][c][j] * (acc[i][j] - zz * sum[i][j]);
-                        }
+                            for (int j = 0; j < 4; j++) {
+                                const float zz = Z ? 16.f + (float)z[d][t][4 * c + j] : 24.f;
+#pragma unroll
+                                for (int i = 0; i < MT; i++) y[i * NT + t][j] += (float)s[d][t][4 * c + j] * (acc[i * NT + t][j] - zz * sum[i][j]);
+                            }
                     }
                 }
             }
         }
     if (wave > 0)
 #pragma unroll
-        for (int i = 0; i < MT; i++) joint[wave - 1][i][lane] = y[i];
+        for (int i = 0; i < MT * NT; i++) joint[wave - 1][i][lane] = y[i];
     __syncthreads();
     if (wave > 0) return;
 #pragma unroll
-    for (int w = 0; w < W4_WAVES - 1; w++)
+    for (int i = 0; i < MT * NT; i++)
 #pragma unroll
-        for (int i = 0; i < MT; i++) y[i] += joint[w][i][lane];
+        for (int w = 0; w < W4_WAVES - 1; w++) y[i] += joint[w][i][lane];
 #pragma unroll
     for (int i = 0; i < MT; i++) {
         const int m = m0 + 16 * i + r;
         if (m >= m_end) continue;
         T *row = reinterpret_cast<T *>(g.y) + m * g.ldy;
         typedef T quad_anywhere __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-        if (n0 + 4 <= g.N) {
-            *reinterpret_cast<quad_anywhere *>(row + n0) = __builtin_convertvector(y[i], quad);
-        } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (n0 + j < g.N) row[n0 + j] = (T)y[i][j];
+        for (int t = 0; t < NT; t++) {
+            const int n = n0 + 16 * t;
+            if (n + 4 <= g.N) {
+                *reinterpret_cast<quad_anywhere *>(row + n) = __builtin_convertvector(y[i * NT + t], quad);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (n + j < g.N) row[n + j] = (T)y[i * NT + t][j];
+            }
         }
     }
 }
@@ -239,12 +263,15 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t *q, int N, i
     }
 }
 
-// dst[e][g][n] = src[e][n][g], zeros for n from N to the padded rows.
+// dst in the kernel's order (see above), zeros for rows from N and groups behind the last.
 template <class T>
-__global__ void __launch_bounds__(256) w4_scales_kernel(const T *src, int N, int groups, int64_t ld, int64_t stride, int64_t padded_n, int64_t total, T *dst) {
+__global__ void __launch_bounds__(256) w4_scales_kernel(const T *src, int N, int groups, int64_t ld, int64_t stride, int tiles_n, int group_blocks, int per_block,
+                                                        int64_t total, T *dst) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t n = i % padded_n, g = i / padded_n % groups, e = i / padded_n / groups;
-        dst[i] = n < N ? src[e * stride + n * ld + g] : (T)0;
+        const int64_t j = i & 3, c = (i >> 2) % per_block, rest = (i >> 2) / per_block, kg = rest & 3, b = (rest >> 2) % group_blocks,
+                      t = (rest >> 2) / group_blocks % tiles_n, e = (rest >> 2) / group_blocks / tiles_n;
+        const int64_t n = t * 16 + kg * 4 + j, g = b * per_block + c;
+        dst[i] = n < N && g < groups ? src[e * stride + n * ld + g] : (T)0;
     }
 }
 
@@ -252,6 +279,13 @@ static int group_shift_of(int group) {
     for (int s = 0; s <= 25; s++)
         if (group == 32 << s) return s;
     return -1;
+}
+
+// Groups of a block of 128 inputs, and the blocks of scales that K makes.
+static int groups_per_block(int group) { return group == 32 ? 4 : group == 64 ? 2 : 1; }
+static int64_t group_blocks_of(int K, int group) {
+    const int64_t span = (int64_t)group * groups_per_block(group);
+    return (K + span - 1) / span;
 }
 
 static unsigned blocks_for(int64_t n) { return (unsigned)(n < 256 * 65536 ? (n + 255) / 256 : 65536); }
@@ -264,7 +298,7 @@ extern "C" int t2sp_w4_sizes(int N, int K, int group, int64_t *q_bytes, int64_t 
     if (!extent_ok(N) || !extent_ok(K) || group_shift_of(group) < 0 || !q_bytes || !scale_elements) return T2SP_ERR_SHAPE;
     const int64_t tiles_n = ((int64_t)N + 15) / 16, blocks_k = ((int64_t)K + 127) / 128;
     *q_bytes = tiles_n * blocks_k * 1024;
-    *scale_elements = ((int64_t)K + group - 1) / group * tiles_n * 16;
+    *scale_elements = tiles_n * 16 * group_blocks_of(K, group) * groups_per_block(group);
     return T2SP_OK;
 }
 
@@ -289,28 +323,48 @@ extern "C" int t2sp_w4_pack(int type, const uint8_t *q, const void *scales, cons
         const int64_t ld = i ? ldz : lds, stride = i ? sz : ss;
         if (size == 4)
             hipLaunchKernelGGL(w4_scales_kernel<uint32_t>, dim3(blocks_for(total)), dim3(256), 0, st, static_cast<const uint32_t *>(from), N, groups, ld,
-                               stride, padded_n, total, static_cast<uint32_t *>(to));
+                               stride, (int)(padded_n / 16), (int)group_blocks_of(K, group), groups_per_block(group), total, static_cast<uint32_t *>(to));
         else
             hipLaunchKernelGGL(w4_scales_kernel<uint16_t>, dim3(blocks_for(total)), dim3(256), 0, st, static_cast<const uint16_t *>(from), N, groups, ld,
-                               stride, padded_n, total, static_cast<uint16_t *>(to));
+                               stride, (int)(padded_n / 16), (int)group_blocks_of(K, group), groups_per_block(group), total, static_cast<uint16_t *>(to));
         if (int err = launched()) return err;
     }
     return T2SP_OK;
 }
 
 namespace t2sp {
-template <class T, int MT, int SHIFT>
+template <class T, int MT, int NT, int SHIFT, bool VEC>
 static int launch_w4(const W4Args &g, hipStream_t st) {
     const int64_t rows = g.ids ? g.M : (g.M + 16 * MT - 1) / (16 * MT);
     if (rows > 65535) return T2SP_ERR_SHAPE;
-    const dim3 grid((unsigned)g.tiles_n, (unsigned)rows);
-    if (g.vec_x) hipLaunchKernelGGL((gemv_w4_kernel<T, MT, SHIFT, true>), grid, dim3(64 * W4_WAVES), 0, st, g);
-    else hipLaunchKernelGGL((gemv_w4_kernel<T, MT, SHIFT, false>), grid, dim3(64 * W4_WAVES), 0, st, g);
+    hipLaunchKernelGGL((gemv_w4_kernel<T, MT, NT, SHIFT, VEC>), dim3((unsigned)((g.tiles_n + NT - 1) / NT), (unsigned)rows), dim3(64 * W4_WAVES), 0, st, g);
     return launched();
 }
-template <class T, int MT>
+template <class T, int MT, int NT, bool VEC>
 static int launch_w4(const W4Args &g, hipStream_t st) {
-    return g.group_shift == 0 ? launch_w4<T, MT, 0>(g, st) : g.group_shift == 1 ? launch_w4<T, MT, 1>(g, st) : launch_w4<T, MT, 2>(g, st);
+    return g.group_shift == 0 ? launch_w4<T, MT, NT, 0, VEC>(g, st)
+                              : g.group_shift == 1 ? launch_w4<T, MT, NT, 1, VEC>(g, st) : launch_w4<T, MT, NT, 2, VEC>(g, st);
+}
+// Several tiles of the matrix per workgroup where enough workgroups are left to fill the CUs.  16384 x 4096, bfloat16, groups of
+// 128: 12.6 us with one row and one tile per workgroup, 11.3 with four; 64 rows: 67 us with one tile, 40 with two.  8192 x 4096 is
+// the border: one row 7.4 us with one tile, 10.8 with four, 64 rows 35 and 21 with two.  Floats have no registers left for it but for one
+// row tile and large groups (16384 x 4096: 24 -> 15 us).
+template <class T>
+static int launch_w4(const W4Args &g, hipStream_t st) {
+    const int64_t cus = machine().cus;
+    constexpr bool narrow = sizeof(T) == 2;
+    if (g.ids || g.M <= 16) {
+        if (!g.vec_x) return launch_w4<T, 1, 1, false>(g, st);
+        if (!g.ids && g.tiles_n >= 4 * cus) {
+            if constexpr (narrow) return launch_w4<T, 1, 4, true>(g, st);
+            else if (g.group_shift >= 2) return launch_w4<T, 1, 4, 2, true>(g, st);
+        }
+        return launch_w4<T, 1, 1, true>(g, st);
+    }
+    if constexpr (narrow)
+        if (g.vec_x && g.tiles_n >= 2 * cus) return g.M <= 32 ? launch_w4<T, 2, 2, true>(g, st) : launch_w4<T, 4, 2, true>(g, st);
+    if (!g.vec_x) return launch_w4<T, 2, 1, false>(g, st);
+    return g.M <= 32 ? launch_w4<T, 2, 1, true>(g, st) : launch_w4<T, 4, 1, true>(g, st);
 }
 }  // namespace t2sp
 
@@ -334,11 +388,11 @@ extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *
     g.blocks_k = (int)(((int64_t)K + 127) / 128); g.tiles_n = (int)(((int64_t)N + 15) / 16);
     g.group_shift = group_shift_of(group);
     g.groups = (K + group - 1) / group;
+    g.group_blocks = (int)group_blocks_of(K, group);
     g.vec_x = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && (int64_t)K % 8 == 0;
     const hipStream_t st = (hipStream_t)stream;
     return with_types(type, type, [&](auto *t, auto *) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (ids || M <= 16) return launch_w4<T, 1>(g, st);
-        return launch_w4<T, 4>(g, st);
+        return launch_w4<T>(g, st);
     });
 }
