@@ -159,7 +159,8 @@ static_assert(sizeof(struct halide_filter_metadata_t) == 32, "halide_filter_meta
  * Halide::Runtime::Buffer<float> (Halide/src/runtime/HalideBuffer.h:1050-1061:
  * raw_buffer() and the implicit conversion to halide_buffer_t*) for the subset
  * those drivers use: dense allocation, operator() element access, extents.
- * Element types: float, and unsigned char for the character buffers of pairhmm. */
+ * Element types: float, unsigned char for the character buffers of pairhmm and the numbers of gemv_w4, and
+ * int32_t for offsets, labels and ids. */
 #include <cstring>
 #include <initializer_list>
 #include <new>
@@ -170,8 +171,8 @@ extern "C" void t2sp_host_free(void *p);
 namespace t2sp {
 template <typename T>
 class Buffer {
-    static_assert(std::is_same<T, float>::value || std::is_same<T, uint8_t>::value,
-                  "float (every operator) and unsigned char (the characters of pairhmm) are the element types of this path");
+    static_assert(std::is_same<T, float>::value || std::is_same<T, uint8_t>::value || std::is_same<T, int32_t>::value,
+                  "float (every operator), unsigned char and int32_t are the element types of this path");
     T *storage_ = nullptr;           // from t2sp_host_malloc: page-locked when a device is present
     std::vector<halide_dimension_t> dims_;
     halide_buffer_t buf_;
@@ -195,7 +196,7 @@ class Buffer {
         buf_.device_interface = nullptr;
         buf_.host = (uint8_t *)(external ? external : storage_);
         buf_.flags = 0;
-        buf_.type.code = std::is_same<T, float>::value ? halide_type_float : halide_type_uint;
+        buf_.type.code = std::is_same<T, float>::value ? halide_type_float : std::is_same<T, int32_t>::value ? halide_type_int : halide_type_uint;
         buf_.type.bits = (uint8_t)(8 * sizeof(T));
         buf_.type.lanes = 1;
         buf_.dimensions = nd;

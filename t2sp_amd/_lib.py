@@ -132,3 +132,8 @@ def _declare(L):
     L.t2sp_w4_sizes.argtypes = [i32, i32, i32, p64, p64]
     L.t2sp_w4_pack.argtypes = [i32, vp, vp, vp, i32, i32, i32, i32] + [i64] * 6 + [vp, vp, vp, vp]
     L.t2sp_gemv_w4.argtypes = [i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, vp]
+    for name, args in (("gemm_grouped", [i32] + [bp] * 4), ("gemm_grouped_wgrad", [bp] * 4), ("xent", [bp] * 5), ("xent_grad", [bp] * 7),
+                       ("gemv_w4", [i32] + [bp] * 6)):
+        getattr(L, name).argtypes = args
+        getattr(L, name + "_ns").argtypes = args
+        getattr(L, name + "_ns").restype = ctypes.c_double

@@ -38,7 +38,13 @@ assert ctypes.sizeof(halide_dimension_t) == 16
 assert ctypes.sizeof(halide_buffer_t) == 56
 
 FLOAT32 = (2, 32, 1)
+FLOAT16 = (2, 16, 1)
+BFLOAT16 = (4, 16, 1)        # halide_type_bfloat of the Halide versions that have it
 UINT8 = (1, 8, 1)
+INT32 = (0, 32, 1)
+INT64 = (0, 64, 1)
+NUMPY_TYPES = {"float32": FLOAT32, "float16": FLOAT16, "uint8": UINT8, "int32": INT32, "int64": INT64}
+TORCH_TYPES = dict(NUMPY_TYPES, bfloat16=BFLOAT16)
 
 
 class HalideBuffer:
@@ -74,8 +80,8 @@ class HalideBuffer:
 
     @classmethod
     def from_numpy(cls, a):
-        """Host buffer over a float32 (or, for character data, uint8) numpy array with non-negative strides."""
-        assert isinstance(a, np.ndarray) and a.dtype in (np.float32, np.uint8)
+        """Host buffer over a numpy array (float32, or another of NUMPY_TYPES where an operator takes it) with non-negative strides."""
+        assert isinstance(a, np.ndarray) and a.dtype.name in NUMPY_TYPES
         size = a.dtype.itemsize
         assert all(s % size == 0 for s in a.strides)
         ext, st = cls._dims_of(a.shape, [s // size for s in a.strides])
@@ -85,15 +91,16 @@ class HalideBuffer:
         for d in range(len(ext)):            # size-1 axes carry no stride information
             if ext[d] == 1:
                 st[d] = 1 if d == 0 else st[d - 1] * max(ext[d - 1], 1)
-        return cls(ext, st, host=a.ctypes.data, keep=a, type_=FLOAT32 if a.dtype == np.float32 else UINT8)
+        return cls(ext, st, host=a.ctypes.data, keep=a, type_=NUMPY_TYPES[a.dtype.name])
 
     @classmethod
     def from_torch(cls, t):
-        """Device buffer over a float32 torch CUDA tensor (used in place, no copies)."""
-        import torch
-        assert t.is_cuda and t.dtype in (torch.float32, torch.uint8)
+        """Device buffer over a torch CUDA tensor (float32, or another of TORCH_TYPES where an operator takes it; used in
+        place, no copies)."""
+        name = str(t.dtype).rpartition(".")[2]
+        assert t.is_cuda and name in TORCH_TYPES
         ext, st = cls._dims_of(t.shape, t.stride())
-        return cls(ext, st, device=t.data_ptr(), keep=t, type_=FLOAT32 if t.dtype == torch.float32 else UINT8)
+        return cls(ext, st, device=t.data_ptr(), keep=t, type_=TORCH_TYPES[name])
 
     @classmethod
     def from_axes(cls, x, axes):

@@ -16,12 +16,15 @@
 // has no specification in the reference and uses the names of mttkrp-interface.h.  Ranks are those
 // of the FPGA flow's buffers; the entries also accept the other forms their headers list.
 #include "gbmv3-interface.h"
+#include "gemm_grouped-interface.h"
+#include "gemv_w4-interface.h"
 #include "ger-interface.h"
 #include "pairhmm-interface.h"
 #include "qrd-interface.h"
 #include "symv-interface.h"
 #include "syrk-interface.h"
 #include "t2sp_buffer.h"
+#include "xent-interface.h"
 
 namespace {
 
@@ -93,6 +96,15 @@ T2SP_METADATA(pairhmm, {"H", IN, 2, U8}, {"R", IN, 2, U8}, {"delta", IN, 2, F32}
               {"beta_gap", IN, 2, F32}, {"deserializer", OUT, 4, F32})
 T2SP_METADATA(qrd, {"a", IN, 3, F32}, {"QDeserializer", OUT, 3, F32}, {"RDeserializer", OUT, 3, F32})
 
+// The products of a language model's layers have no specification in the reference; names as in their headers.
+T2SP_METADATA(gemm_grouped, {"OpB", SCALAR, 0, I32}, {"X", IN, 2, F32}, {"W", IN, 3, F32}, {"Offsets", IN, 1, I32}, {"Y", OUT, 2, F32})
+T2SP_METADATA(gemm_grouped_wgrad, {"X", IN, 2, F32}, {"dY", IN, 2, F32}, {"Offsets", IN, 1, I32}, {"dW", OUT, 3, F32})
+T2SP_METADATA(xent, {"H", IN, 2, F32}, {"W", IN, 2, F32}, {"Labels", IN, 1, I32}, {"Loss", OUT, 1, F32}, {"Lse", OUT, 1, F32})
+T2SP_METADATA(xent_grad, {"H", IN, 2, F32}, {"W", IN, 2, F32}, {"Labels", IN, 1, I32}, {"Lse", IN, 1, F32}, {"DLoss", IN, 1, F32},
+              {"dH", OUT, 2, F32}, {"dW", OUT, 2, F32})
+T2SP_METADATA(gemv_w4, {"Group", SCALAR, 0, I32}, {"X", IN, 2, F32}, {"Q", IN, 2, U8}, {"S", IN, 2, F32}, {"Z", IN, 2, F32}, {"Ids", IN, 1, I32},
+              {"Y", OUT, 2, F32})
+
 // The argv forms: args[i] points at the i-th scalar, or is the i-th halide_buffer_t* itself.
 extern "C" int syrk_argv(void **a) {
     if (!a) return halide_error_code_buffer_argument_is_null;
@@ -118,4 +130,24 @@ extern "C" int pairhmm_argv(void **a) {
 extern "C" int qrd_argv(void **a) {
     if (!a) return halide_error_code_buffer_argument_is_null;
     return qrd(buf(a[0]), buf(a[1]), buf(a[2]));
+}
+extern "C" int gemm_grouped_argv(void **a) {
+    if (!a) return halide_error_code_buffer_argument_is_null;
+    return gemm_grouped(i32(a[0]), buf(a[1]), buf(a[2]), buf(a[3]), buf(a[4]));
+}
+extern "C" int gemm_grouped_wgrad_argv(void **a) {
+    if (!a) return halide_error_code_buffer_argument_is_null;
+    return gemm_grouped_wgrad(buf(a[0]), buf(a[1]), buf(a[2]), buf(a[3]));
+}
+extern "C" int xent_argv(void **a) {
+    if (!a) return halide_error_code_buffer_argument_is_null;
+    return xent(buf(a[0]), buf(a[1]), buf(a[2]), buf(a[3]), buf(a[4]));
+}
+extern "C" int xent_grad_argv(void **a) {
+    if (!a) return halide_error_code_buffer_argument_is_null;
+    return xent_grad(buf(a[0]), buf(a[1]), buf(a[2]), buf(a[3]), buf(a[4]), buf(a[5]), buf(a[6]));
+}
+extern "C" int gemv_w4_argv(void **a) {
+    if (!a) return halide_error_code_buffer_argument_is_null;
+    return gemv_w4(i32(a[0]), buf(a[1]), buf(a[2]), buf(a[3]), buf(a[4]), buf(a[5]), buf(a[6]));
 }

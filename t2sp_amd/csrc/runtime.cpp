@@ -163,10 +163,11 @@ int Staged::input(const halide_buffer_t *b, const Span &s, const char *op, int e
     return 0;
 }
 
-int Staged::output(halide_buffer_t *b, const Span &s, const char *op, bool partial) {
+int Staged::output(halide_buffer_t *b, const Span &s, const char *op, bool partial, int element_bytes) {
     span_ = s.span;
+    element_bytes_ = element_bytes;
     out_ = b;
-    const size_t bytes = (size_t)s.span * sizeof(float);
+    const size_t bytes = (size_t)s.span * element_bytes;
     if (b->device) {
         ptr_ = reinterpret_cast<float *>(b->device);
         return 0;
@@ -187,7 +188,7 @@ int Staged::finish(const char *op) {
         out_->flags &= ~(uint64_t)halide_buffer_flag_host_dirty;
         return 0;
     }
-    const size_t bytes = (size_t)span_ * sizeof(float);
+    const size_t bytes = (size_t)span_ * element_bytes_;
     if (bytes && hipMemcpy(out_->host, ptr_, bytes, hipMemcpyDeviceToHost) != hipSuccess)
         return report(halide_error_code_copy_to_host_failed, op, "device to host copy failed");
     out_->flags &= ~(uint64_t)(halide_buffer_flag_device_dirty | halide_buffer_flag_host_dirty);

@@ -76,7 +76,7 @@ public:
     // Output: use b->device when present, else pool memory (pre-filled from the
     // host when the buffer is not dense, so that gaps keep their contents).
     // `partial`: the kernels write only part of the buffer; the rest must keep what it holds.
-    int output(halide_buffer_t *b, const Span &s, const char *op, bool partial = false);
+    int output(halide_buffer_t *b, const Span &s, const char *op, bool partial = false, int element_bytes = 4);
     // After the kernels: copy a pool-backed output down to the host, or mark a
     // caller-staged one device_dirty.
     int finish(const char *op);
@@ -87,6 +87,7 @@ private:
     bool pooled_ = false;
     halide_buffer_t *out_ = nullptr;
     int64_t span_ = 0;
+    int element_bytes_ = 4;
 };
 
 // hipEvent bracket around the kernels of one entry-point call, on the library

@@ -12,7 +12,7 @@ import ctypes
 import numpy as np
 
 from ._lib import lib
-from .buffer import HalideBuffer
+from .buffer import HalideBuffer, NUMPY_TYPES
 from .ops import T2spError, _check, _is_torch, host_empty
 
 BAD_TYPE, SHAPE, BAD_DIMENSIONS = -3, -8, -43
@@ -31,7 +31,8 @@ def _torch():
         _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         _set_device = torch.cuda.set_device
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-        torch.cuda.init()
+        if torch.cuda.is_available():
+            torch.cuda.init()
         _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     return _codes
 
@@ -107,6 +108,66 @@ def _enqueue(op, index, like, need, call):
         raise T2spError(op, code)
 
 
+# ---------------------------------------------------------------------------------------------- numpy: the operator entries
+def _entry(op, *args):
+    wrapped = [HalideBuffer.wrap(a) if isinstance(a, np.ndarray) else a for a in args]
+    _check(op, getattr(lib(), op)(*[a.ref if isinstance(a, HalideBuffer) else a for a in wrapped]))
+
+
+def _host_out(op, out, shape, dtype):
+    if out is None:
+        return host_empty(shape) if dtype == np.float32 else np.empty(shape, dtype)
+    _need(op, isinstance(out, np.ndarray), BAD_TYPE)
+    return out
+
+
+def _host_arrays(op, *arrays):
+    for a in arrays:
+        _need(op, isinstance(a, np.ndarray) and a.dtype.name in NUMPY_TYPES, BAD_TYPE)
+
+
+def _host_grouped(op, X, W, offsets, opb, out):
+    _host_arrays(op, X, W, offsets)
+    _need(op, X.ndim == 2 and W.ndim == 3, BAD_DIMENSIONS)
+    Y = _host_out(op, out, (X.shape[0], W.shape[1] if opb else W.shape[2]), X.dtype)
+    _entry(op, int(bool(opb)), X, W, offsets, Y)
+    return Y
+
+
+def _host_wgrad(op, X, dY, offsets, out):
+    _host_arrays(op, X, dY, offsets)
+    _need(op, X.ndim == 2 and dY.ndim == 2 and offsets.ndim == 1, BAD_DIMENSIONS)
+    _need(op, offsets.shape[0] >= 2)
+    dW = _host_out(op, out, (offsets.shape[0] - 1, X.shape[1], dY.shape[1]), X.dtype)
+    _entry(op, X, dY, offsets, dW)
+    return dW
+
+
+def _host_xent(op, H, W, labels, loss, lse):
+    _host_arrays(op, H, W, labels)
+    _need(op, H.ndim == 2, BAD_DIMENSIONS)
+    loss, lse = (_host_out(op, t, (H.shape[0],), np.float32) for t in (loss, lse))
+    _entry(op, H, W, labels, loss, lse)
+    return loss, lse
+
+
+def _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW):
+    _host_arrays(op, H, W, labels, lse, dloss)
+    dH, dW = _host_out(op, dH, H.shape, H.dtype), _host_out(op, dW, W.shape, H.dtype)
+    _entry(op, H, W, labels, lse, dloss, dH, dW)
+    return dH, dW
+
+
+def _host_gemv_w4(op, x, w, ids, out):
+    _host_arrays(op, x, *(() if ids is None else (ids,)))
+    _need(op, x.ndim == 2, BAD_DIMENSIONS)
+    _need(op, (ids is None) == (w.E is None) and isinstance(w.Q, np.ndarray))
+    y = _host_out(op, out, (x.shape[0], w.N), x.dtype)
+    _entry(op, w.group, x, w.Q, w.S, w.Z, ids, y)
+    return y
+
+
+# ---------------------------------------------------------------------------------------------- torch: the thin layer
 def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
     """Y[r] = X[r] @ op(W[e]) for the rows offsets[e] <= r < offsets[e + 1] of group e.
 
@@ -194,10 +255,10 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
     g[t, v] = (exp(z[t, v] - lse[t]) - [v == labels[t]]) * dloss[t]; tokens without a label take no part.
 
     lse: what xent returned; dloss: T float32.  The results have H's type, or float32 (out_dtype, or the type of dH / dW).
-    `wanted` leaves one out (its place in the result is None)."""
+    `wanted` leaves one out (its place in the result is None; numpy arrays: both are computed)."""
     op = "xent_grad"
     if not _is_torch(H):
-        return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW, wanted)
+        return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW)
     code, index, T, V, D, bits = _xent_args(op, H, W, labels)
     _floats(op, lse, index, T)
     _floats(op, dloss, index, T)
@@ -226,6 +287,8 @@ class W4:
 
     def __init__(self, E, N, K, group, Q, S, Z):
         self.E, self.N, self.K, self.group, self.Q, self.S, self.Z = E, N, K, group, Q, S, Z
+        if isinstance(Q, np.ndarray):        # host arrays as they are: the entry lays them out on the device
+            return
         self.dtype, self.code, self.index = S.dtype, _torch()[S.dtype], S.get_device()
         self.pointers = Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None
 
@@ -238,6 +301,10 @@ def pack_w4(q, scales, zeros=None, group=128):
     (..., N, ceil(K / group)) of the type of the rows they will meet (float32, float16 or bfloat16).  group: a power of two
     from 32 on; at least K for one scale per row."""
     op = "pack_w4"
+    if not _is_torch(q):
+        _host_arrays(op, q, scales, *(() if zeros is None else (zeros,)))
+        _need(op, q.ndim in (2, 3), BAD_DIMENSIONS)
+        return W4(q.shape[0] if q.ndim == 3 else None, q.shape[-2], q.shape[-1], int(group), q, scales, zeros)
     code, index = _tensors(op, (q.dim(),) * 2, *((scales,) if zeros is None else (scales, zeros)))
     _need(op, q.dtype is torch.uint8, BAD_TYPE)
     _need(op, q.dim() in (2, 3), BAD_DIMENSIONS)
@@ -267,7 +334,9 @@ def gemv_w4(x, w, ids=None, out=None):
 
     With matrices for E experts, ids (M int32) picks the matrix of each row; a row whose id is outside 0 .. E - 1 is zeros."""
     op = "gemv_w4"
-    _need(op, x.dtype is w.dtype, BAD_TYPE)
+    if not _is_torch(x):
+        return _host_gemv_w4(op, x, w, ids, out)
+    _need(op, x.dtype is getattr(w, "dtype", None), BAD_TYPE)
     _need(op, x.dim() == 2, BAD_DIMENSIONS)
     M, K = x.shape
     index = w.index
