@@ -306,13 +306,17 @@ template <class T>
 __global__ void __launch_bounds__(256) pad_rows_kernel(const T *src, T *dst, int64_t rows, int64_t cols, int64_t ld, int64_t batch_stride,
                                                        int64_t chunks_per_row, int64_t chunks) {
     constexpr int CE = 16 / sizeof(T);
-    typedef T chunk __attribute__((ext_vector_type(CE)));
+    typedef typename Chunk<T>::type chunk;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / chunks_per_row, c = (i % chunks_per_row) * CE;
         const T *s = src + (row / rows) * batch_stride + (row % rows) * ld + c;
         chunk v;
+        if (c + CE <= cols) {                        // (memory takes 16 bytes at any element's alignment)
+            v = *reinterpret_cast<const typename Chunk<T>::anywhere *>(s);
+        } else {
 #pragma unroll
-        for (int j = 0; j < CE; j++) v[j] = c + j < cols ? s[j] : (T)0;
+            for (int j = 0; j < CE; j++) v[j] = c + j < cols ? s[j] : (T)0;
+        }
         *reinterpret_cast<chunk *>(dst + i * CE) = v;
     }
 }

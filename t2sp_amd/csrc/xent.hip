@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(const float *dloss, co
 
 // Hz[t, :] = H[t, :] * (dloss[t] / max |dloss|) rounded to the type, zeros for tokens without a label and from D to ld.
 template <class T>
-__global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int64_t ldh, bool vec, const void *labels, int lab64, const float *dloss,
+__global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int64_t ldh, const void *labels, int lab64, const float *dloss,
                                                                  const float *scale, int rows, int V, int D, T *Hz, int64_t ld, int64_t chunks) {
     constexpr int CE = 16 / sizeof(T);
     typedef T chunk __attribute__((ext_vector_type(CE)));
@@ -187,9 +187,14 @@ __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int
         if (label >= 0 && label < V) {
             const float by = *scale == 0.f ? 0.f : dloss[t] / *scale;
             const T *s = H + t * ldh + c;
-            if (vec) v = *reinterpret_cast<const chunk *>(s);
+            if (c + CE <= D) {
+                v = *reinterpret_cast<const typename Chunk<T>::anywhere *>(s);
+            } else {
 #pragma unroll
-            for (int j = 0; j < CE; j++) v[j] = (T)((float)(vec ? v[j] : c + j < D ? s[j] : (T)0) * by);
+                for (int j = 0; j < CE; j++) v[j] = c + j < D ? s[j] : (T)0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < CE; j++) v[j] = (T)((float)v[j] * by);
         } else {
 #pragma unroll
             for (int j = 0; j < CE; j++) v[j] = (T)0.f;
@@ -471,7 +476,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
         const int64_t chunks = (int64_t)g.T * r.ldd * size / 16;
         if (chunks) {
             hipLaunchKernelGGL(xent_weighted_rows_kernel<T>, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
-                               static_cast<const T *>(H), ldh, r.h == (size_t)-1, g.labels, g.lab64, g.dloss, scale, g.T, g.V, g.D,
+                               static_cast<const T *>(H), ldh, g.labels, g.lab64, g.dloss, scale, g.T, g.V, g.D,
                                reinterpret_cast<T *>(room + r.hz), r.ldd, chunks);
             if ((err = launched())) return err;
         }
