@@ -107,6 +107,7 @@ struct ProductTile {
     static constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES, LDS = S * STAGE;
     static constexpr int A_LOADS = BM / 16 >= NW ? BM / 16 / NW : 1, B_LOADS = BN / 16 / NW;
     static constexpr int LOADS = A_LOADS + B_LOADS;                         // per wave and stage
+    static constexpr bool TURNS = SZ == 2 && NW == 8 && AS == KMAJOR;        // see product_run
     static constexpr int A_READS = MT * (AS == KMAJOR ? 1 : SZ == 2 ? 2 : 4), B_READS = NT * (BS == KMAJOR ? 1 : SZ == 2 ? 2 : 4);
     static constexpr int LANE_N = 4 * NT;                                   // columns a lane ends up with, per row
     static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "whole accumulator tiles");
@@ -274,13 +275,46 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
         __builtin_amdgcn_sched_barrier(0);
     };
 
+    const int stages = (k_len + P::KS - 1) / P::KS;
+    if constexpr (P::TURNS) {
+        // Two waves share a SIMD, one of each half of the workgroup, and take turns: while one multiplies (its 32 MFMAs
+        // fill the SIMD's matrix unit for 512 cycles), the other reads its operands of the next stage from LDS and sends the loads
+        // of a later one.  A barrier ends every turn, the second half of the waves runs one turn behind.  With both waves in step
+        // the matrix units were idle a third of the time, around the barriers (MEASURED_TURNS).
+        // Stage t is read in the turns 2 t and 2 t + 1 and must have landed before them; its buffer is free in turn 2 t + 2,
+        // where the loads of stage t + S are first sent.  A wave sees to its own loads of stage t + 1 at the end of its turn with t.
+        const bool behind = wave >= P::NW / 2;
+#pragma unroll
+        for (int s = 0; s < P::S - 1; s++) issue();
+        wait_loads<(P::S - 2) * P::LOADS>();
+        __builtin_amdgcn_s_barrier();
+        if (behind) __builtin_amdgcn_s_barrier();
+        typename P::Frags f;
+        for (int t = 0; t < stages; t++) {
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(f);
+            issue();
+            wait_loads<(P::S - 2) * P::LOADS>();
+            wait_lds_reads();
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            multiply(f);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_barrier();
+        }
+        if (!behind) __builtin_amdgcn_s_barrier();
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        return;
+    }
 #pragma unroll
     for (int s = 0; s < P::S; s++) issue();
     wait_loads<(P::S - 1) * P::LOADS>();
     __builtin_amdgcn_s_barrier();
     typename P::Frags f0, f1;
     fetch(f0);
-    const int stages = (k_len + P::KS - 1) / P::KS;
     // Sums of floats are taken in runs of RUN stages (256 elements of k) that are added up on the vector units: the error of
     // one running sum over k grows with sqrt(k), that of two levels with sqrt(256 + k / 256) (8192 of k: 1.0e-6 -> 3e-7
     // of the result's norm).  Results of 16-bit operands are rounded far above that.
