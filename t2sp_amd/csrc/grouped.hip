@@ -26,6 +26,7 @@ struct GroupedArgs {
     int T, E, K, N;
     int64_t ldx, ldw, sw, ldy;           // in elements; sw: between matrices
     int col_tiles, xcds;
+    int die_cus;                         // CUs of a die
 };
 
 __device__ __forceinline__ int group_edge(const GroupedArgs &g, int e) {
@@ -35,11 +36,13 @@ __device__ __forceinline__ int group_edge(const GroupedArgs &g, int e) {
 
 struct GroupTile {
     int group, row0, rows, col_tile;     // rows: of the group from row0 on
+    bool half;                           // only the first BM / 2 of them
 };
 
 // The output tile of workgroup `block`, false when there is none.  Every wave does the same work; the results are
-// uniform over the wave.
-template <int BM>
+// uniform over the wave.  HALVES: when the tiles that are left for a die's last round of workgroups would fill at most half of
+// its CUs, each of them goes to two workgroups, by halves of its rows.
+template <int BM, bool HALVES = false>
 __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, GroupTile *out) {
     const int lane = threadIdx.x & 63;
     auto tiles_of = [&](int e, int *start, int *rows) {
@@ -65,7 +68,17 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
     }
     total *= g.col_tiles;
     const int64_t run = (total + g.xcds - 1) / g.xcds;
-    const int64_t at = block / g.xcds, w = (block % g.xcds) * run + at;
+    const int64_t first = (block % g.xcds) * run;
+    int64_t at = block / g.xcds;
+    int half = -1;
+    if (HALVES) {
+        const int64_t mine = total - first < run ? total - first : run, whole = mine > 0 ? mine / g.die_cus * g.die_cus : 0;
+        if (at >= whole && 2 * (mine - whole) <= g.die_cus) {
+            half = (int)((at - whole) & 1);
+            at = whole + (at - whole) / 2;
+        }
+    }
+    const int64_t w = first + at;
     if (at >= run || w >= total) return false;
     int64_t before = 0;                              // tiles of the groups in front of this chunk of 64
     for (int e0 = 0; e0 < g.E;) {
@@ -80,7 +93,12 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
             out->group = e0 + l;
             out->row0 = __builtin_amdgcn_readlane(start, l) + m * BM;
             out->rows = __builtin_amdgcn_readlane(rows, l) - m * BM;
-            return true;
+            out->half = half >= 0;
+            if (half > 0) {
+                out->row0 += BM / 2;
+                out->rows -= BM / 2;
+            }
+            return out->rows > 0;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
         e0 += 64;
@@ -91,15 +109,12 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
 }
 
 template <class P, class O>
-__global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    GroupTile t;
-    if (!find_tile<P::BM>(g, blockIdx.x, &t)) return;
-    const int n0 = t.col_tile * P::BN;
+__device__ __forceinline__ void grouped_tile(const GroupedArgs &g, const GroupTile &t, int n0, char *smem) {
+    const int have = t.half && t.rows > P::BM ? P::BM : t.rows;
     TileSource a, b;
     a.p = g.X + t.row0 * g.ldx * P::SZ;
     a.ld = (uint32_t)(g.ldx * P::SZ);
-    a.count = t.rows;
+    a.count = have;
     b.p = g.W + t.group * g.sw * P::SZ + (P::BS == KMAJOR ? n0 * g.ldw : (int64_t)n0) * P::SZ;
     b.ld = (uint32_t)(g.ldw * P::SZ);
     b.count = g.N - n0;
@@ -111,8 +126,27 @@ __global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int m = (wave / P::WN) * P::TM + 16 * i + (lane & 15);
-        if (m < t.rows) store_row<P, O>(g.Y + (t.row0 + m) * g.ldy * sizeof(O), n, g.N, acc[i]);
+        if (m < have) store_row<P, O>(g.Y + (t.row0 + m) * g.ldy * sizeof(O), n, g.N, acc[i]);
     }
+}
+
+template <class P, class O>
+__global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    GroupTile t;
+    if constexpr (P::BM == 256) {
+        // Tiles of at most 128 rows, a group's last one or a half, take the same waves in half the time.  (16384 rows in 16 groups,
+        // 2048 -> 4096: 4.5 rounds of workgroups, every fourth row tile a partial one: 280 us without, 272 with;
+        // 4096 rows in 8 groups, 4096 -> 4096: 194 and 172)
+        if (!find_tile<P::BM, true>(g, blockIdx.x, &t)) return;
+        if (t.half || t.rows <= 128) {
+            grouped_tile<ProductTile<typename P::T, 128, P::BN, P::WM, P::WN, P::AS, P::BS, P::S>, O>(g, t, t.col_tile * P::BN, smem);
+            return;
+        }
+    } else {
+        if (!find_tile<P::BM>(g, blockIdx.x, &t)) return;
+    }
+    grouped_tile<P, O>(g, t, t.col_tile * P::BN, smem);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows per group
@@ -342,7 +376,10 @@ static int64_t most_row_tiles(int T, int E, int bm) { return T / bm + (E < T ? E
 template <class P, class O>
 static int launch_forward(GroupedArgs g, hipStream_t stream) {
     g.col_tiles = (g.N + P::BN - 1) / P::BN;
-    const int64_t blocks = (most_row_tiles(g.T, g.E, P::BM) * g.col_tiles + g.xcds - 1) / g.xcds * g.xcds;
+    g.die_cus = machine().cus / g.xcds;
+    // (halves: up to half a die's CUs more workgroups per die)
+    const int64_t runs = (most_row_tiles(g.T, g.E, P::BM) * g.col_tiles + g.xcds - 1) / g.xcds + (P::BM == 256 ? (g.die_cus + 1) / 2 : 0);
+    const int64_t blocks = runs * g.xcds;
     if (blocks > 0x7fffffff / P::THREADS) return T2SP_ERR_SHAPE;
     auto kern = grouped_kernel<P, O>;
     if (allow_lds(kern, P::LDS)) return T2SP_ERR_LAUNCH;
