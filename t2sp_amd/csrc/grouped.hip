@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g
 // ------------------------------------------------------------------------------------------------ few rows per group
 // Decoding: a group has a handful of rows, and what takes time is reading its matrix once.  A workgroup owns up to 16 MT
 // rows of a group and a strip of columns; its eight waves take pieces of K in turn and are joined through LDS in a
-// fixed order.  The matrix goes from memory straight into MFMA operands, 8 loads of 16 bytes per lane in flight and two
+// fixed order.  The matrix goes from memory straight into MFMA operands, 8 or 16 loads of 16 bytes per lane in flight and two
 // or more workgroups per CU (a CU needs about 50 KB in flight to draw its share of HBM's rate):
 //   KMAJOR  32 columns; a lane's 16 bytes are k of its column, as the MFMA wants them; 256 bytes of a column per piece.
 //   KROWS   16 EPC columns (128 of 16 bits, 64 floats): lane l reads EPC columns of k rows EPC (l / 16) + 0 .. EPC - 1, a block
@@ -167,18 +167,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const char *p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, 0x7fffffff, 0x00020000);
 }
 
-template <class T, int BS>
+template <class T, int BS, int MT = 1>
 struct FewRows {
     static constexpr int SZ = sizeof(T), EPC = 16 / SZ, STEP = 64 / SZ;     // k per MFMA step
     static constexpr int WAVES = 8, THREADS = 64 * WAVES;
     static constexpr int NT = BS == KMAJOR ? 2 : EPC, COLS = 16 * NT;
-    static constexpr int STEPS = BS == KMAJOR ? 4 : SZ == 2 ? 1 : 2;        // per piece: 8 loads of the matrix
+    static constexpr int LOADS = BS == KROWS && SZ == 2 && MT == 1 ? 16 : 8;  // of the matrix per piece
+    static constexpr int STEPS = BS == KMAJOR ? LOADS / NT : LOADS / EPC;
     static constexpr int LDS = WAVES * 16 * COLS * 4;
 };
 
 template <class T, class O, int BS, int MT>
 __global__ void __launch_bounds__(512) grouped_few_rows_kernel(const GroupedArgs g) {
-    using F = FewRows<T, BS>;
+    using F = FewRows<T, BS, MT>;
     constexpr int EPC = F::EPC, NT = F::NT, SZ = F::SZ;
     __shared__ __attribute__((aligned(16))) float joint[F::WAVES][16][F::COLS];
     GroupTile t;

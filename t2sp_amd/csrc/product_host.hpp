@@ -46,7 +46,7 @@ struct TileShape {
     double a, c;
     int ends = 4;
 };
-constexpr TileShape SHAPE_256{256, 256, -0.2, 0.9, 10}, SHAPE_128{128, 128, 0.06, 0.335}, SHAPE_64{64, 128, 0.12, 0.21};
+constexpr TileShape SHAPE_256{256, 256, -0.1, 0.75, 10}, SHAPE_128{128, 128, 0.1, 0.28, 7}, SHAPE_64{64, 128, 0.08, 0.205, 4};
 constexpr TileShape SHAPE_128F{128, 128, 0.1, 1.02}, SHAPE_64F{64, 64, 0.12, 0.285};
 inline double tiles_cost(const TileShape &s, int64_t tiles, int64_t k_bytes) {
     const int64_t cus = machine().cus, n = (tiles + cus - 1) / cus;
