@@ -90,22 +90,23 @@ def _matrix(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * _row(t))
 
 
-def _enqueue(op, index, like, need, call):
-    """call(workspace, bytes, stream) on device `index`'s current stream, with `need` (a function, or None) bytes of
-    workspace.  The workspace's owner may be dropped after the call: torch's allocator hands the memory out again only to
+class _On:
+    """Makes device `index` current around a call (used when it is not)."""
+
+    def __init__(self, index, back):
+        self.index, self.back = index, back
+
+    def __enter__(self):
+        _set_device(self.index)
+
+    def __exit__(self, *exc):
+        _set_device(self.back)
+
+
+def _room(like, nbytes):
+    """A workspace, or None.  Its owner may be dropped after the call: torch's allocator hands the memory out again only to
     work that is ordered behind it."""
-    back = _current_device()
-    if index != back:
-        _set_device(index)
-    try:
-        nbytes = need() if need else 0
-        room = like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        code = call(room.data_ptr() if nbytes else None, nbytes, _raw_stream(index))
-    finally:
-        if index != back:
-            _set_device(back)
-    if code:
-        raise T2spError(op, code)
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 # ---------------------------------------------------------------------------------------------- numpy: the operator entries
@@ -189,11 +190,16 @@ def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
     _need(op, E >= 1 and K >= 1 and N >= 1)
     bits = _vector(op, offsets, _int_bits, index, E + 1)
     Y, out_code = _result(op, out, (T, N), X, out_dtype)
+    back = _current_device()
+    if back != index:
+        with _On(index, back):
+            return gemm_grouped(X, W, offsets, opb, Y)
     L = lib()
     x, w, ldx, ldw, sw = X.data_ptr(), W.data_ptr(), _row(X), _row(W), _matrix(W)
-    _enqueue(op, index, X, lambda: L.t2sp_gemm_grouped_workspace_bytes(code, opb, x, w, T, E, K, N, ldx, ldw, sw),
-             lambda ws, nbytes, stream: L.t2sp_gemm_grouped(code, out_code, opb, x, w, offsets.data_ptr(), bits, Y.data_ptr(), T, E, K, N,
-                                                            ldx, ldw, sw, _row(Y), ws, nbytes, stream))
+    nbytes = L.t2sp_gemm_grouped_workspace_bytes(code, opb, x, w, T, E, K, N, ldx, ldw, sw)
+    room = _room(X, nbytes)
+    _check(op, L.t2sp_gemm_grouped(code, out_code, opb, x, w, offsets.data_ptr(), bits, Y.data_ptr(), T, E, K, N, ldx, ldw, sw, _row(Y),
+                                   room.data_ptr() if nbytes else None, nbytes, _raw_stream(index)))
     return Y
 
 
@@ -210,11 +216,16 @@ def gemm_grouped_wgrad(X, dY, offsets, out=None, out_dtype=None):
     _need(op, dY.shape[0] == T and E >= 1 and K >= 1 and N >= 1)
     bits = _vector(op, offsets, _int_bits, index, E + 1)
     dW, out_code = _result(op, out, (E, K, N), X, out_dtype)
+    back = _current_device()
+    if back != index:
+        with _On(index, back):
+            return gemm_grouped_wgrad(X, dY, offsets, dW)
     L = lib()
     x, dy, ldx, ldy = X.data_ptr(), dY.data_ptr(), _row(X), _row(dY)
-    _enqueue(op, index, X, lambda: L.t2sp_gemm_grouped_wgrad_workspace_bytes(code, x, dy, T, E, K, N, ldx, ldy),
-             lambda ws, nbytes, stream: L.t2sp_gemm_grouped_wgrad(code, out_code, x, dy, offsets.data_ptr(), bits, dW.data_ptr(), T, E, K, N,
-                                                                  ldx, ldy, _row(dW), _matrix(dW), ws, nbytes, stream))
+    nbytes = L.t2sp_gemm_grouped_wgrad_workspace_bytes(code, x, dy, T, E, K, N, ldx, ldy)
+    room = _room(X, nbytes)
+    _check(op, L.t2sp_gemm_grouped_wgrad(code, out_code, x, dy, offsets.data_ptr(), bits, dW.data_ptr(), T, E, K, N, ldx, ldy, _row(dW),
+                                         _matrix(dW), room.data_ptr() if nbytes else None, nbytes, _raw_stream(index)))
     return dW
 
 
@@ -242,11 +253,16 @@ def xent(H, W, labels, loss=None, lse=None):
     code, index, T, V, D, bits = _xent_args(op, H, W, labels)
     loss = H.new_empty(T, dtype=torch.float32) if loss is None else _floats(op, loss, index, T)
     lse = H.new_empty(T, dtype=torch.float32) if lse is None else _floats(op, lse, index, T)
+    back = _current_device()
+    if back != index:
+        with _On(index, back):
+            return xent(H, W, labels, loss, lse)
     L = lib()
     h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
-    _enqueue(op, index, H, lambda: L.t2sp_xent_workspace_bytes(code, h, w, T, V, D, ldh, ldw),
-             lambda ws, nbytes, stream: L.t2sp_xent(code, h, w, labels.data_ptr(), bits, loss.data_ptr(), lse.data_ptr(), T, V, D, ldh, ldw, ws,
-                                                    nbytes, stream))
+    nbytes = L.t2sp_xent_workspace_bytes(code, h, w, T, V, D, ldh, ldw)
+    room = _room(H, nbytes)
+    _check(op, L.t2sp_xent(code, h, w, labels.data_ptr(), bits, loss.data_ptr(), lse.data_ptr(), T, V, D, ldh, ldw,
+                           room.data_ptr() if nbytes else None, nbytes, _raw_stream(index)))
     return loss, lse
 
 
@@ -272,13 +288,18 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
         out_code = other
     if out_code is None:
         return None, None
+    back = _current_device()
+    if back != index:
+        with _On(index, back):
+            return xent_grad(H, W, labels, lse, dloss, dH, dW, wanted=(False, False))      # (what is wanted is allocated by now)
     L = lib()
     h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
-    _enqueue(op, index, H, lambda: L.t2sp_xent_grad_workspace_bytes(code, h, w, T, V, D, ldh, ldw),
-             lambda ws, nbytes, stream: L.t2sp_xent_grad(code, out_code, h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
-                                                         dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None,
-                                                         T, V, D, ldh, ldw, _row(dH) if dH is not None else D, _row(dW) if dW is not None else D,
-                                                         ws, nbytes, stream))
+    nbytes = L.t2sp_xent_grad_workspace_bytes(code, h, w, T, V, D, ldh, ldw)
+    room = _room(H, nbytes)
+    _check(op, L.t2sp_xent_grad(code, out_code, h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
+                                dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None, T, V, D, ldh, ldw,
+                                _row(dH) if dH is not None else D, _row(dW) if dW is not None else D,
+                                room.data_ptr() if nbytes else None, nbytes, _raw_stream(index)))
     return dH, dW
 
 
@@ -321,11 +342,11 @@ def pack_w4(q, scales, zeros=None, group=128):
     S = scales.new_empty(E * se.value)
     Z = torch.empty_like(S) if zeros is not None else None
     each = lambda t: _matrix(t) if t.dim() == 3 else 0
-    _enqueue(op, index, q, None,
-             lambda ws, nbytes, stream: L.t2sp_w4_pack(code, q.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, E, N,
-                                                       K, group, _row(q), each(q), _row(scales), each(scales),
-                                                       _row(zeros) if zeros is not None else 0, each(zeros) if zeros is not None else 0,
-                                                       Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None, stream))
+    with _On(index, _current_device()):
+        _check(op, L.t2sp_w4_pack(code, q.data_ptr(), scales.data_ptr(), zeros.data_ptr() if zeros is not None else None, E, N, K, group,
+                                  _row(q), each(q), _row(scales), each(scales), _row(zeros) if zeros is not None else 0,
+                                  each(zeros) if zeros is not None else 0, Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None,
+                                  _raw_stream(index)))
     return W4(E if q.dim() == 3 else None, N, K, group, Q, S, Z)
 
 
@@ -336,21 +357,27 @@ def gemv_w4(x, w, ids=None, out=None):
     op = "gemv_w4"
     if not _is_torch(x):
         return _host_gemv_w4(op, x, w, ids, out)
-    _need(op, x.dtype is getattr(w, "dtype", None), BAD_TYPE)
-    _need(op, x.dim() == 2, BAD_DIMENSIONS)
-    M, K = x.shape
-    index = w.index
-    _need(op, K == w.K and x.get_device() == index and (x.stride(1) == 1 or K <= 1) and (ids is None) == (w.E is None))
+    if x.dtype is not getattr(w, "dtype", None):
+        raise T2spError(op, BAD_TYPE)
+    if x.dim() != 2:
+        raise T2spError(op, BAD_DIMENSIONS)
+    (M, K), index = x.shape, w.index
+    ldx = x.stride(0)
+    if K != w.K or x.get_device() != index or (x.stride(1) != 1 and K > 1) or (ids is None) != (w.E is None):
+        raise T2spError(op, SHAPE)
     if ids is not None:
         _vector(op, ids, {torch.int32: 32}, index, M)
     if out is None:
-        y, ldy = x.new_empty((M, w.N)), w.N
+        out, ldy = x.new_empty((M, w.N)), w.N
     else:
         _need(op, out.dtype is x.dtype, BAD_TYPE)
-        y, _ = _result(op, out, (M, w.N), x)
-        ldy = _row(y)
+        _result(op, out, (M, w.N), x)
+        ldy = _row(out)
+    back = _current_device()
+    if back != index:
+        with _On(index, back):
+            return gemv_w4(x, w, ids, out)
     Q, S, Z = w.pointers
-    _enqueue(op, index, x, None,
-             lambda ws, nbytes, stream: lib().t2sp_gemv_w4(w.code, x.data_ptr(), Q, S, Z, ids.data_ptr() if ids is not None else None, y.data_ptr(),
-                                                           M, w.N, K, w.E or 1, w.group, _row(x), ldy, stream))
-    return y
+    _check(op, lib().t2sp_gemv_w4(w.code, x.data_ptr(), Q, S, Z, None if ids is None else ids.data_ptr(), out.data_ptr(), M, w.N, K, w.E or 1, w.group,
+                                  ldx if M > 1 or ldx > K else K, ldy, _raw_stream(index)))
+    return out
