@@ -378,7 +378,7 @@ static int64_t most_row_tiles(int T, int E, int bm) { return T / bm + (E < T ? E
 template <class P, class O>
 static int launch_forward(GroupedArgs g, hipStream_t stream) {
     g.col_tiles = (g.N + P::BN - 1) / P::BN;
-    g.die_cus = machine().cus / g.xcds;
+    g.die_cus = std::max(1, machine().cus / g.xcds);
     // (halves: up to half a die's CUs more workgroups per die)
     const int64_t runs = (most_row_tiles(g.T, g.E, P::BM) * g.col_tiles + g.xcds - 1) / g.xcds + (P::BM == 256 ? (g.die_cus + 1) / 2 : 0);
     const int64_t blocks = runs * g.xcds;

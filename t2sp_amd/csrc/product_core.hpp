@@ -85,10 +85,16 @@ constexpr uint32_t OUT_OF_RANGE = 0x80000000u;      // a lane offset that the de
 // waits with wait_loads().  (The m0 write needs one instruction between itself and the load.)
 __device__ __forceinline__ void load_to_lds(pv4u rsrc, uint32_t off, uint32_t lds_base) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-                 :: "v"(off), "s"(rsrc), "s"(lds_base) : "memory");
+                 :: "v"(off), "s"(rsrc), "s"(lds_base) : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+// s_barrier, with nothing moved across it by the compiler (the builtin alone says nothing about memory).
+__device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
@@ -289,8 +295,8 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
 #pragma unroll
         for (int s = 0; s < P::S - 1; s++) issue();
         wait_loads<(P::S - 2) * P::LOADS>();
-        __builtin_amdgcn_s_barrier();
-        if (behind) __builtin_amdgcn_s_barrier();
+        meet();
+        if (behind) meet();
         typename P::Frags f;
         for (int t = 0; t < stages; t++) {
             __builtin_amdgcn_sched_barrier(0);
@@ -298,23 +304,23 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
             issue();
             wait_loads<(P::S - 2) * P::LOADS>();
             wait_lds_reads();
-            __builtin_amdgcn_s_barrier();
+            meet();
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             multiply(f);
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_barrier();
+            meet();
         }
-        if (!behind) __builtin_amdgcn_s_barrier();
+        if (!behind) meet();
         wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
+        meet();
         return;
     }
 #pragma unroll
     for (int s = 0; s < P::S; s++) issue();
     wait_loads<(P::S - 1) * P::LOADS>();
-    __builtin_amdgcn_s_barrier();
+    meet();
     typename P::Frags f0, f1;
     fetch(f0);
     // Sums of floats are taken in runs of RUN stages (256 elements of k) that are added up on the vector units: the error of
@@ -340,12 +346,12 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
                     }
         wait_loads<(P::S - 2) * P::LOADS>();          // stage t + 1 has landed
         wait_lds_reads();                             // this wave's operands of stage t are in registers:
-        __builtin_amdgcn_s_barrier();                 // its buffer may be overwritten
+        meet();                 // its buffer may be overwritten
         issue();
         fetch_and_multiply(f1, f0);
         wait_loads<(P::S - 2) * P::LOADS>();
         wait_lds_reads();
-        __builtin_amdgcn_s_barrier();
+        meet();
         issue();
         fetch_and_multiply(f0, f1);
     }
@@ -356,7 +362,7 @@ __device__ __forceinline__ void product_run(const TileSource &A, const TileSourc
             for (int j = 0; j < P::NT; j++) acc[i][j] += whole[i][j];
     wait_loads<0>();
     wait_lds_reads();
-    __builtin_amdgcn_s_barrier();
+    meet();
 }
 
 // The position that workgroup `block` of `total` takes when every die works on a contiguous run of positions (workgroup

@@ -58,8 +58,11 @@ inline double tiles_cost(const TileShape &s, int64_t groups, int64_t rows, int64
     return tiles_cost(s, (row_tiles + (groups > 1 ? row_tiles / 20 + 1 : 0)) * ((cols + s.cols - 1) / s.cols), k_bytes);
 }
 // The tile edge for a product of `rows` x `cols`: 256, 128 or 64 (64 only where its operand layouts have that tile).
-inline int pick_tile(int64_t groups, int64_t rows, int64_t cols, int64_t k, int size, bool small = true) {
-    const double c256 = size == 2 ? tiles_cost(SHAPE_256, groups, rows, cols, k * size) : 1e30;
+// `epilogue`: stages that the 256 x 256 tile's epilogue takes beyond a plain store.
+inline int pick_tile(int64_t groups, int64_t rows, int64_t cols, int64_t k, int size, bool small = true, int epilogue = 0) {
+    TileShape large = SHAPE_256;
+    large.ends += epilogue;
+    const double c256 = size == 2 ? tiles_cost(large, groups, rows, cols, k * size) : 1e30;
     const double c128 = tiles_cost(size == 2 ? SHAPE_128 : SHAPE_128F, groups, rows, cols, k * size);
     const double c64 = small ? tiles_cost(size == 2 ? SHAPE_64 : SHAPE_64F, groups, rows, cols, k * size) : 1e30;
     return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;

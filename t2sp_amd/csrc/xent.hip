@@ -349,6 +349,9 @@ constexpr int64_t G_BYTES = 128 << 20;   // of the piece of p - [label]: it then
                                          // kernel and the two products that read it ...
 constexpr int MIN_PIECE = 4096;          // ... but a piece is long enough that adding up dH costs little beside it
 
+// The tile of the logits; 65536 exponentials are worth four stages (777 x 50001 x 1022, half: 129 us in 256 x 256 tiles, 120 in
+// 128 x 128; 2048 x 32000 x 2048, bfloat16: 238 us in 256 x 256 tiles).
+static int logits_shape(int64_t T, int64_t V, int64_t D, int size) { return pick_tile(1, T, V, D, size, true, 4); }
 // Columns of the forward pass's tile.
 static int tile_cols(int tile, int size) { return tile == 64 && size == 2 ? 128 : tile; }
 
@@ -376,7 +379,7 @@ static XentRoom xent_room(bool backward, int type, const void *H, const void *W,
     r.h = loadable(H, ldh, D, size) ? (size_t)-1 : take((size_t)T * r.ldd * size);
     r.w = loadable(W, ldw, D, size) ? (size_t)-1 : take((size_t)V * r.ldd * size);
     if (!backward) {
-        const int cols = tile_cols(pick_tile(1, T, V, D, size), size);
+        const int cols = tile_cols(logits_shape(T, V, D, size), size);
         r.part = take((size_t)((V + cols - 1) / cols) * T * sizeof(float2));
         r.hit = take((size_t)T * sizeof(float));
     } else {
@@ -453,7 +456,7 @@ template <class T, int AS, int BS> using Large = std::conditional_t<sizeof(T) ==
 
 template <class T>
 static int xent_forward(XentArgs g, float *loss, float *lse, hipStream_t st) {
-    const int tile = pick_tile(1, g.T, g.V, g.D, sizeof(T)), cols = tile_cols(tile, sizeof(T));
+    const int tile = logits_shape(g.T, g.V, g.D, sizeof(T)), cols = tile_cols(tile, sizeof(T));
     int err = tile == 256 ? launch_stats<Large<T, KMAJOR, KMAJOR>>(g, st)
                           : tile == 128 ? launch_stats<Tile128<T, KMAJOR, KMAJOR>>(g, st) : launch_stats<Tile64<T, KMAJOR>>(g, st);
     if (err) return err;
@@ -487,7 +490,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
         g.G = room + r.g;
         g.ldg = padded_cols(g.vp, size);
         if (g.T) {
-            const int tile = pick_tile(1, g.T, g.vp, g.D, size);
+            const int tile = logits_shape(g.T, g.vp, g.D, size);
             err = tile == 256 ? launch_probabilities<Large<T, KMAJOR, KMAJOR>>(g, st)
                               : tile == 128 ? launch_probabilities<Tile128<T, KMAJOR, KMAJOR>>(g, st) : launch_probabilities<Tile64<T, KMAJOR>>(g, st);
             if (err) return err;

@@ -249,6 +249,34 @@ def test_streams_and_threads_at_once():
     assert not failed, failed
 
 
+@pytest.mark.parametrize("cus,xcds", [(1, 1), (3, 8), (38, 1), (304, 8), (64, 4)])
+def test_planned_for_other_machines(cus, xcds):
+    """Launches planned for other numbers of CUs and dies (a partitioned device) cover every tile: values against float64."""
+    import torch
+    L = t2sp_amd.lib()
+    X, W, dY = normal((1200, 136), 70), normal((5, 136, 520), 71), normal((1200, 520), 72)
+    bounds = [0, 700, 700, 830, 831, 1190]
+    off = torch.tensor(bounds, dtype=torch.int32).cuda()
+    Hh, Wv = normal((300, 64), 73).bfloat16(), normal((1000, 64), 74, 0.2).bfloat16()
+    lab = torch.arange(300).cuda()
+    want = t2sp_amd.xent(Hh, Wv, lab)[0]
+    L.t2sp_set_machine(cus, xcds)
+    try:
+        for half in (False, True):
+            x, w, d = (t.bfloat16() if half else t for t in (X, W, dY))
+            Y, dW = t2sp_amd.gemm_grouped(x, w, off, out_dtype=torch.float32), t2sp_amd.gemm_grouped_wgrad(x, d, off, out_dtype=torch.float32)
+            by_group(lambda e, s: Bounded(x[s]).mm(Bounded(w[e])), bounds).check(Y[:1190])
+            for e in range(5):
+                s = slice(bounds[e], bounds[e + 1])
+                Bounded(x[s]).t().mm(Bounded(d[s])).check(dW[e])
+        loss, lse = t2sp_amd.xent(Hh, Wv, lab)
+        assert torch.allclose(loss, want, rtol=0, atol=1e-5)     # (sums of 1000 terms near 1, in another order)
+        dH, _ = t2sp_amd.xent_grad(Hh, Wv, lab, lse, torch.full((300,), 1 / 300, device="cuda"))
+        assert torch.isfinite(dH.float()).all()
+    finally:
+        L.t2sp_set_machine(0, 0)
+
+
 def test_driver_in_cpp_prints_success(tmp_path):
     """tests/drivers/gemm_grouped-run.cpp: the C++ interface with host buffers (built by `make -C tests/drivers`)."""
     import os
