@@ -15,6 +15,7 @@
 #include "product_host.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace t2sp {
 
@@ -409,28 +410,55 @@ static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
     return launched();
 }
 
-// Groups are taken as equally large for these choices.  Beside the tiles' cost stands the time to read the matrices at the
-// rate each form reached on 0.5 GB of them (TB/s): the larger of the two and a quarter of the smaller.
+// What a product takes in each form (microseconds), from the extents alone: groups of T / E rows make half a row tile more than
+// whole ones would (their sizes differ), the workgroups share the CUs, n to a CU, and a stage of 64 bytes of k takes
+// a + n (c + fill x the 16-row blocks that hold rows); `ends` stages go into start and store.  Beside that stands the reading of the
+// matrices at `rate` TB/s: the larger of the two and a quarter of the smaller.  Fitted to 350 products of 16-bit elements a
+// layout and 300 of floats (4 to 8192 rows in 1 to 64 groups of any sizes, 64 to 4096 x 64 to 4096): the form picked took 1.5
+// percent more than the best of the six (floats, KMAJOR: 3), geometric mean over those kept out of the fit, 10 to 20 percent at the
+// 95th percentile; equally large groups and one fit for both layouts had cost 2 percent (KMAJOR) and 8 (KROWS).
+struct GroupShape {
+    int rows, cols;
+    double a, c, fill;
+    int ends;
+    double rate;
+};
+template <class T, int BS>
+struct GroupShapes {
+    static constexpr bool H = sizeof(T) == 2, KC = BS == KMAJOR;
+    static constexpr int COLS = FewRows<T, BS>::COLS;
+    static constexpr GroupShape FEW1 = H ? KC ? GroupShape{16, COLS, 0.047, 0.052, 0, 22, 8.5} : GroupShape{16, COLS, 0, 0.128, 0, 32, 7.3}
+                                         : KC ? GroupShape{16, COLS, 0.035, 0.062, 0, 25, 9.1} : GroupShape{16, COLS, 0.050, 0.076, 0, 25, 7.9};
+    static constexpr GroupShape FEW2 = H ? KC ? GroupShape{32, COLS, 0.047, 0.041, 0.024, 25, 7.1} : GroupShape{32, COLS, 0.009, 0.101, 0.023, 46, 7.0}
+                                         : KC ? GroupShape{32, COLS, 0.050, 0.037, 0.031, 30, 7.5} : GroupShape{32, COLS, 0.056, 0.059, 0.035, 30, 7.7};
+    static constexpr GroupShape FEW4 = H ? KC ? GroupShape{64, COLS, 0.032, 0.053, 0.026, 37, 5.4} : GroupShape{64, COLS, 0.025, 0.059, 0.031, 61, 5.5}
+                                         : KC ? GroupShape{64, COLS, 0.033, 0.053, 0.029, 41, 6.2} : GroupShape{64, COLS, 0.018, 0.069, 0.051, 39, 7.1};
+    static constexpr GroupShape T64 = H ? KC ? GroupShape{64, 128, 0.100, 0.187, 0, 10, 6.9} : GroupShape{64, 128, 0.113, 0.151, 0, 12, 6.6}
+                                        : KC ? GroupShape{64, 64, 0.168, 0.231, 0, 8, 7.8} : GroupShape{64, 64, 0.143, 0.233, 0, 9, 7.6};
+    static constexpr GroupShape T128 = H ? KC ? GroupShape{128, 128, 0.071, 0.212, 0, 15, 7.3} : GroupShape{128, 128, 0.046, 0.219, 0, 15, 8.5}
+                                         : KC ? GroupShape{128, 128, 0.132, 0.909, 0, 5, 7.0} : GroupShape{128, 128, 0.145, 0.878, 0, 5, 6.4};
+    static constexpr GroupShape T256 = KC ? GroupShape{256, 256, -0.093, 0.521, 0, 15, 5.3} : GroupShape{256, 256, -0.211, 0.687, 0, 12, 6.7};
+};
+static double grouped_cost(const GroupShape &s, int T, int E, int K, int N, int size) {
+    const double groups = E < T ? E : T, k_bytes = (double)K * size, cus = machine().cus, per = T / groups;
+    const double row_tiles = groups == 1 ? std::ceil(per / s.rows) : groups * std::max(1.0, per / s.rows + 0.5);
+    const double share = row_tiles * ((N + s.cols - 1) / s.cols) / cus, n = std::max(1.0, groups == 1 ? std::ceil(share) : share + 0.3);
+    const double work = (k_bytes / 64 + s.ends) * (s.a + n * (s.c + s.fill * std::min((double)s.rows, T / row_tiles) / 16));
+    const double reads = groups * k_bytes * N / (s.rate * 1e6);
+    return std::max(work, reads) + 0.25 * std::min(work, reads);
+}
+
 template <class T, class O, int BS>
 static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
-    constexpr int size = sizeof(T), cols = FewRows<T, BS>::COLS;
-    constexpr bool kc = BS == KMAJOR;
-    const int64_t groups = g.E < g.T ? g.E : g.T, per = (g.T + groups - 1) / groups, k_bytes = (int64_t)g.K * size;
-    const double bytes = (double)groups * k_bytes * g.N;
-    auto cost = [&](const TileShape &s, double rate) {
-        const double c = tiles_cost(s, groups, per, g.N, k_bytes), h = bytes / (rate * 1e6);
-        return c > h ? c + 0.25 * h : h + 0.25 * c;
-    };
-    const double few1 = cost({16, cols, kc ? 0.06 : 0.14, kc ? 0.09 : 0.07}, kc ? 4.65 : 4.6),
-                 few2 = cost({32, cols, kc ? 0.06 : 0.14, kc ? 0.13 : 0.11}, kc ? 4.7 : 4.6),
-                 few4 = cost({64, cols, kc ? 0.06 : 0.14, kc ? 0.25 : 0.24}, kc ? 4.1 : 4.6);
-    const double c256 = size == 2 ? cost(SHAPE_256, kc ? 4.2 : 5.9) : 1e30, c128 = cost(size == 2 ? SHAPE_128 : SHAPE_128F, kc ? 4.7 : 5.6),
-                 c64 = cost(size == 2 ? SHAPE_64 : SHAPE_64F, kc ? 4.9 : 5.3);
-    const double best = std::min({few1, few2, few4, c256, c128, c64});
+    typedef GroupShapes<T, BS> S;
+    auto cost = [&](const GroupShape &s) { return grouped_cost(s, g.T, g.E, g.K, g.N, sizeof(T)); };
+    const double few1 = cost(S::FEW1), few2 = cost(S::FEW2), few4 = cost(S::FEW4), c64 = cost(S::T64), c128 = cost(S::T128),
+                 c256 = sizeof(T) == 2 ? cost(S::T256) : 1e30;
+    const double best = std::min({few1, few2, few4, c64, c128, c256});
     if (best == few1) return launch_few_rows<T, O, BS, 1>(g, stream);
     if (best == few2) return launch_few_rows<T, O, BS, 2>(g, stream);
     if (best == few4) return launch_few_rows<T, O, BS, 4>(g, stream);
-    if constexpr (size == 2)
+    if constexpr (sizeof(T) == 2)
         if (best == c256) return launch_forward<Tile256<T, KMAJOR, BS>, O>(g, stream);
     if (best == c128) return launch_forward<Tile128<T, KMAJOR, BS>, O>(g, stream);
     return launch_forward<Tile64<T, BS>, O>(g, stream);
