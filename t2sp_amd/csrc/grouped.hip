@@ -410,13 +410,14 @@ static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
     return launched();
 }
 
-// What a product takes in each form (microseconds), from the extents alone: groups of T / E rows make half a row tile more than
-// whole ones would (their sizes differ), the workgroups share the CUs, n to a CU, and a stage of 64 bytes of k takes
-// a + n (c + fill x the 16-row blocks that hold rows); `ends` stages go into start and store.  Beside that stands the reading of the
-// matrices at `rate` TB/s: the larger of the two and a quarter of the smaller.  Fitted to 350 products of 16-bit elements a
-// layout and 300 of floats (4 to 8192 rows in 1 to 64 groups of any sizes, 64 to 4096 x 64 to 4096): the form picked took 1.5
-// percent more than the best of the six (floats, KMAJOR: 3), geometric mean over those kept out of the fit, 10 to 20 percent at the
-// 95th percentile; equally large groups and one fit for both layouts had cost 2 percent (KMAJOR) and 8 (KROWS).
+// What a product takes in each form (microseconds), from the extents alone: as if every row chose its group freely, so that
+// E (1 - exp(-T / E)) groups have rows, and their ends make half a row tile more than whole tiles would.  The workgroups share
+// the CUs, n to a CU, and a stage of 64 bytes of k takes a + n (c + fill x the 16-row blocks that hold rows); `ends` stages go
+// into start and store.  Beside that stands the reading of the matrices at `rate` TB/s: the larger of the two and a quarter of
+// the smaller.  Fitted to 600 products of 16-bit elements a layout and 500 of floats (1 to 8192 rows in 1 to 64 groups of any sizes,
+// 64 to 4096 x 64 to 4096, matrices not in the caches).  Of those kept out of the fit, the form picked took 1 to 3 percent
+// more than the best of the six (geometric mean) and 6 to 16 at the 95th percentile; equally large groups and fewer
+// constants had cost 3 to 7 percent and 13 to 32.
 struct GroupShape {
     int rows, cols;
     double a, c, fill;
@@ -427,22 +428,22 @@ template <class T, int BS>
 struct GroupShapes {
     static constexpr bool H = sizeof(T) == 2, KC = BS == KMAJOR;
     static constexpr int COLS = FewRows<T, BS>::COLS;
-    static constexpr GroupShape FEW1 = H ? KC ? GroupShape{16, COLS, 0.047, 0.052, 0, 22, 8.5} : GroupShape{16, COLS, 0, 0.128, 0, 32, 7.3}
-                                         : KC ? GroupShape{16, COLS, 0.035, 0.062, 0, 25, 9.1} : GroupShape{16, COLS, 0.050, 0.076, 0, 25, 7.9};
-    static constexpr GroupShape FEW2 = H ? KC ? GroupShape{32, COLS, 0.047, 0.041, 0.024, 25, 7.1} : GroupShape{32, COLS, 0.009, 0.101, 0.023, 46, 7.0}
-                                         : KC ? GroupShape{32, COLS, 0.050, 0.037, 0.031, 30, 7.5} : GroupShape{32, COLS, 0.056, 0.059, 0.035, 30, 7.7};
-    static constexpr GroupShape FEW4 = H ? KC ? GroupShape{64, COLS, 0.032, 0.053, 0.026, 37, 5.4} : GroupShape{64, COLS, 0.025, 0.059, 0.031, 61, 5.5}
-                                         : KC ? GroupShape{64, COLS, 0.033, 0.053, 0.029, 41, 6.2} : GroupShape{64, COLS, 0.018, 0.069, 0.051, 39, 7.1};
-    static constexpr GroupShape T64 = H ? KC ? GroupShape{64, 128, 0.100, 0.187, 0, 10, 6.9} : GroupShape{64, 128, 0.113, 0.151, 0, 12, 6.6}
-                                        : KC ? GroupShape{64, 64, 0.168, 0.231, 0, 8, 7.8} : GroupShape{64, 64, 0.143, 0.233, 0, 9, 7.6};
-    static constexpr GroupShape T128 = H ? KC ? GroupShape{128, 128, 0.071, 0.212, 0, 15, 7.3} : GroupShape{128, 128, 0.046, 0.219, 0, 15, 8.5}
-                                         : KC ? GroupShape{128, 128, 0.132, 0.909, 0, 5, 7.0} : GroupShape{128, 128, 0.145, 0.878, 0, 5, 6.4};
-    static constexpr GroupShape T256 = KC ? GroupShape{256, 256, -0.093, 0.521, 0, 15, 5.3} : GroupShape{256, 256, -0.211, 0.687, 0, 12, 6.7};
+    static constexpr GroupShape FEW1 = H ? KC ? GroupShape{16, COLS, 0.046, 0.058, 0, 19, 8.9} : GroupShape{16, COLS, 0, 0.129, 0, 36, 5.9}
+                                         : KC ? GroupShape{16, COLS, 0.031, 0.063, 0, 28, 8.7} : GroupShape{16, COLS, 0.048, 0.085, 0, 22, 6.5};
+    static constexpr GroupShape FEW2 = H ? KC ? GroupShape{32, COLS, 0.048, 0.050, 0.023, 23, 7.4} : GroupShape{32, COLS, 0, 0.118, 0.021, 45, 5.8}
+                                         : KC ? GroupShape{32, COLS, 0.039, 0.052, 0.027, 27, 7.4} : GroupShape{32, COLS, 0.037, 0.091, 0.030, 25, 6.9};
+    static constexpr GroupShape FEW4 = H ? KC ? GroupShape{64, COLS, 0.027, 0.066, 0.024, 35, 5.5} : GroupShape{64, COLS, 0, 0.098, 0.035, 56, 5.4}
+                                         : KC ? GroupShape{64, COLS, 0.017, 0.070, 0.032, 37, 5.7} : GroupShape{64, COLS, 0, 0.101, 0.044, 37, 6.5};
+    static constexpr GroupShape T64 = H ? KC ? GroupShape{64, 128, 0.049, 0.248, 0, 8, 6.0} : GroupShape{64, 128, 0.091, 0.165, 0, 12, 6.4}
+                                        : KC ? GroupShape{64, 64, 0.153, 0.234, 0, 9, 7.8} : GroupShape{64, 64, 0.134, 0.232, 0, 9, 8.0};
+    static constexpr GroupShape T128 = H ? KC ? GroupShape{128, 128, 0.026, 0.253, 0, 14, 5.8} : GroupShape{128, 128, 0.015, 0.233, 0, 17, 8.5}
+                                         : KC ? GroupShape{128, 128, 0.008, 0.958, 0, 6, 6.9} : GroupShape{128, 128, 0.062, 0.923, 0, 5, 7.0};
+    static constexpr GroupShape T256 = KC ? GroupShape{256, 256, -0.171, 0.625, 0, 13, 5.6} : GroupShape{256, 256, -0.139, 0.548, 0, 17, 8.1};
 };
 static double grouped_cost(const GroupShape &s, int T, int E, int K, int N, int size) {
-    const double groups = E < T ? E : T, k_bytes = (double)K * size, cus = machine().cus, per = T / groups;
-    const double row_tiles = groups == 1 ? std::ceil(per / s.rows) : groups * std::max(1.0, per / s.rows + 0.5);
-    const double share = row_tiles * ((N + s.cols - 1) / s.cols) / cus, n = std::max(1.0, groups == 1 ? std::ceil(share) : share + 0.3);
+    const double groups = E == 1 ? 1 : E * (1 - std::exp(-(double)T / E)), k_bytes = (double)K * size, cus = machine().cus, per = T / groups;
+    const double row_tiles = E == 1 ? std::ceil(per / s.rows) : groups * std::max(1.0, per / s.rows + 0.5);
+    const double share = row_tiles * ((N + s.cols - 1) / s.cols) / cus, n = std::max(1.0, E == 1 ? std::ceil(share) : share + 0.3);
     const double work = (k_bytes / 64 + s.ends) * (s.a + n * (s.c + s.fill * std::min((double)s.rows, T / row_tiles) / 16));
     const double reads = groups * k_bytes * N / (s.rate * 1e6);
     return std::max(work, reads) + 0.25 * std::min(work, reads);
