@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "machine.hpp"
@@ -33,14 +35,19 @@ inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 int launch_pad_rows(const void *src, void *dst, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t batch_stride,
                     int size, hipStream_t stream);
 
+// out[e][r][0 .. cols) = sum over parts of plane[part][e * rows + r][0 .. cols), in their order; rows of planes have ldp elements, a
+// multiple of four.
+int launch_join_planes(const float *planes, int parts, int64_t batch, int64_t rows, int64_t cols, int64_t ldp, void *out, int out_type,
+                       int64_t ldo, int64_t batch_stride, hipStream_t stream);
+
 template <class K> int allow_lds(K kern, int bytes) {
     if (bytes <= 64 * 1024) return T2SP_OK;
     return hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess ? T2SP_OK
                                                                                                                : T2SP_ERR_LAUNCH;
 }
 // Time in microseconds of a product in tiles, for choosing among tile shapes: `tiles` workgroups share the CUs, n to a
-// CU, and a stage of 64 bytes of k then takes a + c n (fitted to sweeps of 1 to 1024 rows in 1 to 32 groups,
-// 2048 x 1024 to 4096 x 2048; what it picks is within a tenth of the best shape there but for a few sizes at the borders).
+// CU, and a stage of 64 bytes of k then takes a + c n (fitted to sweeps of 1 to 4096 rows,
+// k 512 to 4096, 1000 to 20000 columns; what it picks is within a tenth of the best shape there but for a few sizes at the borders).
 struct TileShape {
     int rows, cols;
     double a, c;
@@ -66,6 +73,15 @@ inline int pick_tile(int64_t groups, int64_t rows, int64_t cols, int64_t k, int 
     const double c128 = tiles_cost(size == 2 ? SHAPE_128 : SHAPE_128F, groups, rows, cols, k * size);
     const double c64 = small ? tiles_cost(size == 2 ? SHAPE_64 : SHAPE_64F, groups, rows, cols, k * size) : 1e30;
     return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+}
+
+// Parts that a reduction of `stages` stages is cut into when its output has fewer tiles than the `slots` workgroups that run at
+// once: their planes of partial sums cost a write and a read at about 4 TB/s, a stage `unit` microseconds, the kernel
+// that joins them four; a part has at least four stages.
+inline int split_parts(int64_t tiles, int64_t slots, double stages, double unit, double plane_bytes) {
+    const double plane = plane_bytes / 2e6, most = std::min((double)(slots / (tiles > 0 ? tiles : 1)), stages / 4);
+    const double parts = std::floor(std::min(most, std::sqrt(stages * unit / plane)));
+    return parts >= 2 && stages * unit * (1 - 1 / parts) > 4 + parts * plane ? (int)parts : 1;
 }
 
 // f(element type, result type) as null pointers, for a pair that out_type_ok accepts.

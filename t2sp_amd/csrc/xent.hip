@@ -245,23 +245,27 @@ struct XentProductArgs {
     int row_tiles, col_tiles, xcds;
     const float *scale;                  // dW: max |dloss|
     float by;
-    int splits;                          // dH: the reduction in this many parts, each with a plane of floats
+    int splits;                          // the reduction in this many parts, each (dW: if more than one) with a plane of floats
     int64_t plane;
     int add;                             // dH: add to the planes (a later piece of the vocabulary)
 };
 
-// dW[v0 + m, n] = scale * sum_t G[t, m] Hz[t, n]
+// dW[v0 + m, n] = scale * sum_t G[t, m] Hz[t, n], or one of several planes with the sums over part of the tokens
 template <class P, class O>
 __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     int m0, n0;
-    panel_tile(die_run(blockIdx.x, gridDim.x, g.xcds), g.row_tiles, g.col_tiles, &m0, &n0);
+    const unsigned at = die_run(blockIdx.x, gridDim.x, g.xcds), tiles = (unsigned)g.row_tiles * g.col_tiles, s = at / tiles;
+    panel_tile(at % tiles, g.row_tiles, g.col_tiles, &m0, &n0);
     m0 *= P::BM;
     n0 *= P::BN;
-    const TileSource a{g.A + m0 * P::SZ, (uint32_t)(g.lda * P::SZ), g.a_cols - m0}, b{g.B + n0 * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
+    const int stages = (g.k + P::KS - 1) / P::KS, per = (stages + g.splits - 1) / g.splits * P::KS;
+    const int k0 = (int64_t)s * per < g.k ? (int)s * per : g.k, k = g.k - k0 < per ? g.k - k0 : per;
+    const TileSource a{g.A + (k0 * g.lda + m0) * P::SZ, (uint32_t)(g.lda * P::SZ), g.a_cols - m0},
+        b{g.B + (k0 * g.ldb + n0) * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
     pv4f acc[P::MT][P::NT];
     clear<P>(acc);
-    product_run<P>(a, b, g.k, smem, acc);
+    if (k > 0) product_run<P>(a, b, k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = n0 + (wave % P::WN) * P::TN;
     const float by = *g.scale * g.by;
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
         if (m >= g.rows) continue;
 #pragma unroll
         for (int j = 0; j < P::NT; j++) acc[i][j] *= by;
-        store_row<P, O>(g.out + m * g.ldo * (int64_t)sizeof(O), n, g.cols, acc[i]);
+        store_row<P, O>(g.out + (s * g.plane + m * g.ldo) * (int64_t)sizeof(O), n, g.cols, acc[i]);
     }
 }
 
@@ -338,10 +342,10 @@ __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, 
 struct XentRoom {
     size_t h, w;                         // padded copies of H and W (0: read where they lie)
     size_t part, hit;                    // forward
-    size_t scale, hz, g, planes;         // backward
+    size_t scale, hz, g, planes, dw;     // backward
     size_t total;
     int64_t ldd;                         // elements per row of hz and of the planes
-    int piece, splits;
+    int piece, splits, dw_parts;
 };
 
 constexpr size_t ROOM_ALIGN = 256;
@@ -361,9 +365,15 @@ static int dh_splits(int T, int D, int piece, int size) {
     if (T == 0) return 1;
     const int bm = dh_tile(T, size), bn = tile_cols(bm, size), per_cu = bm == 256 ? 1 : bm == 128 ? 2 : 3;
     const int64_t tiles = (int64_t)((T + bm - 1) / bm) * ((D + bn - 1) / bn), slots = (int64_t)machine().cus * per_cu;
-    int64_t s = slots / tiles;
-    if (s > piece / 512) s = piece / 512;
-    return s < 1 ? 1 : (int)s;
+    const TileShape &s = size == 4 ? (bm == 128 ? SHAPE_128F : SHAPE_64F) : bm == 256 ? SHAPE_256 : bm == 128 ? SHAPE_128 : SHAPE_64;
+    return split_parts(tiles, slots, (double)piece * size / 64, s.a + s.c * per_cu, 4.0 * T * D);
+}
+// The parts that the sums over tokens are cut into when dW has few tiles.  (Both gradients and the loss of 3155 tokens, 64 wide, 709
+// words, float: 297 us whole, 74 in parts)
+static int dw_splits(int T, int D, int piece, int size) {
+    const TileShape &s = size == 2 ? SHAPE_128 : SHAPE_128F;
+    const int64_t tiles = (int64_t)((piece + 127) / 128) * ((D + 127) / 128);
+    return split_parts(tiles, machine().cus, (double)T * size / 64, s.a + s.c, 4.0 * piece * D);
 }
 
 static XentRoom xent_room(bool backward, int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
@@ -393,6 +403,8 @@ static XentRoom xent_room(bool backward, int type, const void *H, const void *W,
         r.hz = take((size_t)T * r.ldd * size);
         r.g = take((size_t)T * padded_cols(piece, size) * size);
         r.planes = take((size_t)r.splits * T * r.ldd * sizeof(float));
+        r.dw_parts = dw_splits(T, D, r.piece, size);
+        r.dw = take(r.dw_parts > 1 ? (size_t)r.dw_parts * r.piece * r.ldd * sizeof(float) : 0);
     }
     r.total = at;
     return r;
@@ -442,7 +454,7 @@ template <class P> static int launch_probabilities(XentArgs g, hipStream_t st) {
 template <class P, class O> static int launch_dw(XentProductArgs g, hipStream_t st) {
     g.row_tiles = (g.rows + P::BM - 1) / P::BM;
     g.col_tiles = (g.cols + P::BN - 1) / P::BN;
-    T2SP_LAUNCH_TILES(P, (xent_dw_kernel<P, O>), (int64_t)g.row_tiles * g.col_tiles, st, g);
+    T2SP_LAUNCH_TILES(P, (xent_dw_kernel<P, O>), (int64_t)g.row_tiles * g.col_tiles * g.splits, st, g);
 }
 template <class P> static int launch_dh(XentProductArgs g, hipStream_t st) {
     g.row_tiles = (g.rows + P::BM - 1) / P::BM;
@@ -467,8 +479,8 @@ static int xent_forward(XentArgs g, float *loss, float *lse, hipStream_t st) {
 }
 
 template <class T, class O>
-static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *H, int64_t ldh, void *dH, void *dW, int64_t lddh, int64_t lddw,
-                         hipStream_t st) {
+static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *H, int64_t ldh, void *dH, void *dW, int out_type, int64_t lddh,
+                         int64_t lddw, hipStream_t st) {
     constexpr int size = sizeof(T);
     const float by = 1.f / GradientScale<T>::value;
     float *scale = reinterpret_cast<float *>(room + r.scale), *planes = reinterpret_cast<float *>(room + r.planes);
@@ -503,8 +515,16 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
             p.out = static_cast<char *>(dW) + v0 * lddw * (int64_t)sizeof(O); p.ldo = lddw;
             p.rows = g.vp; p.cols = g.D; p.k = g.T;
             p.scale = scale; p.by = by;
-            err = pick_tile(1, p.rows, p.cols, p.k, size, false) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
-                                                                      : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
+            p.splits = r.dw_parts;
+            if (r.dw_parts > 1) {
+                char *const out = p.out;
+                p.out = room + r.dw; p.ldo = r.ldd; p.plane = p.rows * p.ldo;
+                if (!(err = launch_dw<Tile128<T, KROWS, KROWS>, float>(p, st)))
+                    err = launch_join_planes(reinterpret_cast<const float *>(room + r.dw), p.splits, 1, p.rows, p.cols, p.ldo, out, out_type, lddw, 0, st);
+            } else {
+                err = pick_tile(1, p.rows, p.cols, p.k, size, false) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
+                                                                          : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
+            }
             if (err) return err;
         }
         if (dH && g.T) {
@@ -581,6 +601,6 @@ extern "C" int t2sp_xent_grad(int type, int out_type, const void *H, const void 
     if (T)
         if (int err = xent_operands(g, r, type_bytes(type), room, H, W, ldh, ldw, st)) return err;
     return with_types(type, out_type, [&](auto *t, auto *o) {
-        return xent_backward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, r, room, H, ldh, dH, dW, lddh, lddw, st);
+        return xent_backward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, r, room, H, ldh, dH, dW, out_type, lddh, lddw, st);
     });
 }

@@ -190,6 +190,25 @@ def test_large_tiles_and_uneven_groups():
     check_wgrad(X, D, sizes)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes,K,N", [([4100], 128, 64), ([3000, 0, 1, 500], 96, 200), ([33, 2500], 65, 41), ([15, 1, 2000, 0, 900], 8, 9)])
+def test_small_matrices_from_many_rows(dtype, sizes, K, N):
+    """Sums over the rows in parts: empty groups, groups shorter than a part, rows off the vector grid, results in a strided view, which
+    keeps what lies around it, float results of 16-bit operands, and the same bits every time."""
+    import torch
+    E, T = len(sizes), sum(sizes)
+    X, D = make((T + 7, K), dtype, 50), make((T + 7, N), dtype, 51)
+    check_wgrad(X, D, sizes, 3)
+    check_wgrad(X, D, sizes, 3, out_dtype=torch.float32)
+    whole = torch.full((E, K + 2, N + 3), 7.0, dtype=dt(dtype), device="cuda")
+    check_wgrad(X, D, sizes, 3, out=whole[:, 1:K + 1, 2:N + 2])
+    inside = torch.zeros_like(whole, dtype=torch.bool)
+    inside[:, 1:K + 1, 2:N + 2] = True
+    assert (whole[~inside] == 7.0).all()
+    again = t2sp_amd.gemm_grouped_wgrad(X, D, offs(sizes, 3))
+    assert torch.equal(again, whole[:, 1:K + 1, 2:N + 2])
+
+
 def test_no_rows():
     import torch
     X, W = make((0, 64), "bfloat16", 30), make((2, 64, 64), "bfloat16", 31)

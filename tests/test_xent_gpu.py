@@ -126,6 +126,16 @@ def test_widths_off_the_vector_grid(dtype, T, V, D):
     check(make((T, D), dtype, 5), make((V, D), dtype, 6, D ** -0.5), lab, mean_of(lab, V))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(2100, 300, 64), (1500, 709, 65), (4000, 3, 8)])
+def test_many_tokens_and_a_small_matrix(dtype, T, V, D):
+    """The gradient of W as sums over parts of the tokens."""
+    lab = labels_for(T, V, 40, 0.3)
+    check(make((T, D), dtype, 41), make((V, D), dtype, 42, 2.0 * D ** -0.5), lab, mean_of(lab, V))
+    if dtype != "float32":
+        check(make((T, D), dtype, 41), make((V, D), dtype, 42, 2.0 * D ** -0.5), lab, mean_of(lab, V), out_dtype=dt("float32"))
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_strided_and_unaligned_views(dtype):
     import torch
