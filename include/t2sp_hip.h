@@ -317,8 +317,9 @@ int t2sp_capsule_packed_f32(const float *P2, int64_t ldp, const float *W2, int64
  * are clamped to 0 .. T, so that no value leads outside the buffers.  sw: elements between the matrices.
  * Every result element is one sum in a fixed order, whatever the group sizes.
  * Operands whose rows are not whole 16-byte chunks (pointer, leading dimension, extent) are first copied
- * to padded rows in `workspace` (16-byte aligned; t2sp_gemm_grouped*_workspace_bytes, 0 when nothing needs
- * a copy): with less room the call is refused with T2SP_ERR_SHAPE.  E * rows of a matrix is at most T2SP_MAX_EXTENT. */
+ * to padded rows in `workspace`, and t2sp_gemm_grouped_wgrad sums few small matrices in parts, as planes of floats
+ * there (16-byte aligned; t2sp_gemm_grouped*_workspace_bytes, 0 when nothing of this applies): with less room the
+ * call is refused with T2SP_ERR_SHAPE.  E * rows of a matrix is at most T2SP_MAX_EXTENT. */
 size_t t2sp_gemm_grouped_workspace_bytes(int type, int opb, const void *X, const void *W, int T, int E, int K, int N,
                                          int64_t ldx, int64_t ldw, int64_t sw);
 int t2sp_gemm_grouped(int type, int out_type, int opb, const void *X, const void *W, const void *offsets,
