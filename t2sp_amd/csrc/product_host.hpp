@@ -31,9 +31,14 @@ inline bool row_ok(int64_t e, int size) { return e >= 1 && e * size <= T2SP_MAX_
 inline int64_t padded_cols(int64_t cols, int size) { return (cols * size + 15) / 16 * 16 / size; }
 inline size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-// dst[b][r][0 .. padded) = src[b][r][0 .. cols), zeros behind: dense rows of whole 16-byte chunks.
-int launch_pad_rows(const void *src, void *dst, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t batch_stride,
-                    int size, hipStream_t stream);
+// dst[b][r][0 .. padded) = src[b][r][0 .. cols), zeros behind: dense rows of whole 16-byte chunks.  Two copies in one launch; one
+// that is not needed has no rows.
+struct PadRows {
+    const void *src;
+    void *dst;
+    int64_t batch, rows, cols, ld, batch_stride;
+};
+int launch_pad_rows(const PadRows &a, const PadRows &b, int size, hipStream_t stream);
 
 // out[e][r][0 .. cols) = sum over parts of plane[part][e * rows + r][0 .. cols), in their order; rows of planes have ldp elements, a
 // multiple of four.

@@ -148,12 +148,14 @@ __global__ void __launch_bounds__(64 * JOIN_WAVES) xent_join_kernel(const float2
     }
 }
 
-// max |dloss| over the tokens with a label.
-__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *dloss, const void *labels, int lab64, int T, int V, float *scale) {
-    __shared__ float joint[16];
+// max |dloss| over the tokens with a label, NaN if one of them is not finite; in every thread of a workgroup.
+template <int THREADS>
+__device__ __forceinline__ float largest_weight(const float *dloss, const void *labels, int lab64, int T, int V) {
+    constexpr int WAVES = THREADS / 64;
+    __shared__ float joint[WAVES];
     float top = 0.f;
     bool bad = false;
-    for (int t = threadIdx.x; t < T; t += 1024) {
+    for (int t = threadIdx.x; t < T; t += THREADS) {
         const int64_t label = label_of(labels, lab64, t);
         if (label >= 0 && label < V) {
             const float v = fabsf(dloss[t]);
@@ -166,26 +168,34 @@ __global__ void __launch_bounds__(1024) xent_scale_kernel(const float *dloss, co
     if (__ballot(bad)) top = __builtin_nanf("");
     if ((threadIdx.x & 63) == 0) joint[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float all = 0.f;
-        for (int w = 0; w < 16; w++) all = joint[w] != joint[w] || all != all ? __builtin_nanf("") : fmaxf(all, joint[w]);
-        *scale = all;
-    }
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) all = joint[w] != joint[w] || all != all ? __builtin_nanf("") : fmaxf(all, joint[w]);
+    return all;
+}
+__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *dloss, const void *labels, int lab64, int T, int V, float *scale) {
+    const float all = largest_weight<1024>(dloss, labels, lab64, T, V);
+    if (threadIdx.x == 0) *scale = all;
 }
 
 // Hz[t, :] = H[t, :] * (dloss[t] / max |dloss|) rounded to the type, zeros for tokens without a label and from D to ld.
-template <class T>
+// FIND: the workgroups look for the maximum themselves, for the kernels behind too (up to FIND_ROWS tokens; a launch less, about 3 us
+// of the host's time).
+constexpr int FIND_ROWS = 2048;
+template <class T, bool FIND>
 __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int64_t ldh, const void *labels, int lab64, const float *dloss,
-                                                                 const float *scale, int rows, int V, int D, T *Hz, int64_t ld, int64_t chunks) {
+                                                                 float *scale, int rows, int V, int D, T *Hz, int64_t ld, int64_t chunks) {
     constexpr int CE = 16 / sizeof(T);
     typedef T chunk __attribute__((ext_vector_type(CE)));
     const int64_t per = ld / CE;
+    const float top = FIND ? largest_weight<256>(dloss, labels, lab64, rows, V) : *scale;
+    if (FIND && blockIdx.x == 0 && threadIdx.x == 0) *scale = top;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int t = (int)(i / per), c = (int)(i % per) * CE;
         const int64_t label = label_of(labels, lab64, t);
         chunk v;
         if (label >= 0 && label < V) {
-            const float by = *scale == 0.f ? 0.f : dloss[t] / *scale;
+            const float by = top == 0.f ? 0.f : dloss[t] / top;
             const T *s = H + t * ldh + c;
             if (c + CE <= D) {
                 v = *reinterpret_cast<const typename Chunk<T>::anywhere *>(s);
@@ -420,15 +430,16 @@ static int xent_operands(XentArgs &g, const XentRoom &r, int size, char *room, c
                          hipStream_t st) {
     g.H = static_cast<const char *>(H); g.W = static_cast<const char *>(W);
     g.ldh = ldh; g.ldw = ldw;
+    PadRows ph{}, pw{};
     if (r.h != (size_t)-1) {
-        if (int err = launch_pad_rows(H, room + r.h, 1, g.T, g.D, ldh, 0, size, st)) return err;
+        ph = {H, room + r.h, 1, g.T, g.D, ldh, 0};
         g.H = room + r.h; g.ldh = r.ldd;
     }
     if (r.w != (size_t)-1) {
-        if (int err = launch_pad_rows(W, room + r.w, 1, g.V, g.D, ldw, 0, size, st)) return err;
+        pw = {W, room + r.w, 1, g.V, g.D, ldw, 0};
         g.W = room + r.w; g.ldw = r.ldd;
     }
-    return T2SP_OK;
+    return launch_pad_rows(ph, pw, size, st);
 }
 
 #define T2SP_LAUNCH_TILES(P, kern, blocks, st, g)                                              \
@@ -486,11 +497,15 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
     float *scale = reinterpret_cast<float *>(room + r.scale), *planes = reinterpret_cast<float *>(room + r.planes);
     int err;
     if (dW) {
-        hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, g.dloss, g.labels, g.lab64, g.T, g.V, scale);
-        if ((err = launched())) return err;
         const int64_t chunks = (int64_t)g.T * r.ldd * size / 16;
+        const bool find = chunks && g.T <= FIND_ROWS;
+        if (!find) {
+            hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, g.dloss, g.labels, g.lab64, g.T, g.V, scale);
+            if ((err = launched())) return err;
+        }
         if (chunks) {
-            hipLaunchKernelGGL(xent_weighted_rows_kernel<T>, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
+            auto kern = find ? xent_weighted_rows_kernel<T, true> : xent_weighted_rows_kernel<T, false>;
+            hipLaunchKernelGGL(kern, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
                                static_cast<const T *>(H), ldh, g.labels, g.lab64, g.dloss, scale, g.T, g.V, g.D,
                                reinterpret_cast<T *>(room + r.hz), r.ldd, chunks);
             if ((err = launched())) return err;
