@@ -519,7 +519,7 @@ static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
 // (8192 rows in one group, 512 x 512, bfloat16: 70 us whole, 22 in parts; float: 533 and 50)
 static int wgrad_parts(int T, int E, int K, int N, int size) {
     const TileShape &s = size == 2 ? SHAPE_128 : SHAPE_128F;
-    const int64_t tiles = (int64_t)E * ((K + 127) / 128) * ((N + 127) / 128);
+    const double tiles = (double)E * ((K + 127) / 128) * ((N + 127) / 128);      // (extents up to 2^30 each: beyond 64 bits)
     return split_parts(tiles, machine().cus, (double)T / E * size / 64, s.a + s.c, 4.0 * E * K * N);
 }
 static int64_t plane_cols(int N) { return (N + 3) / 4 * 4; }

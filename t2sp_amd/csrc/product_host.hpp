@@ -83,8 +83,8 @@ inline int pick_tile(int64_t groups, int64_t rows, int64_t cols, int64_t k, int 
 // Parts that a reduction of `stages` stages is cut into when its output has fewer tiles than the `slots` workgroups that run at
 // once: their planes of partial sums cost a write and a read at about 4 TB/s, a stage `unit` microseconds, the kernel
 // that joins them four; a part has at least four stages.
-inline int split_parts(int64_t tiles, int64_t slots, double stages, double unit, double plane_bytes) {
-    const double plane = plane_bytes / 2e6, most = std::min((double)(slots / (tiles > 0 ? tiles : 1)), stages / 4);
+inline int split_parts(double tiles, int64_t slots, double stages, double unit, double plane_bytes) {
+    const double plane = plane_bytes / 2e6, most = std::min(std::floor((double)slots / std::max(tiles, 1.0)), stages / 4);
     const double parts = std::floor(std::min(most, std::sqrt(stages * unit / plane)));
     return parts >= 2 && stages * unit * (1 - 1 / parts) > 4 + parts * plane ? (int)parts : 1;
 }

@@ -182,3 +182,13 @@ def test_tables_and_argv_forms():
         assert getattr(L, fn + "_argv")(None) == -12
     arr = (ctypes.c_void_p * 4)(None, None, None, None)
     assert L.gemm_grouped_wgrad_argv(arr) == -12
+
+
+def test_workspace_of_the_matrices_gradient():
+    """Planes for sums in parts (few small matrices, many rows); none for many tiles or few rows, up to the largest extents."""
+    L, big = t2sp_amd.lib(), 1 << 30
+    size = lambda T, E, K, N: L.t2sp_gemm_grouped_wgrad_workspace_bytes(BF16, P, P, T, E, K, N, K, N)
+    parts, rest = divmod(size(8192, 1, 512, 512), 512 * 512 * 4)
+    assert parts >= 2 and rest == 0
+    assert size(8192, 64, 2048, 2048) == 0 and size(64, 1, 512, 512) == 0 and size(0, 1, 512, 512) == 0
+    assert size(0, big, big, big) == 0
