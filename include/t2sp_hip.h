@@ -339,9 +339,12 @@ int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, const void *d
  * `labels` are integers of `label_bits` = 32 or 64.  A token whose label is outside 0 .. V - 1 (padding, a
  * prompt) has loss 0, a row of zeros in dH and no part in dW, whatever its rows of H and dloss hold.
  * loss, lse and dloss are float, one per token; a mean's gradient is dloss = 1 / number of tokens.
- * The gradient works through the vocabulary in pieces: p - [label] of one piece, rounded to `type`, passes
- * through the workspace (16-byte aligned, t2sp_xent*_workspace_bytes, required), as do padded copies of
- * operands whose rows are not whole 16-byte chunks.  Sums are in float and in a fixed order. */
+ * The gradient works through the vocabulary in pieces: p - [label] of one piece passes through the workspace
+ * (16-byte aligned, t2sp_xent*_workspace_bytes, required), as do padded copies of operands whose rows are not
+ * whole 16-byte chunks.  16-bit types: p - [label] enters the products as the sum of two numbers of `type`, 16
+ * (bfloat16) or 22 (half) bits of it, which leaves less than the float sums of z do.  t2sp_xent_grad_rounded is the
+ * same call with p - [label] rounded to one number of `type`: a third to two fifths less time, and an error of half
+ * a step of the type in every p - [label] (float: no difference).  Sums are in float and in a fixed order. */
 size_t t2sp_xent_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw);
 int t2sp_xent(int type, const void *H, const void *W, const void *labels, int label_bits, float *loss, float *lse,
               int T, int V, int D, int64_t ldh, int64_t ldw, void *workspace, size_t workspace_bytes, void *stream);
@@ -350,6 +353,10 @@ size_t t2sp_xent_grad_workspace_bytes(int type, const void *H, const void *W, in
 int t2sp_xent_grad(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits,
                    const float *lse, const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh,
                    int64_t ldw, int64_t lddh, int64_t lddw, void *workspace, size_t workspace_bytes, void *stream);
+int t2sp_xent_grad_rounded(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits,
+                           const float *lse, const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh,
+                           int64_t ldw, int64_t lddh, int64_t lddw, void *workspace, size_t workspace_bytes,
+                           void *stream);
 
 /* Products with 4-bit weights and group scales, for the few rows of tokens being decoded:
  *   y[m,n] = sum_k x[m,k] * (q[n,k] - z[n,k/group]) * s[n,k/group],  q in 0 .. 15, z = 8 without zero points

@@ -128,7 +128,8 @@ def _declare(L):
         getattr(L, name).argtypes = [i32, vp, vp, i32, i32, i32, i64, i64]
         getattr(L, name).restype = sz
     L.t2sp_xent.argtypes = [i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, i64, i64, vp, sz, vp]
-    L.t2sp_xent_grad.argtypes = [i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, vp, sz, vp]
+    for name in ("t2sp_xent_grad", "t2sp_xent_grad_rounded"):
+        getattr(L, name).argtypes = [i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, vp, sz, vp]
     L.t2sp_w4_sizes.argtypes = [i32, i32, i32, p64, p64]
     L.t2sp_w4_pack.argtypes = [i32, vp, vp, vp, i32, i32, i32, i32] + [i64] * 6 + [vp, vp, vp, vp]
     L.t2sp_gemv_w4.argtypes = [i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, vp]

@@ -10,10 +10,13 @@
 // to the workspace, 8 bytes per row and tile instead of 1024, and a second kernel joins them.
 //
 // Backward, for one piece of the vocabulary after the other: the tile of z is computed again, its epilogue writes
-// p - [label] rounded to the operands' type (the one rounding besides the results': it enters two matrix products on
-// the 16-bit matrix cores, and its relative error of at most half a step averages out over V or T terms); then the
-// piece's rows of dW (complete) and its part of dH (added up in float) are two more products.  8 T D V operations in
-// all, of which 2 T D V pay for not holding T x V logits.
+// p - [label], and the piece's rows of dW (complete) and its part of dH (added up in float) are two more products.
+// p - [label] is a float, which the 16-bit matrix cores do not take: it goes in as the sum of two numbers of the operands'
+// type, its rounding and the rounding of what that leaves (16 bits with bfloat16, 22 with half), and both products run over
+// both.  12 T D V operations in all, of which 2 T D V pay for not holding T x V logits and 4 T D V for the second number.
+// What they leave is below what the float sums of z do (2048 tokens, 4096 wide, 32000 words, bfloat16, float results: the
+// gradients are off by 8e-7 and 5e-7 in norm, by 2e-7 for the two numbers alone, by 1.1e-4 with one; a third number changes
+// nothing).  Callers who accept half a step of the type in p - [label] (t2sp_xent_grad_rounded) have one: 8 T D V.
 //
 // Scales.  dloss is kept out of the rounded matrix: dH's rows are multiplied by it at the end, and for dW it goes into
 // the rows of H, as dloss[t] / max |dloss| (exactly 1 in the usual case of equal weights: then the copy of H is exact).
@@ -37,8 +40,9 @@ struct XentArgs {
     float *hit;                          // [T]: z at the label
     // backward
     const float *lse, *dloss;
-    char *G;                             // [T][ldg] p - [label] of the piece, zeros from vp to ldg
+    char *G;                             // [numbers][T][ldg] p - [label] of the piece, zeros from vp to ldg
     int64_t ldg;
+    int numbers;                         // of the type that p - [label] is the sum of
     int v0, vp;                          // the piece: words v0 .. v0 + vp - 1
 };
 
@@ -242,7 +246,12 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
             const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (v == hot ? 1.f : 0.f);
             acc[i][c / 4][c % 4] = valid && v < g.vp ? p * GradientScale<T>::value : 0.f;
         }
-        store_row<P, T>(g.G + t * g.ldg * (int64_t)sizeof(T), n0 + (wave % P::WN) * P::TN, (int)g.ldg, acc[i]);
+        char *row = g.G + t * g.ldg * (int64_t)sizeof(T);
+        for (int j = 0; j < g.numbers; j++, row += g.T * g.ldg * (int64_t)sizeof(T)) {
+            store_row<P, T>(row, n0 + (wave % P::WN) * P::TN, (int)g.ldg, acc[i]);
+#pragma unroll
+            for (int c = 0; c < P::LANE_N; c++) acc[i][c / 4][c % 4] -= (float)(T)acc[i][c / 4][c % 4];
+        }
     }
 }
 
@@ -251,6 +260,8 @@ struct XentProductArgs {
     char *out;
     int64_t lda, ldb, ldo;               // elements
     int rows, cols, k;                   // of the result; the reduction
+    int numbers;                         // matrices that A is the sum of, `next` bytes apart
+    int64_t next;
     int a_cols, b_cols;                  // elements in a row of A (dW) and B, whole 16-byte chunks
     int row_tiles, col_tiles, xcds;
     const float *scale;                  // dW: max |dloss|
@@ -271,11 +282,12 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
     n0 *= P::BN;
     const int stages = (g.k + P::KS - 1) / P::KS, per = (stages + g.splits - 1) / g.splits * P::KS;
     const int k0 = (int64_t)s * per < g.k ? (int)s * per : g.k, k = g.k - k0 < per ? g.k - k0 : per;
-    const TileSource a{g.A + (k0 * g.lda + m0) * P::SZ, (uint32_t)(g.lda * P::SZ), g.a_cols - m0},
-        b{g.B + (k0 * g.ldb + n0) * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
+    TileSource a{g.A + (k0 * g.lda + m0) * P::SZ, (uint32_t)(g.lda * P::SZ), g.a_cols - m0};
+    const TileSource b{g.B + (k0 * g.ldb + n0) * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
     pv4f acc[P::MT][P::NT];
     clear<P>(acc);
-    if (k > 0) product_run<P>(a, b, k, smem, acc);
+    if (k > 0)
+        for (int i = 0; i < g.numbers; i++, a.p += g.next) product_run<P>(a, b, k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = n0 + (wave % P::WN) * P::TN;
     const float by = *g.scale * g.by;
@@ -300,11 +312,12 @@ __global__ void __launch_bounds__(P::THREADS) xent_dh_kernel(const XentProductAr
     n0 *= P::BN;
     const int stages = (g.k + P::KS - 1) / P::KS, per = (stages + g.splits - 1) / g.splits * P::KS;
     const int k0 = (int64_t)s * per < g.k ? (int)s * per : g.k, k = g.k - k0 < per ? g.k - k0 : per;
-    const TileSource a{g.A + (m0 * g.lda + k0) * P::SZ, (uint32_t)(g.lda * P::SZ), g.rows - m0},
-        b{g.B + (k0 * g.ldb + n0) * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
+    TileSource a{g.A + (m0 * g.lda + k0) * P::SZ, (uint32_t)(g.lda * P::SZ), g.rows - m0};
+    const TileSource b{g.B + (k0 * g.ldb + n0) * P::SZ, (uint32_t)(g.ldb * P::SZ), g.b_cols - n0};
     pv4f acc[P::MT][P::NT];
     clear<P>(acc);
-    if (k > 0) product_run<P>(a, b, k, smem, acc);
+    if (k > 0)
+        for (int i = 0; i < g.numbers; i++, a.p += g.next) product_run<P>(a, b, k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = n0 + (wave % P::WN) * P::TN;
 #pragma unroll
@@ -361,7 +374,10 @@ struct XentRoom {
 constexpr size_t ROOM_ALIGN = 256;
 constexpr int64_t G_BYTES = 128 << 20;   // of the piece of p - [label]: it then stays in the 256 MB cache between its
                                          // kernel and the two products that read it ...
-constexpr int MIN_PIECE = 4096;          // ... but a piece is long enough that adding up dH costs little beside it
+constexpr int MIN_PIECE = 4096;          // ... but a piece is long enough that adding up dH costs little beside it (beyond 8192
+                                         // tokens it is therefore larger than G_BYTES: 2 GB at 131072 tokens)
+// Numbers of the type that p - [label] takes.
+static int numbers_of(int type, bool rounded) { return type_bytes(type) == 2 && !rounded ? 2 : 1; }
 
 // The tile of the logits; 65536 exponentials are worth four stages (777 x 50001 x 1022, half: 129 us in 256 x 256 tiles, 120 in
 // 128 x 128; 2048 x 32000 x 2048, bfloat16: 238 us in 256 x 256 tiles).
@@ -371,22 +387,22 @@ static int tile_cols(int tile, int size) { return tile == 64 && size == 2 ? 128 
 
 // The tile of dH (the rows of T decide: its columns and the split fill the chip) and the parts of its reduction.
 static int dh_tile(int T, int size) { return T > 128 && size == 2 ? 256 : T > 64 ? 128 : 64; }
-static int dh_splits(int T, int D, int piece, int size) {
+static int dh_splits(int T, int D, int piece, int size, int numbers) {
     if (T == 0) return 1;
     const int bm = dh_tile(T, size), bn = tile_cols(bm, size), per_cu = bm == 256 ? 1 : bm == 128 ? 2 : 3;
     const int64_t tiles = (int64_t)((T + bm - 1) / bm) * ((D + bn - 1) / bn), slots = (int64_t)machine().cus * per_cu;
     const TileShape &s = size == 4 ? (bm == 128 ? SHAPE_128F : SHAPE_64F) : bm == 256 ? SHAPE_256 : bm == 128 ? SHAPE_128 : SHAPE_64;
-    return split_parts(tiles, slots, (double)piece * size / 64, s.a + s.c * per_cu, 4.0 * T * D);
+    return split_parts(tiles, slots, (double)piece * size * numbers / 64, s.a + s.c * per_cu, 4.0 * T * D);
 }
 // The parts that the sums over tokens are cut into when dW has few tiles.  (Both gradients and the loss of 3155 tokens, 64 wide, 709
 // words, float: 297 us whole, 74 in parts)
-static int dw_splits(int T, int D, int piece, int size) {
+static int dw_splits(int T, int D, int piece, int size, int numbers) {
     const TileShape &s = size == 2 ? SHAPE_128 : SHAPE_128F;
     const int64_t tiles = (int64_t)((piece + 127) / 128) * ((D + 127) / 128);
-    return split_parts(tiles, machine().cus, (double)T * size / 64, s.a + s.c, 4.0 * piece * D);
+    return split_parts(tiles, machine().cus, (double)T * size * numbers / 64, s.a + s.c, 4.0 * piece * D);
 }
 
-static XentRoom xent_room(bool backward, int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
+static XentRoom xent_room(bool backward, int numbers, int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
     const int size = type_bytes(type);
     XentRoom r{};
     r.ldd = padded_cols(D, size);
@@ -403,17 +419,17 @@ static XentRoom xent_room(bool backward, int type, const void *H, const void *W,
         r.part = take((size_t)((V + cols - 1) / cols) * T * sizeof(float2));
         r.hit = take((size_t)T * sizeof(float));
     } else {
-        int64_t piece = G_BYTES / ((int64_t)(T > 0 ? T : 1) * size) / 256 * 256;
+        int64_t piece = G_BYTES / ((int64_t)(T > 0 ? T : 1) * size * numbers) / 256 * 256;
         if (piece < MIN_PIECE) piece = MIN_PIECE;
         if (piece >= V) piece = V;
         else piece = round_up((V + (V + piece - 1) / piece - 1) / ((V + piece - 1) / piece), 256);     // equal pieces
         r.piece = (int)piece;
-        r.splits = dh_splits(T, D, r.piece, size);
+        r.splits = dh_splits(T, D, r.piece, size, numbers);
         r.scale = take(sizeof(float));
         r.hz = take((size_t)T * r.ldd * size);
-        r.g = take((size_t)T * padded_cols(piece, size) * size);
+        r.g = take((size_t)T * padded_cols(piece, size) * size * numbers);
         r.planes = take((size_t)r.splits * T * r.ldd * sizeof(float));
-        r.dw_parts = dw_splits(T, D, r.piece, size);
+        r.dw_parts = dw_splits(T, D, r.piece, size, numbers);
         r.dw = take(r.dw_parts > 1 ? (size_t)r.dw_parts * r.piece * r.ldd * sizeof(float) : 0);
     }
     r.total = at;
@@ -529,6 +545,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
             p.B = room + r.hz; p.ldb = r.ldd; p.b_cols = (int)r.ldd;
             p.out = static_cast<char *>(dW) + v0 * lddw * (int64_t)sizeof(O); p.ldo = lddw;
             p.rows = g.vp; p.cols = g.D; p.k = g.T;
+            p.numbers = g.numbers; p.next = g.T * g.ldg * (int64_t)size;
             p.scale = scale; p.by = by;
             p.splits = r.dw_parts;
             if (r.dw_parts > 1) {
@@ -537,7 +554,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
                 if (!(err = launch_dw<Tile128<T, KROWS, KROWS>, float>(p, st)))
                     err = launch_join_planes(reinterpret_cast<const float *>(room + r.dw), p.splits, 1, p.rows, p.cols, p.ldo, out, out_type, lddw, 0, st);
             } else {
-                err = pick_tile(1, p.rows, p.cols, p.k, size, false) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
+                err = pick_tile(1, p.rows, p.cols, (int64_t)p.k * p.numbers, size, false) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
                                                                           : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
             }
             if (err) return err;
@@ -547,6 +564,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
             p.B = g.W + v0 * g.ldw * size; p.ldb = g.ldw; p.b_cols = (int)r.ldd;
             p.out = reinterpret_cast<char *>(planes); p.ldo = r.ldd; p.plane = (int64_t)g.T * r.ldd;
             p.rows = g.T; p.cols = g.D; p.k = g.vp;
+            p.numbers = g.numbers; p.next = g.T * g.ldg * (int64_t)size;
             p.splits = r.splits; p.add = v0 > 0;
             const int tile = dh_tile(g.T, size);
             err = tile == 256 ? launch_dh<Large<T, KMAJOR, KROWS>>(p, st)
@@ -569,7 +587,7 @@ using namespace t2sp;
 
 extern "C" size_t t2sp_xent_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
     if (!xent_args_ok(type, T, V, D, ldh, ldw)) return 0;
-    return xent_room(false, type, H, W, T, V, D, ldh, ldw).total;
+    return xent_room(false, 1, type, H, W, T, V, D, ldh, ldw).total;
 }
 
 extern "C" int t2sp_xent(int type, const void *H, const void *W, const void *labels, int label_bits, float *loss, float *lse, int T, int V, int D,
@@ -577,7 +595,7 @@ extern "C" int t2sp_xent(int type, const void *H, const void *W, const void *lab
     if (!xent_args_ok(type, T, V, D, ldh, ldw) || (label_bits != 32 && label_bits != 64)) return T2SP_ERR_SHAPE;
     if (T == 0) return T2SP_OK;
     if (!H || !W || !labels || !loss) return T2SP_ERR_SHAPE;
-    const XentRoom r = xent_room(false, type, H, W, T, V, D, ldh, ldw);
+    const XentRoom r = xent_room(false, 1, type, H, W, T, V, D, ldh, ldw);
     if (!workspace || workspace_bytes < r.total || reinterpret_cast<uintptr_t>(workspace) % 16) return T2SP_ERR_SHAPE;
     const hipStream_t st = (hipStream_t)stream;
     char *room = static_cast<char *>(workspace);
@@ -593,18 +611,19 @@ extern "C" int t2sp_xent(int type, const void *H, const void *W, const void *lab
 
 extern "C" size_t t2sp_xent_grad_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
     if (!xent_args_ok(type, T, V, D, ldh, ldw)) return 0;
-    return xent_room(true, type, H, W, T, V, D, ldh, ldw).total;
+    const size_t full = xent_room(true, numbers_of(type, false), type, H, W, T, V, D, ldh, ldw).total;
+    return std::max(full, xent_room(true, numbers_of(type, true), type, H, W, T, V, D, ldh, ldw).total);
 }
 
-extern "C" int t2sp_xent_grad(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits, const float *lse,
-                              const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw,
-                              void *workspace, size_t workspace_bytes, void *stream) {
+static int xent_gradients(bool rounded, int type, int out_type, const void *H, const void *W, const void *labels, int label_bits, const float *lse,
+                          const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw,
+                          void *workspace, size_t workspace_bytes, void *stream) {
     if (!xent_args_ok(type, T, V, D, ldh, ldw) || !out_type_ok(type, out_type) || (label_bits != 32 && label_bits != 64) || !stride_ok(lddh) ||
         !stride_ok(lddw) || (dH && lddh < D) || (dW && lddw < D))
         return T2SP_ERR_SHAPE;
     if ((!dH && !dW) || (T == 0 && !dW)) return T2SP_OK;
     if (T && (!H || !W || !labels || !lse || !dloss)) return T2SP_ERR_SHAPE;
-    const XentRoom r = xent_room(true, type, H, W, T, V, D, ldh, ldw);
+    const XentRoom r = xent_room(true, numbers_of(type, rounded), type, H, W, T, V, D, ldh, ldw);
     if (!workspace || workspace_bytes < r.total || reinterpret_cast<uintptr_t>(workspace) % 16) return T2SP_ERR_SHAPE;
     const hipStream_t st = (hipStream_t)stream;
     char *room = static_cast<char *>(workspace);
@@ -613,9 +632,23 @@ extern "C" int t2sp_xent_grad(int type, int out_type, const void *H, const void 
     g.T = T; g.V = V; g.D = D;
     g.xcds = machine().xcds;
     g.lse = lse; g.dloss = dloss;
+    g.numbers = numbers_of(type, rounded);
     if (T)
         if (int err = xent_operands(g, r, type_bytes(type), room, H, W, ldh, ldw, st)) return err;
     return with_types(type, out_type, [&](auto *t, auto *o) {
         return xent_backward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, r, room, H, ldh, dH, dW, out_type, lddh, lddw, st);
     });
+}
+
+extern "C" int t2sp_xent_grad(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits, const float *lse,
+                              const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh, int64_t ldw, int64_t lddh, int64_t lddw,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    return xent_gradients(false, type, out_type, H, W, labels, label_bits, lse, dloss, dH, dW, T, V, D, ldh, ldw, lddh, lddw, workspace,
+                          workspace_bytes, stream);
+}
+extern "C" int t2sp_xent_grad_rounded(int type, int out_type, const void *H, const void *W, const void *labels, int label_bits, const float *lse,
+                                      const float *dloss, void *dH, void *dW, int T, int V, int D, int64_t ldh, int64_t ldw, int64_t lddh,
+                                      int64_t lddw, void *workspace, size_t workspace_bytes, void *stream) {
+    return xent_gradients(true, type, out_type, H, W, labels, label_bits, lse, dloss, dH, dW, T, V, D, ldh, ldw, lddh, lddw, workspace,
+                          workspace_bytes, stream);
 }

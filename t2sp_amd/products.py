@@ -266,12 +266,15 @@ def xent(H, W, labels, loss=None, lse=None):
     return loss, lse
 
 
-def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted=(True, True)):
+def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted=(True, True), rounded=False):
     """Gradients (dH, dW) of sum_t dloss[t] * loss[t] (see xent): dH = g @ W, dW = g.T @ H with
     g[t, v] = (exp(z[t, v] - lse[t]) - [v == labels[t]]) * dloss[t]; tokens without a label take no part.
 
     lse: what xent returned; dloss: T float32.  The results have H's type, or float32 (out_dtype, or the type of dH / dW).
-    `wanted` leaves one out (its place in the result is None; numpy arrays: both are computed)."""
+    `wanted` leaves one out (its place in the result is None; numpy arrays: both are computed).
+    16-bit types: g enters the products with 16 (bfloat16) or 22 (half) of a float's 24 bits, as the sum of two numbers of
+    the type.  rounded=True takes it rounded to one, for a third less time and an error of half a step of the type in every g
+    (tensors only)."""
     op = "xent_grad"
     if not _is_torch(H):
         return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW)
@@ -291,15 +294,16 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
     back = _current_device()
     if back != index:
         with _On(index, back):
-            return xent_grad(H, W, labels, lse, dloss, dH, dW, wanted=(False, False))      # (what is wanted is allocated by now)
+            return xent_grad(H, W, labels, lse, dloss, dH, dW, wanted=(False, False), rounded=rounded)      # (what is wanted is allocated by now)
     L = lib()
     h, w, ldh, ldw = H.data_ptr(), W.data_ptr(), _row(H), _row(W)
     nbytes = L.t2sp_xent_grad_workspace_bytes(code, h, w, T, V, D, ldh, ldw)
     room = _room(H, nbytes)
-    _check(op, L.t2sp_xent_grad(code, out_code, h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
-                                dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None, T, V, D, ldh, ldw,
-                                _row(dH) if dH is not None else D, _row(dW) if dW is not None else D,
-                                room.data_ptr() if nbytes else None, nbytes, _raw_stream(index)))
+    grad = L.t2sp_xent_grad_rounded if rounded else L.t2sp_xent_grad
+    _check(op, grad(code, out_code, h, w, labels.data_ptr(), bits, lse.data_ptr(), dloss.data_ptr(),
+                    dH.data_ptr() if dH is not None else None, dW.data_ptr() if dW is not None else None, T, V, D, ldh, ldw,
+                    _row(dH) if dH is not None else D, _row(dW) if dW is not None else D,
+                    room.data_ptr() if nbytes else None, nbytes, _raw_stream(index)))
     return dH, dW
 
 
