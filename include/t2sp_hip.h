@@ -338,7 +338,9 @@ int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, const void *d
  *                   dH = g W (T x D),  dW = g^T H (V x D); either may be NULL
  * `labels` are integers of `label_bits` = 32 or 64.  A token whose label is outside 0 .. V - 1 (padding, a
  * prompt) has loss 0, a row of zeros in dH and no part in dW, whatever its rows of H and dloss hold.
- * loss, lse and dloss are float, one per token; a mean's gradient is dloss = 1 / number of tokens.
+ * loss, lse and dloss are float, one per token; a mean's gradient is dloss = 1 / number of tokens.  Tokens' weights may
+ * differ by any factor; half: in dW, tokens lighter than 2^-30 of the heaviest (dloss times the largest element of the
+ * row of H) lose bits, as half has no smaller numbers.
  * The gradient works through the vocabulary in pieces: p - [label] of one piece passes through the workspace
  * (16-byte aligned, t2sp_xent*_workspace_bytes, required), as do padded copies of operands whose rows are not
  * whole 16-byte chunks.  16-bit types: p - [label] enters the products as the sum of two numbers of `type`, 16

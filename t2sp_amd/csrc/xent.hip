@@ -18,10 +18,15 @@
 // gradients are off by 8e-7 and 5e-7 in norm, by 2e-7 for the two numbers alone, by 1.1e-4 with one; a third number changes
 // nothing).  Callers who accept half a step of the type in p - [label] (t2sp_xent_grad_rounded) have one: 8 T D V.
 //
-// Scales.  dloss is kept out of the rounded matrix: dH's rows are multiplied by it at the end, and for dW it goes into
-// the rows of H, as dloss[t] / max |dloss| (exactly 1 in the usual case of equal weights: then the copy of H is exact).
-// half has no room below 2^-24 for the probabilities of a large vocabulary: p - [label] is stored times 2^15 there
-// (at most 32768 in magnitude) and the products are scaled back in float.
+// Weights of the tokens.  dloss[t] = m 2^x with 1/2 <= |m| < 1 is a factor of both products' reductions or rows.  p - [label]
+// is stored times m 2^b, the rows of H for dW are copied times 2^a, exactly, with a + b = x + C for one C of all tokens; dH's rows
+// are multiplied by 2^(x - b) at the end, dW by 2^-C.  bfloat16 and float: b = 0, and C makes the largest a zero.  half has
+// room between 2^-24 and 2^16 only, so its b is 15 (the probabilities of a large vocabulary reach far below 1, and together
+// the two numbers go down to 2^-40 of that) and C is the largest for which no copied element exceeds 2^15.  A lighter token's
+// a is smaller by d = its distance, as a power of two, from the token that decides C.  Up to d = 20 that costs no bits of
+// elements down to 2^-8 of the row's largest; the next 10 are taken from b; then a falls further.  So weights (times the size of
+// the row) down to 2^-30 of the heaviest keep their bits, below that elements underflow.  (With dloss / max |dloss| rounded into
+// the copy, weights of 1e-6 of the heaviest put dW off by 2 %.)
 // The copy of H also holds zeros for tokens without a label: what their rows hold (padding may be anything) reaches
 // no sum.
 #include "product_core.hpp"
@@ -40,7 +45,8 @@ struct XentArgs {
     float *hit;                          // [T]: z at the label
     // backward
     const float *lse, *dloss;
-    char *G;                             // [numbers][T][ldg] p - [label] of the piece, zeros from vp to ldg
+    const int *common, *row_exp;         // see the weights of the tokens above; row_exp: half only
+    char *G;                             // [numbers][T][ldg] p - [label] times m 2^b of the piece, zeros from vp to ldg
     int64_t ldg;
     int numbers;                         // of the type that p - [label] is the sum of
     int v0, vp;                          // the piece: words v0 .. v0 + vp - 1
@@ -152,54 +158,98 @@ __global__ void __launch_bounds__(64 * JOIN_WAVES) xent_join_kernel(const float2
     }
 }
 
-// max |dloss| over the tokens with a label, NaN if one of them is not finite; in every thread of a workgroup.
-template <int THREADS>
-__device__ __forceinline__ float largest_weight(const float *dloss, const void *labels, int lab64, int T, int V) {
-    constexpr int WAVES = THREADS / 64;
-    __shared__ float joint[WAVES];
-    float top = 0.f;
-    bool bad = false;
-    for (int t = threadIdx.x; t < T; t += THREADS) {
-        const int64_t label = label_of(labels, lab64, t);
-        if (label >= 0 && label < V) {
-            const float v = fabsf(dloss[t]);
-            bad |= !(v < __builtin_inff());
-            top = fmaxf(top, v);
-        }
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-    if (__ballot(bad)) top = __builtin_nanf("");
-    if ((threadIdx.x & 63) == 0) joint[threadIdx.x >> 6] = top;
-    __syncthreads();
-    float all = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) all = joint[w] != joint[w] || all != all ? __builtin_nanf("") : fmaxf(all, joint[w]);
-    return all;
-}
-__global__ void __launch_bounds__(1024) xent_scale_kernel(const float *dloss, const void *labels, int lab64, int T, int V, float *scale) {
-    const float all = largest_weight<1024>(dloss, labels, lab64, T, V);
-    if (threadIdx.x == 0) *scale = all;
+// The weights of the tokens (see above).
+constexpr int NO_EXPONENT = -0x7fffffff - 1;         // of a row without a finite element but zeros
+struct TokenWeight {
+    float g;                                         // m 2^b (dloss itself where it is 0 or not finite)
+    int a, u;                                        // u = x - b
+};
+template <class T>
+__device__ __forceinline__ TokenWeight token_weight(float dloss, const int *row_exp, int t, int common) {
+    if (dloss == 0.f || !(fabsf(dloss) < __builtin_inff())) return {dloss, 0, 0};
+    int x;
+    const float m = frexpf(dloss, &x);
+    if constexpr (!std::is_same_v<T, _Float16>) return {m, x + common, x};
+    const int e = row_exp[t];
+    if (e == NO_EXPONENT) return {ldexpf(m, 15), 0, x - 15};
+    const int lighter = 30 - e - x - common, b = 15 - (lighter <= 20 ? 0 : lighter <= 30 ? lighter - 20 : 10);
+    return {ldexpf(m, b), x + common - b, x - b};
 }
 
-// Hz[t, :] = H[t, :] * (dloss[t] / max |dloss|) rounded to the type, zeros for tokens without a label and from D to ld.
-// FIND: the workgroups look for the maximum themselves, for the kernels behind too (up to FIND_ROWS tokens; a launch less, about 3 us
+// row_exp[t] = e: the largest finite |H[t, :]| is in 2^(e - 1) .. 2^e.  One wave per token.
+__global__ void __launch_bounds__(256) xent_row_exponents_kernel(const _Float16 *H, int64_t ldh, int rows, int D, int *row_exp) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < rows; t += (int64_t)gridDim.x * 4) {
+        const _Float16 *h = H + t * ldh;
+        float top = 0.f;
+        auto take = [&](_Float16 v) {
+            const float f = fabsf((float)v);
+            top = f < __builtin_inff() ? fmaxf(top, f) : top;
+        };
+        const int whole = D / 8 * 8;
+        for (int c = lane * 8; c < whole; c += 512) {
+            const Chunk<_Float16>::type v = *reinterpret_cast<const Chunk<_Float16>::anywhere *>(h + c);
+#pragma unroll
+            for (int j = 0; j < 8; j++) take(v[j]);
+        }
+        if (whole + lane < D) take(h[whole + lane]);
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+        int e = NO_EXPONENT;
+        if (top > 0.f) frexpf(top, &e);
+        if (lane == 0) row_exp[t] = e;
+    }
+}
+
+// C, from the tokens with a label and a finite weight other than 0; in every thread of a workgroup.
+template <class T, int THREADS>
+__device__ __forceinline__ int common_exponent(const float *dloss, const void *labels, int lab64, const int *row_exp, int rows, int V) {
+    constexpr int WAVES = THREADS / 64, NONE = 0x7fffffff;
+    __shared__ int joint[WAVES];
+    int least = NONE;
+    for (int t = threadIdx.x; t < rows; t += THREADS) {
+        const int64_t label = label_of(labels, lab64, t);
+        const float v = fabsf(dloss[t]);
+        if (label < 0 || label >= V || !(v > 0.f && v < __builtin_inff())) continue;
+        int x, e = 30;
+        frexpf(v, &x);
+        if constexpr (std::is_same_v<T, _Float16>) e = row_exp[t];
+        if (e != NO_EXPONENT) least = min(least, 30 - e - x);
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) least = min(least, __shfl_xor(least, m, 64));
+    if ((threadIdx.x & 63) == 0) joint[threadIdx.x >> 6] = least;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) least = min(least, joint[w]);
+    return least == NONE ? 0 : least;
+}
+template <class T>
+__global__ void __launch_bounds__(1024) xent_common_kernel(const float *dloss, const void *labels, int lab64, const int *row_exp, int rows, int V,
+                                                           int *common) {
+    const int c = common_exponent<T, 1024>(dloss, labels, lab64, row_exp, rows, V);
+    if (threadIdx.x == 0) *common = c;
+}
+
+// Hz[t, :] = 2^a H[t, :], zeros for tokens without a label and from D to ld.
+// FIND: the workgroups look for C themselves, for the kernels behind too (up to FIND_ROWS tokens; a launch less, about 3 us
 // of the host's time).
 constexpr int FIND_ROWS = 2048;
 template <class T, bool FIND>
 __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int64_t ldh, const void *labels, int lab64, const float *dloss,
-                                                                 float *scale, int rows, int V, int D, T *Hz, int64_t ld, int64_t chunks) {
+                                                                 const int *row_exp, int *common, int rows, int V, int D, T *Hz, int64_t ld,
+                                                                 int64_t chunks) {
     constexpr int CE = 16 / sizeof(T);
     typedef T chunk __attribute__((ext_vector_type(CE)));
     const int64_t per = ld / CE;
-    const float top = FIND ? largest_weight<256>(dloss, labels, lab64, rows, V) : *scale;
-    if (FIND && blockIdx.x == 0 && threadIdx.x == 0) *scale = top;
+    const int c0 = FIND ? common_exponent<T, 256>(dloss, labels, lab64, row_exp, rows, V) : *common;
+    if (FIND && blockIdx.x == 0 && threadIdx.x == 0) *common = c0;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int t = (int)(i / per), c = (int)(i % per) * CE;
         const int64_t label = label_of(labels, lab64, t);
         chunk v;
         if (label >= 0 && label < V) {
-            const float by = top == 0.f ? 0.f : dloss[t] / top;
+            const int a = token_weight<T>(dloss[t], row_exp, t, c0).a;
             const T *s = H + t * ldh + c;
             if (c + CE <= D) {
                 v = *reinterpret_cast<const typename Chunk<T>::anywhere *>(s);
@@ -208,7 +258,7 @@ __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int
                 for (int j = 0; j < CE; j++) v[j] = c + j < D ? s[j] : (T)0.f;
             }
 #pragma unroll
-            for (int j = 0; j < CE; j++) v[j] = (T)((float)v[j] * by);
+            for (int j = 0; j < CE; j++) v[j] = (T)ldexpf((float)v[j], a);
         } else {
 #pragma unroll
             for (int j = 0; j < CE; j++) v[j] = (T)0.f;
@@ -216,9 +266,6 @@ __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int
         *reinterpret_cast<chunk *>(Hz + i * CE) = v;
     }
 }
-
-template <class T> struct GradientScale { static constexpr float value = 1.f; };
-template <> struct GradientScale<_Float16> { static constexpr float value = 32768.f; };
 
 template <class P>
 __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const XentArgs g) {
@@ -230,7 +277,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
     n0 *= P::BN;
     pv4f acc[P::MT][P::NT];
     logits_tile<P>(g, m0, n0, smem, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, common = *g.common;
     const int n = n0 + (wave % P::WN) * P::TN + P::lane_column(lane);
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
@@ -238,13 +285,13 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
         if (t >= g.T) continue;
         const int64_t label = label_of(g.labels, g.lab64, t);
         const bool valid = label >= 0 && label < g.V;
-        const float lse = g.lse[t];
+        const float lse = g.lse[t], weight = valid ? token_weight<T>(g.dloss[t], g.row_exp, t, common).g : 0.f;
         const int64_t hot = label - g.v0;
 #pragma unroll
         for (int c = 0; c < P::LANE_N; c++) {
             const int v = n + 8 * (c / 4) + c % 4;
             const float p = exp_of(acc[i][c / 4][c % 4] - lse) - (v == hot ? 1.f : 0.f);
-            acc[i][c / 4][c % 4] = valid && v < g.vp ? p * GradientScale<T>::value : 0.f;
+            acc[i][c / 4][c % 4] = valid && v < g.vp ? p * weight : 0.f;
         }
         char *row = g.G + t * g.ldg * (int64_t)sizeof(T);
         for (int j = 0; j < g.numbers; j++, row += g.T * g.ldg * (int64_t)sizeof(T)) {
@@ -264,14 +311,13 @@ struct XentProductArgs {
     int64_t next;
     int a_cols, b_cols;                  // elements in a row of A (dW) and B, whole 16-byte chunks
     int row_tiles, col_tiles, xcds;
-    const float *scale;                  // dW: max |dloss|
-    float by;
+    const int *common;                   // dW: C
     int splits;                          // the reduction in this many parts, each (dW: if more than one) with a plane of floats
     int64_t plane;
     int add;                             // dH: add to the planes (a later piece of the vocabulary)
 };
 
-// dW[v0 + m, n] = scale * sum_t G[t, m] Hz[t, n], or one of several planes with the sums over part of the tokens
+// dW[v0 + m, n] = 2^-C sum_t G[t, m] Hz[t, n], or one of several planes with the sums over part of the tokens
 template <class P, class O>
 __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -290,13 +336,15 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
         for (int i = 0; i < g.numbers; i++, a.p += g.next) product_run<P>(a, b, k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = n0 + (wave % P::WN) * P::TN;
-    const float by = *g.scale * g.by;
+    const int by = -*g.common;
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int m = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
         if (m >= g.rows) continue;
 #pragma unroll
-        for (int j = 0; j < P::NT; j++) acc[i][j] *= by;
+        for (int j = 0; j < P::NT; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[i][j][c] = ldexpf(acc[i][j][c], by);
         store_row<P, O>(g.out + (s * g.plane + m * g.ldo) * (int64_t)sizeof(O), n, g.cols, acc[i]);
     }
 }
@@ -333,10 +381,10 @@ __global__ void __launch_bounds__(P::THREADS) xent_dh_kernel(const XentProductAr
     }
 }
 
-// dH[t, n] = dloss[t] * by * sum_s plane[s][t, n], zeros for tokens without a label.
-template <class O>
+// dH[t, n] = 2^(x - b) sum_s plane[s][t, n], zeros for tokens without a label.
+template <class T, class O>
 __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, int splits, int64_t plane, int64_t ld, const void *labels, int lab64,
-                                                           const float *dloss, float by, int V, int D, O *dH, int64_t ldo, int64_t chunks) {
+                                                           const float *dloss, const int *row_exp, const int *common, int V, int D, O *dH, int64_t ldo, int64_t chunks) {
     const int64_t per = ld / 4;
     typedef O quad __attribute__((ext_vector_type(4)));
     typedef O quad_anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
@@ -347,7 +395,9 @@ __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, 
         if (label >= 0 && label < V) {
 #pragma unroll 4
             for (int s = 0; s < splits; s++) sum += *reinterpret_cast<const pv4f *>(planes + s * plane + t * ld + n);
-            sum *= dloss[t] * by;
+            const int u = token_weight<T>(dloss[t], row_exp, t, *common).u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum[j] = ldexpf(sum[j], u);
         }
         O *o = dH + t * ldo + n;
         if (n + 4 <= D) {
@@ -365,7 +415,7 @@ __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, 
 struct XentRoom {
     size_t h, w;                         // padded copies of H and W (0: read where they lie)
     size_t part, hit;                    // forward
-    size_t scale, hz, g, planes, dw;     // backward
+    size_t common, row_exp, hz, g, planes, dw;     // backward
     size_t total;
     int64_t ldd;                         // elements per row of hz and of the planes
     int piece, splits, dw_parts;
@@ -425,7 +475,8 @@ static XentRoom xent_room(bool backward, int numbers, int type, const void *H, c
         else piece = round_up((V + (V + piece - 1) / piece - 1) / ((V + piece - 1) / piece), 256);     // equal pieces
         r.piece = (int)piece;
         r.splits = dh_splits(T, D, r.piece, size, numbers);
-        r.scale = take(sizeof(float));
+        r.common = take(sizeof(int));
+        r.row_exp = take(type == T2SP_TYPE_F16 ? (size_t)T * sizeof(int) : 0);
         r.hz = take((size_t)T * r.ldd * size);
         r.g = take((size_t)T * padded_cols(piece, size) * size * numbers);
         r.planes = take((size_t)r.splits * T * r.ldd * sizeof(float));
@@ -509,23 +560,28 @@ template <class T, class O>
 static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *H, int64_t ldh, void *dH, void *dW, int out_type, int64_t lddh,
                          int64_t lddw, hipStream_t st) {
     constexpr int size = sizeof(T);
-    const float by = 1.f / GradientScale<T>::value;
-    float *scale = reinterpret_cast<float *>(room + r.scale), *planes = reinterpret_cast<float *>(room + r.planes);
+    float *planes = reinterpret_cast<float *>(room + r.planes);
+    int *common = reinterpret_cast<int *>(room + r.common), *row_exp = reinterpret_cast<int *>(room + r.row_exp);
     int err;
-    if (dW) {
-        const int64_t chunks = (int64_t)g.T * r.ldd * size / 16;
-        const bool find = chunks && g.T <= FIND_ROWS;
-        if (!find) {
-            hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, g.dloss, g.labels, g.lab64, g.T, g.V, scale);
+    g.common = common; g.row_exp = row_exp;
+    if constexpr (std::is_same_v<T, _Float16>)
+        if (g.T) {
+            hipLaunchKernelGGL(xent_row_exponents_kernel, dim3((unsigned)std::min((g.T + 3) / 4, 16384)), dim3(256), 0, st, static_cast<const T *>(H), ldh,
+                               g.T, g.D, row_exp);
             if ((err = launched())) return err;
         }
-        if (chunks) {
-            auto kern = find ? xent_weighted_rows_kernel<T, true> : xent_weighted_rows_kernel<T, false>;
-            hipLaunchKernelGGL(kern, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
-                               static_cast<const T *>(H), ldh, g.labels, g.lab64, g.dloss, scale, g.T, g.V, g.D,
-                               reinterpret_cast<T *>(room + r.hz), r.ldd, chunks);
-            if ((err = launched())) return err;
-        }
+    const int64_t chunks = dW ? (int64_t)g.T * r.ldd * size / 16 : 0;
+    const bool find = chunks && g.T <= FIND_ROWS;
+    if (!find) {
+        hipLaunchKernelGGL(xent_common_kernel<T>, dim3(1), dim3(1024), 0, st, g.dloss, g.labels, g.lab64, row_exp, g.T, g.V, common);
+        if ((err = launched())) return err;
+    }
+    if (chunks) {
+        auto kern = find ? xent_weighted_rows_kernel<T, true> : xent_weighted_rows_kernel<T, false>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
+                           static_cast<const T *>(H), ldh, g.labels, g.lab64, g.dloss, row_exp, common, g.T, g.V, g.D,
+                           reinterpret_cast<T *>(room + r.hz), r.ldd, chunks);
+        if ((err = launched())) return err;
     }
     for (int v0 = 0; v0 < g.V; v0 += r.piece) {
         g.v0 = v0;
@@ -546,7 +602,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
             p.out = static_cast<char *>(dW) + v0 * lddw * (int64_t)sizeof(O); p.ldo = lddw;
             p.rows = g.vp; p.cols = g.D; p.k = g.T;
             p.numbers = g.numbers; p.next = g.T * g.ldg * (int64_t)size;
-            p.scale = scale; p.by = by;
+            p.common = common;
             p.splits = r.dw_parts;
             if (r.dw_parts > 1) {
                 char *const out = p.out;
@@ -573,9 +629,9 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
         }
     }
     if (dH && g.T) {
-        const int64_t chunks = (int64_t)g.T * r.ldd / 4;
-        hipLaunchKernelGGL(xent_dh_join_kernel<O>, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st, planes,
-                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, by, g.V, g.D, static_cast<O *>(dH), lddh, chunks);
+        const int64_t quads = (int64_t)g.T * r.ldd / 4;
+        hipLaunchKernelGGL((xent_dh_join_kernel<T, O>), dim3((unsigned)(quads < 256 * 16384 ? (quads + 255) / 256 : 16384)), dim3(256), 0, st, planes,
+                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, row_exp, common, g.V, g.D, static_cast<O *>(dH), lddh, quads);
         return launched();
     }
     return T2SP_OK;

@@ -6,7 +6,7 @@ ee = (3 |z - lse| + 2) u the relative error of an exponential, el = 3 max ee + V
 in test_xent_gpu.py):
   g     p (el + ee) and two roundings in float (the difference, the token's weight): 2u |g|; then as the sum of n = 2
         numbers of the type, each of which rounds what those before it leave: u_T^n |g| (half: not below half
-        of its smallest step 2^-24, on a scale of 2^15: 2^-40 of the largest weight's); one number alone: u_T |g|
+        of its smallest step, 2^-25, on a scale of m 2^15 with |dloss| = m 2^x, m >= 1/2: 2^-39 |dloss|); one number alone: u_T |g|
   dH    sum |dg w| + (n V + 8) u sum |g w| (1 + u_T),   dW  sum |dg h| + (n T + 8) u sum |g h| (1 + u_T)   (n numbers: n times
         the terms)"""
 import numpy as np
@@ -44,7 +44,7 @@ def bounds(H, W, labels, dloss, rounded=False):
     numbers = 1 if rounded or H.dtype == torch.float32 else 2
     dg = p * l.abs()[:, None] * (el[:, None] + ee) * 1.01 + (2 * U + ut ** numbers) * 1.01 * g.abs()
     if H.dtype == torch.float16:
-        dg = dg + 2.0 ** -40 * l.abs()[:, None]
+        dg = dg + 2.0 ** -39 * l.abs()[:, None]
     dH, dW = g @ w, g.t() @ h
     bH = dg @ w.abs() + (numbers * V + 8) * U * (1 + ut) * (g.abs() @ w.abs()) + 2 * U * dH.abs()
     bW = dg.t() @ h.abs() + (numbers * T + 8) * U * (1 + ut) * (g.abs().t() @ h.abs()) + 2 * U * dW.abs()
@@ -89,3 +89,63 @@ def test_rounded_on_request(dtype, T, V, D):
     assert (torch.equal(dH, full[0]) and torch.equal(dW, full[1])) == (dtype == "float32")
     alone, none = t2sp_amd.xent_grad(H, W, lab, lse, d, out_dtype=torch.float32, wanted=(True, False), rounded=True)
     assert none is None and torch.equal(alone, dH)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("ratio", [1e-3, 1e-5, 1e-6, 1e-7, 5e-9])
+@pytest.mark.parametrize("T", [40, 2100])
+def test_a_heavy_token_that_contributes_nothing(dtype, ratio, T):
+    """One well-predicted token of weight 1, the others lighter: all of dW is theirs.  Rows of H differ in size too (by powers of
+    two, so that logits stay exact).  half: p - [label] of light tokens is stored times m 2^b with b down to 5 and |dloss| =
+    m 2^x, 1/2 <= m < 1: half of the smallest step, 2^-25, is 2^-25 / (m 2^5) <= 2^-29 of the weight."""
+    import torch
+    V, D = 60, 64
+    H, W, lab = quarters((T, D), dtype, 1, 4), quarters((V, D), dtype, 2, 1), labels_for(T, V, 3)
+    H[1::3] *= 0.25
+    lab[0] = 7
+    W[:, 0] = 0.0
+    W[7, 0] = 8.0
+    H[0] = 0.0
+    H[0, 0] = 4.0                                            # its label's logit is 32, the others' 0
+    d = ratio * (0.5 + torch.rand(T, generator=torch.Generator().manual_seed(4))).cuda()
+    d[0] = 1.0
+    d[5] = 0.0
+    _, lse = t2sp_amd.xent(H, W, lab)
+    dH, dW = t2sp_amd.xent_grad(H, W, lab, lse, d, out_dtype=torch.float32)
+    wH, wW, bH, bW = bounds(H, W, lab, d)
+    valid = (lab >= 0) & (lab < V)
+    l = torch.where(valid, d.double().abs(), torch.zeros_like(d.double()))[:, None]
+    step = 2.0 ** -29 if dtype == "float16" else 0.0
+    within(dH, wH, bH + step * l * W.double().abs().sum(0))
+    within(dW, wW, bW + step * (l * H.double().abs()).sum(0))
+    assert float((dW.double() - wW).norm() / wW.norm()) < 2e-5
+    only, none = t2sp_amd.xent_grad(H, W, lab, lse, d, out_dtype=torch.float32, wanted=(True, False))
+    assert none is None and torch.equal(only, dH)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -20, 2.0 ** 60])
+def test_weights_of_any_size(dtype, scale):
+    """A power of two in all weights multiplies float gradients by it exactly."""
+    import torch
+    H, W, lab = quarters((70, 64), dtype, 1, 4), quarters((50, 64), dtype, 2, 1), labels_for(70, 50, 3)
+    d = torch.randn(70, generator=torch.Generator().manual_seed(5)).cuda()
+    _, lse = t2sp_amd.xent(H, W, lab)
+    a = t2sp_amd.xent_grad(H, W, lab, lse, d, out_dtype=torch.float32)
+    b = t2sp_amd.xent_grad(H, W, lab, lse, d * scale, out_dtype=torch.float32)
+    assert torch.equal(a[0] * scale, b[0]) and torch.equal(a[1] * scale, b[1])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_a_weight_that_is_not_finite_stays_in_its_token(dtype):
+    import torch
+    H, W, lab = quarters((40, 64), dtype, 1, 4), quarters((50, 64), dtype, 2, 1), labels_for(40, 50, 3, 0.0)
+    d = mean_of(lab, 50)
+    _, lse = t2sp_amd.xent(H, W, lab)
+    want, _ = t2sp_amd.xent_grad(H, W, lab, lse, d, out_dtype=torch.float32)
+    for bad in (float("nan"), float("inf")):
+        d2 = d.clone()
+        d2[9] = bad
+        dH, dW = t2sp_amd.xent_grad(H, W, lab, lse, d2, out_dtype=torch.float32)
+        assert not torch.isfinite(dH[9]).any() and not torch.isfinite(dW).any()
+        assert torch.equal(torch.cat([dH[:9], dH[10:]]), torch.cat([want[:9], want[10:]]))
