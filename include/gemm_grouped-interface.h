@@ -15,7 +15,7 @@ extern "C" {
 #endif
 
 /* Y[r] = X[r] * op(W[e]) for the rows Offsets[e] <= r < Offsets[e+1].  X: (K, T), rows sorted by group; W: (N, K, E),
- * or (K, N, E) when OpB; Offsets: (E + 1), not decreasing (values are clamped to 0 .. T); Y: (N, T).  Rows of Y
+ * or (K, N, E) when OpB; Offsets: (E + 1), not decreasing (values are clamped to 0 .. T and taken as their running maximum); Y: (N, T).  Rows of Y
  * outside every group keep what they held. */
 int gemm_grouped(int32_t OpB, struct halide_buffer_t *X, struct halide_buffer_t *W, struct halide_buffer_t *Offsets,
                  struct halide_buffer_t *Y);

@@ -313,8 +313,9 @@ int t2sp_capsule_packed_f32(const float *P2, int64_t ldp, const float *W2, int64
  *   t2sp_gemm_grouped        Y[r,:] = X[r,:] * op(W[e]);  W[e] is K x N, or N x K with `opb`
  *   t2sp_gemm_grouped_wgrad  dW[e]  = X_e^T * dY_e, K x N; zeros for an empty group
  * The gradient of X is t2sp_gemm_grouped of dY with the other `opb`.  Rows of Y outside every group keep
- * what they held, and rows of X and dY outside every group are never used.  Offsets must not decrease; they
- * are clamped to 0 .. T, so that no value leads outside the buffers.  sw: elements between the matrices.
+ * what they held, and rows of X and dY outside every group are never used.  Offsets are meant not
+ * to decrease; they are clamped to 0 .. T and taken as their running maximum, so that no value leads outside the
+ * buffers or gives a row to two groups.  sw: elements between the matrices.
  * Every result element is one sum in a fixed order, whatever the group sizes.
  * Operands whose rows are not whole 16-byte chunks (pointer, leading dimension, extent) are first copied
  * to padded rows in `workspace`, and t2sp_gemm_grouped_wgrad sums few small matrices in parts, as planes of floats

@@ -10,7 +10,8 @@
 // (a scan over the lanes); workgroups beyond the actual number end at once.  The tiles are then dealt to the dies in
 // contiguous runs, since each die has an L2 of its own: neighbouring tiles read the same columns of one matrix.
 //
-// Offsets are clamped to 0 .. T and to be non-decreasing before use, so no value of theirs leads outside X or Y.
+// Offsets are clamped to 0 .. T and replaced by their running maximum before use: no value of theirs leads outside X or Y,
+// no row belongs to two groups, and the tiles are never more than the launch covers.
 #include "product_core.hpp"
 #include "product_host.hpp"
 
@@ -48,12 +49,25 @@ struct GroupTile {
 template <int BM, bool HALVES = false>
 __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, GroupTile *out) {
     const int lane = threadIdx.x & 63;
-    auto tiles_of = [&](int e, int *start, int *rows) {
-        int a = 0, b = 0;
-        if (e < g.E) { a = group_edge(g, e); b = group_edge(g, e + 1); }
+    // The rows and tiles of group e0 + lane; `high` is the largest offset of the groups in front of e0, then of those behind.
+    auto tiles_of = [&](int e0, int *high, int *start, int *rows) {
+        int a = *high, b = a;
+        if (e0 + lane < g.E) { a = group_edge(g, e0 + lane); b = group_edge(g, e0 + lane + 1); }
+        if (__ballot(b < a || a < *high)) {              // (offsets that decrease, which a caller does not mean to pass)
+            const int front = max(*high, __builtin_amdgcn_readlane(a, 0));
+            b = max(b, front);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(b, d, 64);
+                if (lane >= d) b = max(b, o);
+            }
+            a = __shfl_up(b, 1, 64);
+            if (lane == 0) a = front;
+        }
+        *high = __builtin_amdgcn_readlane(b, 63);        // (used if there are groups behind these 64)
         *start = a;
-        *rows = b > a ? b - a : 0;
-        return (*rows + BM - 1) / BM;
+        *rows = b - a;
+        return (b - a + BM - 1) / BM;
     };
     auto scan = [&](int v) {                         // inclusive prefix sum over the wave
 #pragma unroll
@@ -63,11 +77,11 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
         }
         return v;
     };
-    int start, rows, n = tiles_of(lane, &start, &rows), sum = scan(n);
+    int high = 0, start, rows, n = tiles_of(0, &high, &start, &rows), sum = scan(n), high0 = high;
     int64_t total = __builtin_amdgcn_readlane(sum, 63);
     for (int e0 = 64; e0 < g.E; e0 += 64) {
         int s, r;
-        total += __builtin_amdgcn_readlane(scan(tiles_of(e0 + lane, &s, &r)), 63);
+        total += __builtin_amdgcn_readlane(scan(tiles_of(e0, &high, &s, &r)), 63);
     }
     total *= g.col_tiles;
     const int64_t run = (total + g.xcds - 1) / g.xcds;
@@ -105,7 +119,7 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs &g, unsigned block, 
         }
         before += __builtin_amdgcn_readlane(sum, 63);
         e0 += 64;
-        n = tiles_of(e0 + lane, &start, &rows);
+        n = tiles_of(e0, &high0, &start, &rows);
         sum = scan(n);
     }
     return false;
@@ -289,19 +303,33 @@ __global__ void __launch_bounds__(512) grouped_few_rows_kernel(const GroupedArgs
     }
 }
 
-// The group that is `rank`-th in size (ties: the lower index first); the first 64 groups among themselves, as the
-// groups behind them, which keep their places.
-__device__ __forceinline__ int group_of_rank(const GroupedArgs &g, int rank) {
-    if (rank >= 64) return rank;
+// The group that is `rank`-th in size (ties: the lower index first), its first row and the row behind its last; the first 64
+// groups among themselves, as the groups behind them, which keep their places.  The results are uniform over the wave.
+__device__ __forceinline__ int ranked_group(const GroupedArgs &g, int rank, int *first, int *last) {
     const int lane = threadIdx.x & 63, among = g.E < 64 ? g.E : 64;
-    int size = -1;
-    if (lane < among) size = group_edge(g, lane + 1) - group_edge(g, lane);
-    int place = 0;
-    for (int j = 0; j < among; j++) {
-        const int other = __builtin_amdgcn_readlane(size, j);
-        place += other > size || (other == size && j < lane);
+    int a = 0, b = -1, e = rank;
+    if (lane < among) { a = group_edge(g, lane); b = group_edge(g, lane + 1); }
+    if (rank < 64) {
+        const int size = b - a;
+        int place = 0;
+        for (int j = 0; j < among; j++) {
+            const int other = __builtin_amdgcn_readlane(size, j);
+            place += other > size || (other == size && j < lane);
+        }
+        e = __ffsll((unsigned long long)__ballot(lane < among && place == rank)) - 1;
     }
-    return __ffsll((unsigned long long)__ballot(lane < among && place == rank)) - 1;
+    if (e < 64 && !__ballot(lane < among && b < a)) {
+        *first = __builtin_amdgcn_readlane(a, e);
+        *last = __builtin_amdgcn_readlane(b, e);
+    } else {                                         // the running maximum of the offsets up to e, and with e + 1
+        int high = 0;
+        for (int i = lane; i <= e; i += 64) high = max(high, group_edge(g, i));
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) high = max(high, __shfl_xor(high, m, 64));
+        *first = __builtin_amdgcn_readfirstlane(high);
+        *last = max(*first, group_edge(g, e + 1));
+    }
+    return e;
 }
 
 // dW[e] tile: rows of the tile are K (contiguous in X), columns N (contiguous in dY), the reduction runs over the
@@ -313,13 +341,12 @@ __global__ void __launch_bounds__(P::THREADS) grouped_wgrad_kernel(const Grouped
     // workgroups of a die go through the groups from the largest to the smallest, so that short tiles come last.
     const int row_tiles = (g.K + P::BM - 1) / P::BM;
     const unsigned tiles = (unsigned)row_tiles * g.col_tiles, per_group = tiles * g.parts;
-    int e, k0, n0;
+    int k0, n0, first, last;
     const unsigned rank = blockIdx.x / per_group, at = die_run(blockIdx.x % per_group, per_group, g.xcds), part = at / tiles;
     panel_tile(at % tiles, row_tiles, g.col_tiles, &k0, &n0);
-    e = group_of_rank(g, rank);
+    const int e = ranked_group(g, rank, &first, &last);
     k0 *= P::BM;
     n0 *= P::BN;
-    int first = group_edge(g, e), last = group_edge(g, e + 1);
     if (g.parts > 1) {                               // this part's rows: whole stages
         const int stages = last > first ? (last - first + P::KS - 1) / P::KS : 0, per = (stages + g.parts - 1) / g.parts * P::KS;
         const int64_t from = first + (int64_t)part * per;

@@ -173,7 +173,7 @@ def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
     """Y[r] = X[r] @ op(W[e]) for the rows offsets[e] <= r < offsets[e + 1] of group e.
 
     X: (T, K) rows sorted by group; W: (E, K, N), or (E, N, K) when opb; offsets: E + 1 int32 or int64 on the device,
-    not decreasing (they are clamped to 0 .. T).  Y: (T, N) of X's type, or float32 (out_dtype, or the type of `out`).
+    not decreasing (they are clamped to 0 .. T and taken as their running maximum).  Y: (T, N) of X's type, or float32 (out_dtype, or the type of `out`).
     Rows outside every group are left as they were (in a fresh result: whatever its memory held).  The gradient of X is
     gemm_grouped(dY, W, offsets, opb=1 - opb)."""
     op = "gemm_grouped"
