@@ -11,7 +11,10 @@
 // rows of the matrix, for up to 16 rows of x at once, and a group ends with
 //   y += s * (sum x (16 + q) - (16 + z) * sum x),
 // the last sum from one more MFMA with ones.  Scales and zero points are thus applied in float, once per group.
-// float rows of x go in as three bfloat16 pieces (24 bits together), each with its own MFMAs.
+// float rows of x go in as three bfloat16 pieces (24 bits together), each with its own MFMAs.  Their results are not rounded
+// to 16 bits, so that what the difference above loses would show (rows whose elements have one sign, 4096 inputs: off by
+// 5.6e-7 in norm); the numbers go in as 16 (q - 8) instead, a signed byte made a float, and
+//   y += s * (sum x 16 (q - 8) / 16 - (z - 8) * sum x).
 //
 // Layout (t2sp_w4_pack, made once from plain numbers): blocks of 16 rows x 128 inputs, 1 KB, in which the 16 bytes of
 // lane l are what that lane feeds to four MFMAs: row l % 16, inputs 32 f + 8 (l / 16) + 0..7 for f = 0..3; in a word the
@@ -41,7 +44,7 @@ struct W4Args {
     int vec_x;                           // rows of x are whole 16-byte chunks
 };
 
-// Pieces of x that go through the matrix cores, and 16 + q.
+// Pieces of x that go through the matrix cores, and 16 + q (float: 16 (q - 8)).
 template <class T> struct W4Type;
 template <> struct W4Type<__bf16> {
     using M = __bf16;
@@ -62,7 +65,11 @@ template <> struct W4Type<_Float16> {
 template <> struct W4Type<float> {
     using M = __bf16;
     static constexpr int PIECES = 3;
-    static __device__ __forceinline__ uint32_t pair(uint32_t w, int p) { return W4Type<__bf16>::pair(w, p); }
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, int p) {      // 16 (q - 8): the signed bytes with (q ^ 8) on top
+        const uint32_t bytes = ((w ^ 0x88888888u) << (p & 1 ? 0 : 4)) & 0xf0f0f0f0u;
+        const float lo = (float)(int8_t)(bytes >> (4 * (p & 2))), hi = (float)(int8_t)(bytes >> (4 * (p & 2) + 16));
+        return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+    }
     static constexpr uint32_t ONES = W4Type<__bf16>::ONES;
 };
 
@@ -116,6 +123,7 @@ constexpr int W4_WAVES = 8;
 template <class T, int MT, int NT, int SHIFT, bool VEC>
 __global__ void __launch_bounds__(64 * W4_WAVES) gemv_w4_kernel(const W4Args g) {
     using Op = MatrixOp<typename W4Type<T>::M>;
+    constexpr bool CENTRED = sizeof(T) == 4;
     constexpr int PIECES = W4Type<T>::PIECES, DEEP = MT * NT * sizeof(T) <= 2 ? 4 : MT * sizeof(T) <= 4 ? 2 : 1;
     constexpr int GROUPS = SHIFT == 0 ? 4 : SHIFT == 1 ? 2 : 1;         // of a block
     typedef T quad __attribute__((ext_vector_type(4)));
@@ -211,9 +219,10 @@ __global__ void __launch_bounds__(64 * W4_WAVES) gemv_w4_kernel(const W4Args g) 
                         for (int t = 0; t < NT; t++)
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                const float zz = Z ? 16.f + (float)z[d][t][4 * c + j] : 24.f;
+                                const float less = CENTRED ? 8.f : -16.f, zz = (Z ? (float)z[d][t][4 * c + j] : 8.f) - less;
 #pragma unroll
-                                for (int i = 0; i < MT; i++) y[i * NT + t][j] += (float)s[d][t][4 * c + j] * (acc[i * NT + t][j] - zz * sum[i][j]);
+                                for (int i = 0; i < MT; i++)
+                                    y[i * NT + t][j] += (float)s[d][t][4 * c + j] * ((CENTRED ? 0.0625f : 1.f) * acc[i * NT + t][j] - zz * sum[i][j]);
                             }
                     }
                 }
@@ -348,7 +357,7 @@ static int launch_w4(const W4Args &g, hipStream_t st) {
 // Several tiles of the matrix per workgroup where enough workgroups are left to fill the CUs.  16384 x 4096, bfloat16, groups of
 // 128: 12.6 us with one row and one tile per workgroup, 11.3 with four; 64 rows: 67 us with one tile, 40 with two.  8192 x 4096 is
 // the border: one row 7.4 us with one tile, 10.8 with four, 64 rows 35 and 21 with two.  Floats have no registers left for it but for one
-// row tile and large groups (16384 x 4096: 24 -> 15 us).
+// row tile and large groups (16384 x 4096: 24 us with one tile, 16 with four).
 template <class T>
 static int launch_w4(const W4Args &g, hipStream_t st) {
     const int64_t cus = machine().cus;
