@@ -58,6 +58,13 @@ __device__ __forceinline__ int64_t label_of(const void *labels, int lab64, int t
 
 constexpr float LOG2E = 1.44269504088896340736f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+// What is taken from z before the exponential, for a maximum of `top`: 0 where that is infinite (no word, all words at -inf, or
+// one at inf, whose sum is then inf).
+__device__ __forceinline__ float base_of(float top) { return fabsf(top) < __builtin_inff() ? top : 0.f; }
+// sum (of exponentials above `top`) on the scale of `base`.
+__device__ __forceinline__ float rescaled(float sum, float top, float base) {
+    return sum * exp_of((top == -__builtin_inff() ? base : top) - base);
+}
 
 // The tile of logits of rows m0.., words v0 + n0..
 template <class P>
@@ -101,7 +108,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_stats_kernel(const XentArgs g
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float base = top == -__builtin_inff() ? 0.f : top;         // (no word of the tile, or all at -inf)
+        const float base = base_of(top);
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < P::LANE_N; c++)
@@ -119,9 +126,9 @@ __global__ void __launch_bounds__(P::THREADS) xent_stats_kernel(const XentArgs g
             v[w] = joint[w * P::BM + m];
             top = fmaxf(top, v[w].x);
         }
-        const float base = top == -__builtin_inff() ? 0.f : top;
+        const float base = base_of(top);
 #pragma unroll
-        for (int w = 0; w < P::WN; w++) sum += v[w].y * exp_of((v[w].x == -__builtin_inff() ? base : v[w].x) - base);
+        for (int w = 0; w < P::WN; w++) sum += rescaled(v[w].y, v[w].x, base);
         g.part[(int64_t)tile * g.T + m0 + m] = make_float2(top, sum);
     }
 }
@@ -134,8 +141,8 @@ __global__ void __launch_bounds__(64 * JOIN_WAVES) xent_join_kernel(const float2
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x * 64 + lane;
     float top = -__builtin_inff(), sum = 0.f;
     auto add = [&](float m, float s) {
-        const float to = fmaxf(top, m), base = to == -__builtin_inff() ? 0.f : to;
-        sum = sum * exp_of((top == -__builtin_inff() ? base : top) - base) + s * exp_of((m == -__builtin_inff() ? base : m) - base);
+        const float to = fmaxf(top, m), base = base_of(to);
+        sum = rescaled(sum, top, base) + rescaled(s, m, base);
         top = to;
     };
     if (t < T) {

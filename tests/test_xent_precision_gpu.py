@@ -149,3 +149,36 @@ def test_a_weight_that_is_not_finite_stays_in_its_token(dtype):
         dH, dW = t2sp_amd.xent_grad(H, W, lab, lse, d2, out_dtype=torch.float32)
         assert not torch.isfinite(dH[9]).any() and not torch.isfinite(dW).any()
         assert torch.equal(torch.cat([dH[:9], dH[10:]]), torch.cat([want[:9], want[10:]]))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("V", [5, 300, 5000])
+def test_infinite_logits(dtype, V):
+    """lse of a token with a logit at +inf is +inf (log sum exp), and so is its loss unless that logit is the label's; all logits at
+    -inf give -inf; other tokens are what they were."""
+    import torch
+    T, D = 70, 64
+    inf = float("inf")
+    H, W, lab = quarters((T, D), dtype, 1, 4), quarters((V, D), dtype, 2, 1), labels_for(T, V, 3, 0.0)
+    H[:, 0] = 0.0
+    W[:, 0] = -1.0
+    W[V - 1, 0] = 1.0
+    W[0, 0] = 1.0
+    loss0, lse0 = t2sp_amd.xent(H, W, lab)
+    H[3], H[9] = 0.0, 0.0
+    H[3, 0], H[9, 0] = inf, -inf                             # +inf at the words 0 and V - 1, -inf at the others; the reverse
+    H[11, 5] = float("nan")
+    H[13, 0] = inf                                           # with finite terms beside it
+    lab[3], lab[9] = 1, 0
+    loss, lse = t2sp_amd.xent(H, W, lab)
+    for t in (3, 9, 13):
+        assert lse[t] == inf
+    assert loss[3] == inf and loss[9] == inf and torch.isnan(lse[11]) and torch.isnan(loss[11])
+    loss2, lse2 = t2sp_amd.xent(H, W, torch.full((T,), V - 1, device="cuda"))
+    assert lse2[3] == inf and torch.isnan(loss2[3])
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[[3, 9, 11, 13]] = False
+    assert torch.equal(loss[rest], loss0[rest]) and torch.equal(lse[rest], lse0[rest])
+    W[:, 0] = -1.0
+    lse3 = t2sp_amd.xent(H, W, lab)[1]
+    assert lse3[3] == -inf and lse3[9] == inf and torch.equal(lse3[rest], lse0[rest])
