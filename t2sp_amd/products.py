@@ -75,7 +75,7 @@ def _result(op, out, shape, like, dtype=None):
             return like.new_empty(shape), _codes[like.dtype]
         _need(op, dtype is torch.float32, BAD_TYPE)
         return like.new_empty(shape, dtype=dtype), _F32
-    _need(op, out.dtype is like.dtype or out.dtype is torch.float32, BAD_TYPE)
+    _need(op, (out.dtype is like.dtype or out.dtype is torch.float32) and (dtype is None or dtype is out.dtype), BAD_TYPE)
     _need(op, out.dim() == len(shape), BAD_DIMENSIONS)
     _need(op, tuple(out.shape) == shape and out.get_device() == like.get_device() and (shape[-1] <= 1 or out.stride(-1) == 1))
     return out, _codes[out.dtype]
@@ -115,10 +115,18 @@ def _entry(op, *args):
     _check(op, getattr(lib(), op)(*[a.ref if isinstance(a, HalideBuffer) else a for a in wrapped]))
 
 
-def _host_out(op, out, shape, dtype):
+def _host_out(op, out, shape, like, dtype=None):
+    """`out`, or a fresh array of `dtype` (`like`, the operands' type); that type or float32."""
+    if dtype is not None:
+        try:
+            dtype = np.dtype(dtype)
+        except TypeError:
+            raise T2spError(op, BAD_TYPE)
+        _need(op, dtype == like or dtype == np.float32, BAD_TYPE)
     if out is None:
+        dtype = dtype or like
         return host_empty(shape) if dtype == np.float32 else np.empty(shape, dtype)
-    _need(op, isinstance(out, np.ndarray), BAD_TYPE)
+    _need(op, isinstance(out, np.ndarray) and (dtype is None or dtype == out.dtype), BAD_TYPE)
     return out
 
 
@@ -127,19 +135,19 @@ def _host_arrays(op, *arrays):
         _need(op, isinstance(a, np.ndarray) and a.dtype.name in NUMPY_TYPES, BAD_TYPE)
 
 
-def _host_grouped(op, X, W, offsets, opb, out):
+def _host_grouped(op, X, W, offsets, opb, out, dtype):
     _host_arrays(op, X, W, offsets)
     _need(op, X.ndim == 2 and W.ndim == 3, BAD_DIMENSIONS)
-    Y = _host_out(op, out, (X.shape[0], W.shape[1] if opb else W.shape[2]), X.dtype)
+    Y = _host_out(op, out, (X.shape[0], W.shape[1] if opb else W.shape[2]), X.dtype, dtype)
     _entry(op, int(bool(opb)), X, W, offsets, Y)
     return Y
 
 
-def _host_wgrad(op, X, dY, offsets, out):
+def _host_wgrad(op, X, dY, offsets, out, dtype):
     _host_arrays(op, X, dY, offsets)
     _need(op, X.ndim == 2 and dY.ndim == 2 and offsets.ndim == 1, BAD_DIMENSIONS)
     _need(op, offsets.shape[0] >= 2)
-    dW = _host_out(op, out, (offsets.shape[0] - 1, X.shape[1], dY.shape[1]), X.dtype)
+    dW = _host_out(op, out, (offsets.shape[0] - 1, X.shape[1], dY.shape[1]), X.dtype, dtype)
     _entry(op, X, dY, offsets, dW)
     return dW
 
@@ -152,9 +160,11 @@ def _host_xent(op, H, W, labels, loss, lse):
     return loss, lse
 
 
-def _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW):
+def _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW, dtype):
     _host_arrays(op, H, W, labels, lse, dloss)
-    dH, dW = _host_out(op, dH, H.shape, H.dtype), _host_out(op, dW, W.shape, H.dtype)
+    if dtype is None:
+        dtype = getattr(dH if dH is not None else dW, "dtype", None)
+    dH, dW = _host_out(op, dH, H.shape, H.dtype, dtype), _host_out(op, dW, W.shape, H.dtype, dtype)
     _entry(op, H, W, labels, lse, dloss, dH, dW)
     return dH, dW
 
@@ -178,7 +188,7 @@ def gemm_grouped(X, W, offsets, opb=0, out=None, out_dtype=None):
     gemm_grouped(dY, W, offsets, opb=1 - opb)."""
     op = "gemm_grouped"
     if not _is_torch(X):
-        return _host_grouped(op, X, W, offsets, opb, out)
+        return _host_grouped(op, X, W, offsets, opb, out, out_dtype)
     code, index = _tensors(op, (2, 3), X, W)
     (T, K), (E, N) = X.shape, W.shape[:2]
     opb = 1 if opb else 0
@@ -209,7 +219,7 @@ def gemm_grouped_wgrad(X, dY, offsets, out=None, out_dtype=None):
     X: (T, K), dY: (T, N), offsets as in gemm_grouped.  dW: (E, K, N) of X's type, or float32."""
     op = "gemm_grouped_wgrad"
     if not _is_torch(X):
-        return _host_wgrad(op, X, dY, offsets, out)
+        return _host_wgrad(op, X, dY, offsets, out, out_dtype)
     code, index = _tensors(op, (2, 2), X, dY)
     T, K = X.shape
     N, E = dY.shape[1], offsets.shape[0] - 1 if offsets.dim() else 0
@@ -277,7 +287,7 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
     (tensors only).  float16: in dW, tokens whose weight |dloss| max |H[t]| is below 2^-30 of the heaviest's lose bits."""
     op = "xent_grad"
     if not _is_torch(H):
-        return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW)
+        return _host_xent_grad(op, H, W, labels, lse, dloss, dH, dW, out_dtype)
     code, index, T, V, D, bits = _xent_args(op, H, W, labels)
     _floats(op, lse, index, T)
     _floats(op, dloss, index, T)
