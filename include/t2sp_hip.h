@@ -365,7 +365,8 @@ int t2sp_xent_grad_rounded(int type, int out_type, const void *H, const void *W,
  *   y[m,n] = sum_k x[m,k] * (q[n,k] - z[n,k/group]) * s[n,k/group],  q in 0 .. 15, z = 8 without zero points
  * group: 32, 64, 128, ... (a power of two; at least K for one scale per row).  x, y, scales and zero points
  * are of `type`; sums in float.  E matrices, of which row m takes matrix ids[m] (E = 1 and ids = NULL: all rows
- * take the one); an id outside 0 .. E - 1 gives a row of zeros.  With ids at most 65535 rows.  Infinities and NaN in x
+ * take the one); an id outside 0 .. E - 1 gives a row of zeros.  With ids at most 65535 rows.  Several
+ * rows of x lie at most T2SP_MAX_ROW_BYTES apart.  Infinities and NaN in x
  * give what the formula gives (a row with an infinity takes about a millisecond).
  * The kernel reads a layout of its own that t2sp_w4_pack makes once, on the device, from plain arrays:
  * q one number per byte (its low four bits), N x K with row stride ldq and sq between matrices; scales and

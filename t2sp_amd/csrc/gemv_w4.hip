@@ -447,6 +447,7 @@ extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *
         return T2SP_ERR_SHAPE;
     if (M == 0) return T2SP_OK;
     if (!x || !Q || !S || !y || (!ids && E != 1)) return T2SP_ERR_SHAPE;
+    if (M == 1) ldx = K;                                                 // (a single row's stride carries no information)
     if (ldx * size > T2SP_MAX_ROW_BYTES) return T2SP_ERR_SHAPE;          // (64 rows of x within 31 bits)
     if (reinterpret_cast<uintptr_t>(Q) % 16 || reinterpret_cast<uintptr_t>(S) % 16 || reinterpret_cast<uintptr_t>(Z) % 16) return T2SP_ERR_SHAPE;
     W4Args g{};

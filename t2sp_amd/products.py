@@ -6,6 +6,8 @@ the call returns without waiting, so it can be captured into a HIP graph; worksp
 torch's allocator, which keeps them apart between streams and captured graphs.  Element types are float32, float16
 and bfloat16.  numpy arrays (float32 or float16, host memory) go through the operator entries
 (include/gemm_grouped-interface.h, xent-interface.h, gemv_w4-interface.h), which stage them through the device.
+Rows of a matrix may lie any distance apart but must not overlap (an expanded tensor is refused with -8: pass a copy).
+Results carry no autograd graph, whatever their operands require; the gradients are calls of their own.
 Misuse raises T2spError with the Halide error code that the entry would return."""
 import ctypes
 
@@ -17,6 +19,7 @@ from .ops import T2spError, _check, _is_torch, host_empty
 
 BAD_TYPE, SHAPE, BAD_DIMENSIONS = -3, -8, -43
 _F32 = 0                                     # T2SP_TYPE_F32
+_MAX_ROW_BYTES = 1 << 23                     # T2SP_MAX_ROW_BYTES
 _codes = None                                # torch dtype -> T2SP_TYPE_*; set with the other torch names on first use
 
 
@@ -83,11 +86,11 @@ def _result(op, out, shape, like, dtype=None):
 
 def _row(t):
     """Elements between rows (a single row's stride carries no information)."""
-    return t.stride(-2) if t.shape[-2] > 1 else max(t.stride(-2), t.shape[-1])
+    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
 
 
 def _matrix(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * _row(t))
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * _row(t)
 
 
 class _On:
@@ -325,6 +328,7 @@ class W4:
         if isinstance(Q, np.ndarray):        # host arrays as they are: the entry lays them out on the device
             return
         self.dtype, self.code, self.index = S.dtype, _torch()[S.dtype], S.get_device()
+        self.max_ld = _MAX_ROW_BYTES // S.element_size()
         self.pointers = Q.data_ptr(), S.data_ptr(), Z.data_ptr() if Z is not None else None
 
 
@@ -376,7 +380,9 @@ def gemv_w4(x, w, ids=None, out=None):
     if x.dim() != 2:
         raise T2spError(op, BAD_DIMENSIONS)
     (M, K), index = x.shape, w.index
-    ldx = x.stride(0)
+    ldx = x.stride(0) if M > 1 else K
+    if ldx > w.max_ld:                       # (rows that lie further apart than the kernel reaches, such as every sequence's last one)
+        x, ldx = x.contiguous(), K
     if K != w.K or x.get_device() != index or (x.stride(1) != 1 and K > 1) or (ids is None) != (w.E is None):
         raise T2spError(op, SHAPE)
     if ids is not None:
@@ -393,5 +399,5 @@ def gemv_w4(x, w, ids=None, out=None):
             return gemv_w4(x, w, ids, out)
     Q, S, Z = w.pointers
     _check(op, lib().t2sp_gemv_w4(w.code, x.data_ptr(), Q, S, Z, None if ids is None else ids.data_ptr(), out.data_ptr(), M, w.N, K, w.E or 1, w.group,
-                                  ldx if M > 1 or ldx > K else K, ldy, _raw_stream(index)))
+                                  ldx, ldy, _raw_stream(index)))
     return out
