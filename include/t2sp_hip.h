@@ -299,6 +299,8 @@ int t2sp_capsule_packed_f32(const float *P2, int64_t ldp, const float *W2, int64
 
 /* ---- The products of a language model's layers: elements of 16 or 32 bits, sums in 32 bits. ----
  * They have no counterpart in the reference, whose pipelines are single precision and of one size.
+ * Calls whose launches would take more than 2^31 threads (a thread for about 128 results: 1M tokens x 262144 words)
+ * are refused with T2SP_ERR_SHAPE.
  * `type` is the element type of the operands, `out_type` that of the result: the same type or
  * T2SP_TYPE_F32.  Leading dimensions and strides are in elements and must not be negative. */
 #define T2SP_TYPE_F32 0
@@ -378,6 +380,20 @@ int t2sp_w4_pack(int type, const uint8_t *q, const void *scales, const void *zer
                  void *stream);
 int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *S, const void *Z, const int *ids, void *y, int M,
                  int N, int K, int E, int group, int64_t ldx, int64_t ldy, void *stream);
+
+/* What the launchers of these products choose for aligned operands, for tests (they plan for t2sp_machine_cus()
+ * compute units; no device is needed); T2SP_ERR_SHAPE for extents that the calls refuse.
+ *   t2sp_gemm_grouped_plan: the rows of a tile, 16 to 256; *few: whether the matrix goes straight from memory into
+ *     the matrix cores (16, 32 or 64 rows) instead of through LDS (64, 128 or 256);
+ *   t2sp_gemm_grouped_wgrad_plan: the tile's edge, and the parts that the rows are summed in;
+ *   t2sp_xent_plan: the tile's edge; t2sp_xent_grad_plan: the words of a piece of the vocabulary, and the edges
+ *     and parts (logits' tile, dH's tile, parts of its reduction, dW's tile, parts of its reduction);
+ *   t2sp_gemv_w4_plan: tiles of 16 rows of x, and of the matrix, per workgroup. */
+int t2sp_gemm_grouped_plan(int type, int opb, int T, int E, int K, int N, int *few);
+int t2sp_gemm_grouped_wgrad_plan(int type, int T, int E, int K, int N, int *parts);
+int t2sp_xent_plan(int type, int T, int V, int D);
+int t2sp_xent_grad_plan(int type, int rounded, int T, int V, int D, int *out5);
+int t2sp_gemv_w4_plan(int type, int ids, int M, int N, int K, int group, int *matrix_tiles);
 
 /* dst[sum_d c_d*dst_strides[d]] = src[sum_d c_d*src_strides[d]] for every coordinate c of the
  * box `extents` (nd <= T2SP_MAX_DIMS, dimension 0 fastest).  Device-side replacement of the

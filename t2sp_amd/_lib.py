@@ -130,6 +130,9 @@ def _declare(L):
     L.t2sp_xent.argtypes = [i32, vp, vp, vp, i32, vp, vp, i32, i32, i32, i64, i64, vp, sz, vp]
     for name in ("t2sp_xent_grad", "t2sp_xent_grad_rounded"):
         getattr(L, name).argtypes = [i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, i64, vp, sz, vp]
+    for name, args in (("t2sp_gemm_grouped_plan", [i32] * 6 + [p32]), ("t2sp_gemm_grouped_wgrad_plan", [i32] * 5 + [p32]), ("t2sp_xent_plan", [i32] * 4),
+                       ("t2sp_xent_grad_plan", [i32] * 5 + [p32]), ("t2sp_gemv_w4_plan", [i32] * 6 + [p32])):
+        getattr(L, name).argtypes = args
     L.t2sp_w4_sizes.argtypes = [i32, i32, i32, p64, p64]
     L.t2sp_w4_pack.argtypes = [i32, vp, vp, vp, i32, i32, i32, i32] + [i64] * 6 + [vp, vp, vp, vp]
     L.t2sp_gemv_w4.argtypes = [i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, vp]

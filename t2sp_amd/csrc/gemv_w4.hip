@@ -45,7 +45,7 @@ struct W4Args {
     int64_t ldx, ldy;                    // elements
     int blocks_k, tiles_n;               // of 128 inputs, of 16 rows
     int group_shift;                     // G = 32 << group_shift
-    int groups, group_blocks;            // in K; blocks of scales (of 4, 2 or 1 groups)
+    int group_blocks;                    // of scales (of 4, 2 or 1 groups)
     int vec_x;                           // rows of x are whole 16-byte chunks
 };
 
@@ -419,22 +419,26 @@ static int launch_w4(const W4Args &g, hipStream_t st) {
 // 128: 12.6 us with one row and one tile per workgroup, 11.3 with four; 64 rows: 67 us with one tile, 40 with two.  8192 x 4096 is
 // the border: one row 7.4 us with one tile, 10.8 with four, 64 rows 35 and 21 with two.  Floats have no registers left for it but for one
 // row tile and large groups (16384 x 4096: 24 us with one tile, 16 with four).
+struct W4Form {
+    int mt, nt;                              // tiles of 16 rows of x, of the matrix
+};
+static W4Form w4_form(int size, bool ids, int M, int tiles_n, int group_shift, bool vec_x) {
+    const int cus = machine().cus;
+    if (ids || M <= 16) return {1, vec_x && !ids && tiles_n >= 4 * cus && (size == 2 || group_shift >= 2) ? 4 : 1};
+    if (!vec_x) return {2, 1};
+    return {M <= 32 ? 2 : 4, size == 2 && tiles_n >= 2 * cus ? 2 : 1};
+}
 template <class T>
 static int launch_w4(const W4Args &g, hipStream_t st) {
-    const int64_t cus = machine().cus;
-    constexpr bool narrow = sizeof(T) == 2;
-    if (g.ids || g.M <= 16) {
-        if (!g.vec_x) return launch_w4<T, 1, 1, false>(g, st);
-        if (!g.ids && g.tiles_n >= 4 * cus) {
-            if constexpr (narrow) return launch_w4<T, 1, 4, true>(g, st);
-            else if (g.group_shift >= 2) return launch_w4<T, 1, 4, 2, true>(g, st);
-        }
-        return launch_w4<T, 1, 1, true>(g, st);
+    const W4Form form = w4_form(sizeof(T), g.ids, g.M, g.tiles_n, g.group_shift, g.vec_x);
+    if (!g.vec_x) return form.mt == 1 ? launch_w4<T, 1, 1, false>(g, st) : launch_w4<T, 2, 1, false>(g, st);
+    if constexpr (sizeof(T) == 2) {
+        if (form.nt == 4) return launch_w4<T, 1, 4, true>(g, st);
+        if (form.nt == 2) return form.mt == 2 ? launch_w4<T, 2, 2, true>(g, st) : launch_w4<T, 4, 2, true>(g, st);
+    } else {
+        if (form.nt == 4) return launch_w4<T, 1, 4, 2, true>(g, st);
     }
-    if constexpr (narrow)
-        if (g.vec_x && g.tiles_n >= 2 * cus) return g.M <= 32 ? launch_w4<T, 2, 2, true>(g, st) : launch_w4<T, 4, 2, true>(g, st);
-    if (!g.vec_x) return launch_w4<T, 2, 1, false>(g, st);
-    return g.M <= 32 ? launch_w4<T, 2, 1, true>(g, st) : launch_w4<T, 4, 1, true>(g, st);
+    return form.mt == 1 ? launch_w4<T, 1, 1, true>(g, st) : form.mt == 2 ? launch_w4<T, 2, 1, true>(g, st) : launch_w4<T, 4, 1, true>(g, st);
 }
 }  // namespace t2sp
 
@@ -458,7 +462,6 @@ extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *
     g.ldx = ldx; g.ldy = ldy;
     g.blocks_k = (int)(((int64_t)K + 127) / 128); g.tiles_n = (int)(((int64_t)N + 15) / 16);
     g.group_shift = group_shift_of(group);
-    g.groups = (K + group - 1) / group;
     g.group_blocks = (int)group_blocks_of(K, group);
     g.vec_x = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && (int64_t)K % 8 == 0;
     const hipStream_t st = (hipStream_t)stream;
@@ -466,4 +469,12 @@ extern "C" int t2sp_gemv_w4(int type, const void *x, const void *Q, const void *
         using T = std::remove_pointer_t<decltype(t)>;
         return launch_w4<T>(g, st);
     });
+}
+
+extern "C" int t2sp_gemv_w4_plan(int type, int ids, int M, int N, int K, int group, int *matrix_tiles) {
+    int64_t qb, se;
+    if (!type_bytes(type) || M < 1 || M > T2SP_MAX_EXTENT || t2sp_w4_sizes(N, K, group, &qb, &se) || !matrix_tiles) return T2SP_ERR_SHAPE;
+    const W4Form form = w4_form(type_bytes(type), ids, M, (int)(((int64_t)N + 15) / 16), group_shift_of(group), K % 8 == 0);
+    *matrix_tiles = form.nt;
+    return form.mt;
 }

@@ -526,19 +526,30 @@ static double grouped_cost(const GroupShape &s, int T, int E, int K, int N, int 
     return std::max(work, reads) + 0.25 * std::min(work, reads);
 }
 
-template <class T, class O, int BS>
-static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
+// The rows of a tile; `few`: straight from memory (16, 32 or 64 rows), else through LDS (64, 128 or 256).
+struct GroupForm {
+    int rows;
+    bool few;
+};
+template <class T, int BS>
+static GroupForm forward_form(int rows, int E, int K, int N) {
     typedef GroupShapes<T, BS> S;
-    auto cost = [&](const GroupShape &s) { return grouped_cost(s, g.T, g.E, g.K, g.N, sizeof(T)); };
+    auto cost = [&](const GroupShape &s) { return grouped_cost(s, rows, E, K, N, sizeof(T)); };
     const double few1 = cost(S::FEW1), few2 = cost(S::FEW2), few4 = cost(S::FEW4), c64 = cost(S::T64), c128 = cost(S::T128),
                  c256 = sizeof(T) == 2 ? cost(S::T256) : 1e30;
     const double best = std::min({few1, few2, few4, c64, c128, c256});
-    if (best == few1) return launch_few_rows<T, O, BS, 1>(g, stream);
-    if (best == few2) return launch_few_rows<T, O, BS, 2>(g, stream);
-    if (best == few4) return launch_few_rows<T, O, BS, 4>(g, stream);
+    if (best == few1 || best == few2 || best == few4) return {best == few1 ? 16 : best == few2 ? 32 : 64, true};
+    return {best == c256 ? 256 : best == c128 ? 128 : 64, false};
+}
+template <class T, class O, int BS>
+static int forward_tiles(const GroupedArgs &g, hipStream_t stream) {
+    const GroupForm form = forward_form<T, BS>(g.T, g.E, g.K, g.N);
+    if (form.few) return form.rows == 16   ? launch_few_rows<T, O, BS, 1>(g, stream)
+                         : form.rows == 32 ? launch_few_rows<T, O, BS, 2>(g, stream)
+                                           : launch_few_rows<T, O, BS, 4>(g, stream);
     if constexpr (sizeof(T) == 2)
-        if (best == c256) return launch_forward<Tile256<T, KMAJOR, BS>, O>(g, stream);
-    if (best == c128) return launch_forward<Tile128<T, KMAJOR, BS>, O>(g, stream);
+        if (form.rows == 256) return launch_forward<Tile256<T, KMAJOR, BS>, O>(g, stream);
+    if (form.rows == 128) return launch_forward<Tile128<T, KMAJOR, BS>, O>(g, stream);
     return launch_forward<Tile64<T, BS>, O>(g, stream);
 }
 
@@ -550,6 +561,8 @@ static int wgrad_parts(int T, int E, int K, int N, int size) {
     return split_parts(tiles, machine().cus, (double)T / E * size / 64, s.a + s.c, 4.0 * E * K * N);
 }
 static int64_t plane_cols(int N) { return (N + 3) / 4 * 4; }
+// The tile edge of sums that are not cut.
+static int wgrad_tile(int T, int E, int K, int N, int size) { return pick_tile(E, K, N, (T + E - 1) / E, size, false); }
 
 template <class T, class O>
 static int wgrad_tiles(const GroupedArgs &g, float *planes, int out_type, hipStream_t stream) {
@@ -562,10 +575,8 @@ static int wgrad_tiles(const GroupedArgs &g, float *planes, int out_type, hipStr
         if (int err = launch_wgrad<Tile128<T, KROWS, KROWS>, float>(p, stream)) return err;
         return launch_join_planes(planes, g.parts, g.E, g.K, g.N, p.ldy, g.Y, out_type, g.ldy, g.sw, stream);
     }
-    const int64_t per = (g.T + g.E - 1) / g.E;
-    const int tile = pick_tile(g.E, g.K, g.N, per, sizeof(T), false);
     if constexpr (sizeof(T) == 2)
-        if (tile == 256) return launch_wgrad<Tile256<T, KROWS, KROWS>, O>(g, stream);
+        if (wgrad_tile(g.T, g.E, g.K, g.N, sizeof(T)) == 256) return launch_wgrad<Tile256<T, KROWS, KROWS>, O>(g, stream);
     return launch_wgrad<Tile128<T, KROWS, KROWS>, O>(g, stream);
 }
 
@@ -681,4 +692,19 @@ extern "C" int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, co
     return with_types(type, out_type, [&](auto *t, auto *o) {
         return wgrad_tiles<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(g, reinterpret_cast<float *>(room), out_type, st);
     });
+}
+
+extern "C" int t2sp_gemm_grouped_plan(int type, int opb, int T, int E, int K, int N, int *few) {
+    if (!type_bytes(type) || T < 1 || T > T2SP_MAX_EXTENT || !extent_ok(E) || !extent_ok(K) || !extent_ok(N) || !few) return T2SP_ERR_SHAPE;
+    return with_types(type, type, [&](auto *t, auto *) {
+        using TT = std::remove_pointer_t<decltype(t)>;
+        const GroupForm form = opb ? forward_form<TT, KMAJOR>(T, E, K, N) : forward_form<TT, KROWS>(T, E, K, N);
+        *few = form.few;
+        return form.rows;
+    });
+}
+extern "C" int t2sp_gemm_grouped_wgrad_plan(int type, int T, int E, int K, int N, int *parts) {
+    if (!type_bytes(type) || T < 0 || T > T2SP_MAX_EXTENT || !extent_ok(E) || !extent_ok(K) || !extent_ok(N) || !parts) return T2SP_ERR_SHAPE;
+    *parts = wgrad_parts(T, E, K, N, type_bytes(type));
+    return *parts > 1 ? 128 : wgrad_tile(T, E, K, N, type_bytes(type));
 }

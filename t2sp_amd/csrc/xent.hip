@@ -459,6 +459,8 @@ static int dw_splits(int T, int D, int piece, int size, int numbers) {
     return split_parts(tiles, machine().cus, (double)T * size * numbers / 64, s.a + s.c, 4.0 * piece * D);
 }
 
+static int dw_tile(int T, int D, int piece, int size, int numbers) { return pick_tile(1, piece, D, (int64_t)T * numbers, size, false); }
+
 static XentRoom xent_room(bool backward, int numbers, int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw) {
     const int size = type_bytes(type);
     XentRoom r{};
@@ -617,8 +619,8 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
                 if (!(err = launch_dw<Tile128<T, KROWS, KROWS>, float>(p, st)))
                     err = launch_join_planes(reinterpret_cast<const float *>(room + r.dw), p.splits, 1, p.rows, p.cols, p.ldo, out, out_type, lddw, 0, st);
             } else {
-                err = pick_tile(1, p.rows, p.cols, (int64_t)p.k * p.numbers, size, false) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
-                                                                          : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
+                err = dw_tile(p.k, p.cols, p.rows, size, p.numbers) == 256 ? launch_dw<Large<T, KROWS, KROWS>, O>(p, st)
+                                                                           : launch_dw<Tile128<T, KROWS, KROWS>, O>(p, st);
             }
             if (err) return err;
         }
@@ -714,4 +716,19 @@ extern "C" int t2sp_xent_grad_rounded(int type, int out_type, const void *H, con
                                       int64_t lddw, void *workspace, size_t workspace_bytes, void *stream) {
     return xent_gradients(true, type, out_type, H, W, labels, label_bits, lse, dloss, dH, dW, T, V, D, ldh, ldw, lddh, lddw, workspace,
                           workspace_bytes, stream);
+}
+
+extern "C" int t2sp_xent_plan(int type, int T, int V, int D) {
+    return xent_args_ok(type, T, V, D, D, D) && T ? logits_shape(T, V, D, type_bytes(type)) : T2SP_ERR_SHAPE;
+}
+extern "C" int t2sp_xent_grad_plan(int type, int rounded, int T, int V, int D, int *out5) {
+    if (!xent_args_ok(type, T, V, D, D, D) || !T || !out5) return T2SP_ERR_SHAPE;
+    const int size = type_bytes(type), numbers = numbers_of(type, rounded);
+    const XentRoom r = xent_room(true, numbers, type, nullptr, nullptr, T, V, D, D, D);
+    out5[0] = logits_shape(T, r.piece, D, size);
+    out5[1] = dh_tile(T, size);
+    out5[2] = r.splits;
+    out5[3] = r.dw_parts > 1 ? 128 : dw_tile(T, D, r.piece, size, numbers);
+    out5[4] = r.dw_parts;
+    return r.piece;
 }

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 import t2sp_amd
-from test_grouped_gpu import TYPES, dt, make, within
+import test_products_plans as plans
+from test_grouped_gpu import TYPES, check_forward, check_wgrad, make, within
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,45 @@ def test_offsets_of_any_values(E, T):
     up = np.sort(rng.integers(0, T, E + 1))
     up[rng.integers(0, E + 1, 3)] = 0
     expect(X, W, D, up.tolist(), 0)
+
+
+def on_full_card():
+    """The tables of forms are for 256 compute units."""
+    L = t2sp_amd.lib()
+    if L.t2sp_machine_cus() != 256 or L.t2sp_machine_xcds() != 8:
+        pytest.skip("the forms of these sizes are known for a full card only")
+    return L
+
+
+@pytest.mark.parametrize("case", range(len(plans.FORWARD)))
+def test_every_form_of_the_product(case):
+    """Results of the operands' type and in float; rows in front of and behind the groups are left."""
+    import torch
+    form, types, opb, sizes, K, N = plans.FORWARD[case]
+    T, E = sum(sizes), len(sizes)
+    for dtype in types:
+        assert plans.forward_form(on_full_card(), dtype, opb, T, E, K, N) == form
+        X, W = make((T, K), dtype, 1), make((E, N, K) if opb else (E, K, N), dtype, 2, K ** -0.5)
+        check_forward(X, W, sizes, opb)
+        if dtype != "float32":
+            check_forward(X, W, sizes, opb, out_dtype=torch.float32)
+        first = sizes[0] // 2                               # the same launch with the offsets moved: other rows per tile
+        o = np.concatenate([[first], np.cumsum(sizes)])
+        Y = torch.full((T, N), 3.0, dtype=X.dtype, device="cuda")
+        t2sp_amd.gemm_grouped(X, W, torch.tensor(o, dtype=torch.int32).cuda(), opb=opb, out=Y)
+        assert (Y[:first] == 3).all()
+        within(Y[first:sizes[0]], X[first:sizes[0]].double() @ (W[0].double().t() if opb else W[0].double()),
+               X[first:sizes[0]].double().abs() @ (W[0].double().abs().t() if opb else W[0].double().abs()), K, Y.dtype)
+
+
+@pytest.mark.parametrize("case", range(len(plans.WGRAD)))
+def test_every_form_of_the_gradient_of_the_matrices(case):
+    import torch
+    tile, parts, types, sizes, K, N = plans.WGRAD[case]
+    T = sum(sizes)
+    for dtype in types:
+        assert plans.wgrad_form(on_full_card(), dtype, T, len(sizes), K, N) == (tile, parts)
+        X, D = make((T, K), dtype, 3), make((T, N), dtype, 4)
+        check_wgrad(X, D, sizes)
+        if dtype != "float32":
+            check_wgrad(X, D, sizes, out_dtype=torch.float32)

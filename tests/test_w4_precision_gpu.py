@@ -4,6 +4,8 @@ import numpy as np
 import pytest
 
 import t2sp_amd
+import test_products_plans as plans
+from test_grouped_forms_gpu import on_full_card
 from test_w4_gpu import TYPES, close, dt, rows, weights
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +111,24 @@ def test_infinities_with_a_matrix_for_each_row(dtype):
             same_kind(y[m:m + 1], x[m:m + 1], q[e], s[e], z[e], group)
         else:
             assert (y[m] == 0).all()
+
+
+@pytest.mark.parametrize("case", range(len(plans.W4)))
+@pytest.mark.parametrize("zeros", [False, True])
+def test_every_form_of_the_product(case, zeros):
+    """Matrices whose last tiles are partial and whose last workgroup has tiles behind the last one."""
+    import torch
+    mt, nt, types, M, N, K, group = plans.W4[case]
+    for dtype in types:
+        assert plans.w4_form(on_full_card(), dtype, 0, M, N, K, group) == (mt, nt)
+        q, s, z = weights((N, K), group, dtype, zeros, 9)
+        x = rows(M, K, dtype, 10)
+        out = torch.full((M + 1, N + 9), 7.0, dtype=dt(dtype), device="cuda")
+        w = t2sp_amd.pack_w4(q, s, z, group=group)
+        t2sp_amd.gemv_w4(x, w, out=out[:M, 3:N + 3])
+        close(out[:M, 3:N + 3], x, q, s, z, group)
+        assert (out[:, :3] == 7).all() and (out[:, N + 3:] == 7).all() and (out[M] == 7).all()
+        x[M - 1, 1] = float("inf")
+        y = t2sp_amd.gemv_w4(x, w)
+        assert torch.equal(y[:M - 1], out[:M - 1, 3:N + 3])
+        same_kind(y[M - 1:, -40:], x[M - 1:], q[-40:], s[-40:], None if z is None else z[-40:], group)
