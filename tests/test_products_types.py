@@ -74,3 +74,21 @@ def test_host_arrays_without_rows():
     assert dH.shape == (0, 8) and dW.shape == (20, 8) and (dW == 0).all()
     dW = t2sp_amd.gemm_grouped_wgrad(np.zeros((0, 8), np.float16), np.zeros((0, 5), np.float16), np.zeros(4, np.int32))
     assert dW.shape == (3, 8, 5) and (dW == 0).all()
+
+
+def test_the_rounded_gradient_refuses_what_the_other_does():
+    L = t2sp_amd.lib()
+    if L.t2sp_device_count() > 0:
+        pytest.skip("made-up addresses: for machines without a device")
+    P = 0x7f0000000000
+    names = ("type", "out", "H", "W", "l", "bits", "lse", "dl", "dH", "dW", "T", "V", "D", "ldh", "ldw", "lddh", "lddw", "ws", "wb", "st")
+    good = dict(type=2, out=2, H=P, W=P, l=P, bits=64, lse=P, dl=P, dH=P, dW=P, T=8, V=100, D=64, ldh=64, ldw=64, lddh=64, lddw=64, ws=P, wb=1 << 40,
+                st=None)
+    for f in (L.t2sp_xent_grad, L.t2sp_xent_grad_rounded):
+        call = lambda **k: f(*[dict(good, **k)[n] for n in names])
+        for bad in (dict(type=3), dict(out=1), dict(bits=8), dict(T=-1), dict(V=0), dict(D=0), dict(ldh=63), dict(lddw=63), dict(H=None), dict(lse=None),
+                    dict(ws=None), dict(ws=P + 8), dict(wb=1 << 10)):
+            assert call(**bad) == -8, bad
+        assert call(dH=None, dW=None) == 0 and call(T=0, dW=None) == 0
+    sizes = [L.t2sp_xent_grad_workspace_bytes(t, P, P, 8192, 128000, 4096, 4096, 4096) for t in (0, 1, 2)]
+    assert min(sizes) > 8192 * 4096 * 4 * 2 and max(sizes) < 2 << 30

@@ -182,3 +182,36 @@ def test_infinite_logits(dtype, V):
     W[:, 0] = -1.0
     lse3 = t2sp_amd.xent(H, W, lab)[1]
     assert lse3[3] == -inf and lse3[9] == inf and torch.equal(lse3[rest], lse0[rest])
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rounded", [False, True])
+def test_replayed_graphs_of_both_forms(dtype, rounded):
+    """Weights and hidden states that change between replays; two graphs and eager calls in turn."""
+    import torch
+    T, V, D = 130, 500, 72
+    H, W, lab = quarters((T, D), dtype, 1, 4), quarters((V, D), dtype, 2, 1), labels_for(T, V, 3)
+    d = mean_of(lab, V)
+
+    def step():
+        loss, lse = t2sp_amd.xent(H, W, lab)
+        return (loss, lse) + t2sp_amd.xent_grad(H, W, lab, lse, d, rounded=rounded)
+    step()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, res))
+    gen = torch.Generator().manual_seed(6)
+    for turn in range(4):
+        d.copy_(torch.randn(T, generator=gen) * 10.0 ** (-2 * turn))
+        H.copy_((torch.randint(-4, 5, (T, D), generator=gen).float() / 4).to(dt(dtype)))
+        want = step()
+        for g, res in graphs:
+            for r in res:
+                r.fill_(float("nan"))
+            g.replay()
+        torch.cuda.synchronize()
+        for g, res in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(want, res))
