@@ -14,19 +14,22 @@
 // p - [label] is a float, which the 16-bit matrix cores do not take: it goes in as the sum of two numbers of the operands'
 // type, its rounding and the rounding of what that leaves (16 bits with bfloat16, 22 with half), and both products run over
 // both.  12 T D V operations in all, of which 2 T D V pay for not holding T x V logits and 4 T D V for the second number.
-// What they leave is below what the float sums of z do (2048 tokens, 4096 wide, 32000 words, bfloat16, float results: the
-// gradients are off by 8e-7 and 5e-7 in norm, by 2e-7 for the two numbers alone, by 1.1e-4 with one; a third number changes
-// nothing).  Callers who accept half a step of the type in p - [label] (t2sp_xent_grad_rounded) have one: 8 T D V.
+// What they leave is below what the float sums of z do (8192 tokens, 4096 wide, 128000 words, bfloat16, float results, against
+// float64: dH and dW are off by 6e-7 and 8e-7 in norm, by 9e-8 for the two numbers alone, by 5e-5 with one; a third number
+// changes nothing; torch's products of floats: 6e-6 and 1.5e-6).  Callers who accept half a step of the type in p - [label] (t2sp_xent_grad_rounded) have one: 8 T D V.
 //
-// Weights of the tokens.  dloss[t] = m 2^x with 1/2 <= |m| < 1 is a factor of both products' reductions or rows.  p - [label]
-// is stored times m 2^b, the rows of H for dW are copied times 2^a, exactly, with a + b = x + C for one C of all tokens; dH's rows
-// are multiplied by 2^(x - b) at the end, dW by 2^-C.  bfloat16 and float: b = 0, and C makes the largest a zero.  half has
+// Weights of the tokens.  dloss[t] = top m 2^x with top = max |dloss| and 1/2 <= |m| < 1 is a factor of both products' reductions
+// or rows.  p - [label] is stored times m 2^b, the rows of H for dW are copied times 2^a, exactly, with a + b = x + C for one C of
+// all tokens; dH's rows are multiplied by top 2^(x - b) at the end, dW by top 2^-C.  Equal weights, the usual case, thus change no
+// bit of either matrix (with dloss itself for top m 2^x, and m some fraction in p - [label], the gradients of a mean over 7700 tokens
+// were off by 2.4e-6 in norm instead of 6e-7).  bfloat16 and float: b = 0.  half has
 // room between 2^-24 and 2^16 only, so its b is 15 (the probabilities of a large vocabulary reach far below 1, and together
-// the two numbers go down to 2^-40 of that) and C is the largest for which no copied element exceeds 2^15.  A lighter token's
-// a is smaller by d = its distance, as a power of two, from the token that decides C.  Up to d = 20 that costs no bits of
-// elements down to 2^-8 of the row's largest; the next 10 are taken from b; then a falls further.  So weights (times the size of
-// the row) down to 2^-30 of the heaviest keep their bits, below that elements underflow.  (With dloss / max |dloss| rounded into
-// the copy, weights of 1e-6 of the heaviest put dW off by 2 %.)
+// the two numbers go down to 2^-40 of that) and C is the largest for which no copied element exceeds 2^15, or half of
+// that.  A lighter token's a is smaller by d = its distance, as a power of two, from the token that decides C.  Up to d = 20 that
+// costs no bits of elements down to 2^-8 of the row's largest; the next 10 are taken from b; then a falls further.  So weights (times
+// the size of the row) down to 2^-30 of the heaviest keep their bits, below that elements underflow.  (With dloss / max |dloss|
+// rounded into the copy, weights of 1e-6 of the heaviest put dW off by 2 %.)
+// With p - [label] rounded to one number m goes into the copy of H instead, and into dH's rows at the end.
 // The copy of H also holds zeros for tokens without a label: what their rows hold (padding may be anything) reaches
 // no sum.
 #include "product_core.hpp"
@@ -45,7 +48,8 @@ struct XentArgs {
     float *hit;                          // [T]: z at the label
     // backward
     const float *lse, *dloss;
-    const int *common, *row_exp;         // see the weights of the tokens above; row_exp: half only
+    const struct Common *common;         // see the weights of the tokens above
+    const int *row_exp;                  // half only
     char *G;                             // [numbers][T][ldg] p - [label] times m 2^b of the piece, zeros from vp to ldg
     int64_t ldg;
     int numbers;                         // of the type that p - [label] is the sum of
@@ -167,20 +171,24 @@ __global__ void __launch_bounds__(64 * JOIN_WAVES) xent_join_kernel(const float2
 
 // The weights of the tokens (see above).
 constexpr int NO_EXPONENT = -0x7fffffff - 1;         // of a row without a finite element but zeros
+struct Common {
+    float top;
+    int c;
+};
 struct TokenWeight {
-    float g;                                         // m 2^b (dloss itself where it is 0 or not finite)
-    int a, u;                                        // u = x - b
+    float m;                                         // (dloss itself where it is 0 or not finite)
+    int a, b, u;                                     // u = x - b
 };
 template <class T>
-__device__ __forceinline__ TokenWeight token_weight(float dloss, const int *row_exp, int t, int common) {
-    if (dloss == 0.f || !(fabsf(dloss) < __builtin_inff())) return {dloss, 0, 0};
+__device__ __forceinline__ TokenWeight token_weight(float dloss, const int *row_exp, int t, Common common) {
+    if (dloss == 0.f || !(fabsf(dloss) < __builtin_inff())) return {dloss, 0, 0, 0};
     int x;
-    const float m = frexpf(dloss, &x);
-    if constexpr (!std::is_same_v<T, _Float16>) return {m, x + common, x};
+    const float m = frexpf(dloss / common.top, &x);
+    if constexpr (!std::is_same_v<T, _Float16>) return {m, x + common.c, 0, x};
     const int e = row_exp[t];
-    if (e == NO_EXPONENT) return {ldexpf(m, 15), 0, x - 15};
-    const int lighter = 30 - e - x - common, b = 15 - (lighter <= 20 ? 0 : lighter <= 30 ? lighter - 20 : 10);
-    return {ldexpf(m, b), x + common - b, x - b};
+    if (e == NO_EXPONENT) return {m, 0, 15, x - 15};
+    const int lighter = 30 - e - x - common.c, b = 15 - (lighter <= 20 ? 0 : lighter <= 30 ? lighter - 20 : 10);
+    return {m, x + common.c - b, b, x - b};
 }
 
 // row_exp[t] = e: the largest finite |H[t, :]| is in 2^(e - 1) .. 2^e.  One wave per token.
@@ -208,55 +216,73 @@ __global__ void __launch_bounds__(256) xent_row_exponents_kernel(const _Float16 
     }
 }
 
-// C, from the tokens with a label and a finite weight other than 0; in every thread of a workgroup.
+// top and C, from the tokens with a label and a finite weight other than 0; in every thread of a workgroup.  The exponent of dloss / top
+// is at most one more than the difference of the two exponents: with that half's C is found in the same pass over the tokens as top.
 template <class T, int THREADS>
-__device__ __forceinline__ int common_exponent(const float *dloss, const void *labels, int lab64, const int *row_exp, int rows, int V) {
+__device__ __forceinline__ Common common_weight(const float *dloss, const void *labels, int lab64, const int *row_exp, int rows, int V) {
     constexpr int WAVES = THREADS / 64, NONE = 0x7fffffff;
+    __shared__ float tops[WAVES];
     __shared__ int joint[WAVES];
+    float top = 0.f;
     int least = NONE;
     for (int t = threadIdx.x; t < rows; t += THREADS) {
         const int64_t label = label_of(labels, lab64, t);
         const float v = fabsf(dloss[t]);
         if (label < 0 || label >= V || !(v > 0.f && v < __builtin_inff())) continue;
-        int x, e = 30;
-        frexpf(v, &x);
-        if constexpr (std::is_same_v<T, _Float16>) e = row_exp[t];
-        if (e != NO_EXPONENT) least = min(least, 30 - e - x);
+        top = fmaxf(top, v);
+        if constexpr (std::is_same_v<T, _Float16>) {
+            int x;
+            frexpf(v, &x);
+            if (const int e = row_exp[t]; e != NO_EXPONENT) least = min(least, 30 - e - x);
+        }
     }
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) least = min(least, __shfl_xor(least, m, 64));
-    if ((threadIdx.x & 63) == 0) joint[threadIdx.x >> 6] = least;
+    for (int m = 32; m >= 1; m >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, m, 64));
+        least = min(least, __shfl_xor(least, m, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        tops[threadIdx.x >> 6] = top;
+        joint[threadIdx.x >> 6] = least;
+    }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) least = min(least, joint[w]);
-    return least == NONE ? 0 : least;
+    for (int w = 0; w < WAVES; w++) {
+        top = fmaxf(top, tops[w]);
+        least = min(least, joint[w]);
+    }
+    if (!std::is_same_v<T, _Float16>) return {top, -1};
+    int x;
+    frexpf(top, &x);
+    return {top, least == NONE ? 0 : least + x - 1};
 }
 template <class T>
 __global__ void __launch_bounds__(1024) xent_common_kernel(const float *dloss, const void *labels, int lab64, const int *row_exp, int rows, int V,
-                                                           int *common) {
-    const int c = common_exponent<T, 1024>(dloss, labels, lab64, row_exp, rows, V);
+                                                           Common *common) {
+    const Common c = common_weight<T, 1024>(dloss, labels, lab64, row_exp, rows, V);
     if (threadIdx.x == 0) *common = c;
 }
 
-// Hz[t, :] = 2^a H[t, :], zeros for tokens without a label and from D to ld.
-// FIND: the workgroups look for C themselves, for the kernels behind too (up to FIND_ROWS tokens; a launch less, about 3 us
+// Hz[t, :] = 2^a H[t, :] (one number: times m), zeros for tokens without a label and from D to ld.
+// FIND: the workgroups look for top and C themselves, for the kernels behind too (up to FIND_ROWS tokens; a launch less, about 3 us
 // of the host's time).
 constexpr int FIND_ROWS = 2048;
 template <class T, bool FIND>
 __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int64_t ldh, const void *labels, int lab64, const float *dloss,
-                                                                 const int *row_exp, int *common, int rows, int V, int D, T *Hz, int64_t ld,
-                                                                 int64_t chunks) {
+                                                                 const int *row_exp, Common *common, int numbers, int rows, int V, int D, T *Hz,
+                                                                 int64_t ld, int64_t chunks) {
     constexpr int CE = 16 / sizeof(T);
     typedef T chunk __attribute__((ext_vector_type(CE)));
     const int64_t per = ld / CE;
-    const int c0 = FIND ? common_exponent<T, 256>(dloss, labels, lab64, row_exp, rows, V) : *common;
+    const Common c0 = FIND ? common_weight<T, 256>(dloss, labels, lab64, row_exp, rows, V) : *common;
     if (FIND && blockIdx.x == 0 && threadIdx.x == 0) *common = c0;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
         const int t = (int)(i / per), c = (int)(i % per) * CE;
         const int64_t label = label_of(labels, lab64, t);
         chunk v;
         if (label >= 0 && label < V) {
-            const int a = token_weight<T>(dloss[t], row_exp, t, c0).a;
+            const TokenWeight w = token_weight<T>(dloss[t], row_exp, t, c0);
+            const float m = sizeof(T) == 2 && numbers == 1 ? w.m : 1.f;
             const T *s = H + t * ldh + c;
             if (c + CE <= D) {
                 v = *reinterpret_cast<const typename Chunk<T>::anywhere *>(s);
@@ -265,7 +291,7 @@ __global__ void __launch_bounds__(256) xent_weighted_rows_kernel(const T *H, int
                 for (int j = 0; j < CE; j++) v[j] = c + j < D ? s[j] : (T)0.f;
             }
 #pragma unroll
-            for (int j = 0; j < CE; j++) v[j] = (T)ldexpf((float)v[j], a);
+            for (int j = 0; j < CE; j++) v[j] = (T)ldexpf((float)v[j] * m, w.a);
         } else {
 #pragma unroll
             for (int j = 0; j < CE; j++) v[j] = (T)0.f;
@@ -284,7 +310,8 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
     n0 *= P::BN;
     pv4f acc[P::MT][P::NT];
     logits_tile<P>(g, m0, n0, smem, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, common = *g.common;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Common common = *g.common;
     const int n = n0 + (wave % P::WN) * P::TN + P::lane_column(lane);
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
@@ -292,7 +319,9 @@ __global__ void __launch_bounds__(P::THREADS) xent_probabilities_kernel(const Xe
         if (t >= g.T) continue;
         const int64_t label = label_of(g.labels, g.lab64, t);
         const bool valid = label >= 0 && label < g.V;
-        const float lse = g.lse[t], weight = valid ? token_weight<T>(g.dloss[t], g.row_exp, t, common).g : 0.f;
+        const float lse = g.lse[t];
+        const TokenWeight w = token_weight<T>(valid ? g.dloss[t] : 0.f, g.row_exp, t, common);
+        const float weight = ldexpf(sizeof(T) == 2 && g.numbers == 1 ? 1.f : w.m, w.b);
         const int64_t hot = label - g.v0;
 #pragma unroll
         for (int c = 0; c < P::LANE_N; c++) {
@@ -318,13 +347,13 @@ struct XentProductArgs {
     int64_t next;
     int a_cols, b_cols;                  // elements in a row of A (dW) and B, whole 16-byte chunks
     int row_tiles, col_tiles, xcds;
-    const int *common;                   // dW: C
+    const Common *common;                // dW
     int splits;                          // the reduction in this many parts, each (dW: if more than one) with a plane of floats
     int64_t plane;
     int add;                             // dH: add to the planes (a later piece of the vocabulary)
 };
 
-// dW[v0 + m, n] = 2^-C sum_t G[t, m] Hz[t, n], or one of several planes with the sums over part of the tokens
+// dW[v0 + m, n] = top 2^-C sum_t G[t, m] Hz[t, n], or one of several planes with the sums over part of the tokens
 template <class P, class O>
 __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -343,7 +372,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
         for (int i = 0; i < g.numbers; i++, a.p += g.next) product_run<P>(a, b, k, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = n0 + (wave % P::WN) * P::TN;
-    const int by = -*g.common;
+    const Common by = *g.common;
 #pragma unroll
     for (int i = 0; i < P::MT; i++) {
         const int m = m0 + (wave / P::WN) * P::TM + 16 * i + (lane & 15);
@@ -351,7 +380,7 @@ __global__ void __launch_bounds__(P::THREADS) xent_dw_kernel(const XentProductAr
 #pragma unroll
         for (int j = 0; j < P::NT; j++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) acc[i][j][c] = ldexpf(acc[i][j][c], by);
+            for (int c = 0; c < 4; c++) acc[i][j][c] = by.top * ldexpf(acc[i][j][c], -by.c);
         store_row<P, O>(g.out + (s * g.plane + m * g.ldo) * (int64_t)sizeof(O), n, g.cols, acc[i]);
     }
 }
@@ -388,10 +417,11 @@ __global__ void __launch_bounds__(P::THREADS) xent_dh_kernel(const XentProductAr
     }
 }
 
-// dH[t, n] = 2^(x - b) sum_s plane[s][t, n], zeros for tokens without a label.
+// dH[t, n] = top 2^(x - b) (one number: m) sum_s plane[s][t, n], zeros for tokens without a label.
 template <class T, class O>
 __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, int splits, int64_t plane, int64_t ld, const void *labels, int lab64,
-                                                           const float *dloss, const int *row_exp, const int *common, int V, int D, O *dH, int64_t ldo, int64_t chunks) {
+                                                           const float *dloss, const int *row_exp, const Common *common, int numbers, int V, int D, O *dH, int64_t ldo,
+                                                          int64_t chunks) {
     const int64_t per = ld / 4;
     typedef O quad __attribute__((ext_vector_type(4)));
     typedef O quad_anywhere __attribute__((ext_vector_type(4), aligned(sizeof(O))));
@@ -402,9 +432,10 @@ __global__ void __launch_bounds__(256) xent_dh_join_kernel(const float *planes, 
         if (label >= 0 && label < V) {
 #pragma unroll 4
             for (int s = 0; s < splits; s++) sum += *reinterpret_cast<const pv4f *>(planes + s * plane + t * ld + n);
-            const int u = token_weight<T>(dloss[t], row_exp, t, *common).u;
+            const TokenWeight w = token_weight<T>(dloss[t], row_exp, t, *common);
+            const float by = common->top * (sizeof(T) == 2 && numbers == 1 ? w.m : 1.f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) sum[j] = ldexpf(sum[j], u);
+            for (int j = 0; j < 4; j++) sum[j] = by * ldexpf(sum[j], w.u);
         }
         O *o = dH + t * ldo + n;
         if (n + 4 <= D) {
@@ -484,7 +515,7 @@ static XentRoom xent_room(bool backward, int numbers, int type, const void *H, c
         else piece = round_up((V + (V + piece - 1) / piece - 1) / ((V + piece - 1) / piece), 256);     // equal pieces
         r.piece = (int)piece;
         r.splits = dh_splits(T, D, r.piece, size, numbers);
-        r.common = take(sizeof(int));
+        r.common = take(sizeof(Common));
         r.row_exp = take(type == T2SP_TYPE_F16 ? (size_t)T * sizeof(int) : 0);
         r.hz = take((size_t)T * r.ldd * size);
         r.g = take((size_t)T * padded_cols(piece, size) * size * numbers);
@@ -570,7 +601,8 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
                          int64_t lddw, hipStream_t st) {
     constexpr int size = sizeof(T);
     float *planes = reinterpret_cast<float *>(room + r.planes);
-    int *common = reinterpret_cast<int *>(room + r.common), *row_exp = reinterpret_cast<int *>(room + r.row_exp);
+    Common *common = reinterpret_cast<Common *>(room + r.common);
+    int *row_exp = reinterpret_cast<int *>(room + r.row_exp);
     int err;
     g.common = common; g.row_exp = row_exp;
     if constexpr (std::is_same_v<T, _Float16>)
@@ -588,7 +620,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
     if (chunks) {
         auto kern = find ? xent_weighted_rows_kernel<T, true> : xent_weighted_rows_kernel<T, false>;
         hipLaunchKernelGGL(kern, dim3((unsigned)(chunks < 256 * 16384 ? (chunks + 255) / 256 : 16384)), dim3(256), 0, st,
-                           static_cast<const T *>(H), ldh, g.labels, g.lab64, g.dloss, row_exp, common, g.T, g.V, g.D,
+                           static_cast<const T *>(H), ldh, g.labels, g.lab64, g.dloss, row_exp, common, g.numbers, g.T, g.V, g.D,
                            reinterpret_cast<T *>(room + r.hz), r.ldd, chunks);
         if ((err = launched())) return err;
     }
@@ -640,7 +672,7 @@ static int xent_backward(XentArgs g, const XentRoom &r, char *room, const void *
     if (dH && g.T) {
         const int64_t quads = (int64_t)g.T * r.ldd / 4;
         hipLaunchKernelGGL((xent_dh_join_kernel<T, O>), dim3((unsigned)(quads < 256 * 16384 ? (quads + 255) / 256 : 16384)), dim3(256), 0, st, planes,
-                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, row_exp, common, g.V, g.D, static_cast<O *>(dH), lddh, quads);
+                           r.splits, (int64_t)g.T * r.ldd, r.ldd, g.labels, g.lab64, g.dloss, row_exp, common, g.numbers, g.V, g.D, static_cast<O *>(dH), lddh, quads);
         return launched();
     }
     return T2SP_OK;

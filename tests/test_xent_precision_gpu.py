@@ -215,3 +215,16 @@ def test_replayed_graphs_of_both_forms(dtype, rounded):
         torch.cuda.synchronize()
         for g, res in graphs:
             assert all(torch.equal(a, b) for a, b in zip(want, res))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rounded", [False, True])
+def test_equal_weights_change_no_bit(dtype, rounded):
+    """The gradients for weights of 1 / 7 are those for weights of 1, multiplied by float(1 / 7)."""
+    import torch
+    H, W, lab = quarters((70, 64), dtype, 1, 4), quarters((50, 64), dtype, 2, 1), labels_for(70, 50, 3)
+    _, lse = t2sp_amd.xent(H, W, lab)
+    one = torch.ones(70, device="cuda")
+    a = t2sp_amd.xent_grad(H, W, lab, lse, one, out_dtype=torch.float32, rounded=rounded)
+    b = t2sp_amd.xent_grad(H, W, lab, lse, one / 7, out_dtype=torch.float32, rounded=rounded)
+    assert torch.equal(a[0] * (one[0] / 7), b[0]) and torch.equal(a[1] * (one[0] / 7), b[1])
