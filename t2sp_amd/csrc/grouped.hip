@@ -169,8 +169,9 @@ __global__ void __launch_bounds__(P::THREADS) grouped_kernel(const GroupedArgs g
 // ------------------------------------------------------------------------------------------------ few rows per group
 // Decoding: a group has a handful of rows, and what takes time is reading its matrix once.  A workgroup owns up to 16 MT
 // rows of a group and a strip of columns; its eight waves take pieces of K in turn and are joined through LDS in a
-// fixed order.  The matrix goes from memory straight into MFMA operands, 8 or 16 loads of 16 bytes per lane in flight and two
-// or more workgroups per CU (a CU needs about 50 KB in flight to draw its share of HBM's rate):
+// fixed order.  The matrix goes from memory straight into MFMA operands, 8 or 16 loads of 16 bytes per lane in flight, 64 or 128
+// KB a workgroup (a CU needs about 50 KB in flight to draw its share of HBM's rate, and nothing is under way between two pieces).
+// Two workgroups share a CU with 16 or 32 rows (80 to 111 registers), one with 64 and for 16-bit KROWS (160 to 219):
 //   KMAJOR  32 columns; a lane's 16 bytes are k of its column, as the MFMA wants them; 256 bytes of a column per piece.
 //   KROWS   16 EPC columns (128 of 16 bits, 64 floats): lane l reads EPC columns of k rows EPC (l / 16) + 0 .. EPC - 1, a block
 //           that it transposes in its own registers (one v_perm per two elements; floats need none); accumulator tile j
@@ -491,10 +492,10 @@ static int launch_wgrad(GroupedArgs g, hipStream_t stream) {
 // E (1 - exp(-T / E)) groups have rows, and their ends make half a row tile more than whole tiles would.  The workgroups share
 // the CUs, n to a CU, and a stage of 64 bytes of k takes a + n (c + fill x the 16-row blocks that hold rows); `ends` stages go
 // into start and store.  Beside that stands the reading of the matrices at `rate` TB/s: the larger of the two and a quarter of
-// the smaller.  Fitted to 600 products of 16-bit elements a layout and 500 of floats (1 to 8192 rows in 1 to 64 groups of any sizes,
-// 64 to 4096 x 64 to 4096, matrices not in the caches).  Of those kept out of the fit, the form picked took 1 to 3 percent
-// more than the best of the six (geometric mean) and 6 to 16 at the 95th percentile; equally large groups and fewer
-// constants had cost 3 to 7 percent and 13 to 32.
+// the smaller.  Fitted to measured products of 1 to 8192 rows in 1 to 64 groups of any sizes, 64 to 4096 x 64 to 4096, matrices not in
+// the caches.  Over 60 other such products for each of bfloat16 and float in each layout, the form picked takes 2 to 5 percent more
+// than the best of the six (geometric mean) and 7 to 20 at the 95th percentile; the worst (1.7 to 2 times) are
+// mostly calls of 5 us with fewer rows than groups.
 struct GroupShape {
     int rows, cols;
     double a, c, fill;
