@@ -348,7 +348,7 @@ int t2sp_gemm_grouped_wgrad(int type, int out_type, const void *X, const void *d
  * (16-byte aligned, t2sp_xent*_workspace_bytes, required), as do padded copies of operands whose rows are not
  * whole 16-byte chunks.  16-bit types: p - [label] enters the products as the sum of two numbers of `type`, 16
  * (bfloat16) or 22 (half) bits of it, which leaves less than the float sums of z do.  t2sp_xent_grad_rounded is the
- * same call with p - [label] rounded to one number of `type`: a third to two fifths less time, and an error of half
+ * same call with p - [label] rounded to one number of `type`: a quarter to a third less time, and an error of half
  * a step of the type in every p - [label] (float: no difference).  Sums are in float and in a fixed order. */
 size_t t2sp_xent_workspace_bytes(int type, const void *H, const void *W, int T, int V, int D, int64_t ldh, int64_t ldw);
 int t2sp_xent(int type, const void *H, const void *W, const void *labels, int label_bits, float *loss, float *lse,

@@ -286,7 +286,7 @@ def xent_grad(H, W, labels, lse, dloss, dH=None, dW=None, out_dtype=None, wanted
     lse: what xent returned; dloss: T float32.  The results have H's type, or float32 (out_dtype, or the type of dH / dW).
     `wanted` leaves one out (its place in the result is None; numpy arrays: both are computed).
     16-bit types: g enters the products with 16 (bfloat16) or 22 (half) of a float's 24 bits, as the sum of two numbers of
-    the type.  rounded=True takes it rounded to one, for a third less time and an error of half a step of the type in every g
+    the type.  rounded=True takes it rounded to one, for up to a third less time and an error of half a step of the type in every g
     (tensors only).  float16: in dW, tokens whose weight |dloss| max |H[t]| is below 2^-30 of the heaviest's lose bits."""
     op = "xent_grad"
     if not _is_torch(H):
